@@ -29,8 +29,8 @@ NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", 
               "-Xcompiler", "-fPIC", "-Xcompiler", "-Wall", "--expt-relaxed-constexpr",
               "-diag-suppress", "177", "-diag-suppress", "550"]
 # sources compiled without --use_fast_math: their exponentials, tanh and divisions feed routers, norms and recurrences
-NO_FAST_MATH: set = {"attention_simt.cu", "channel_delta.cu", "gemm_f32.cu", "latent.cu", "lightning.cu", "lightning_tc5.cu", "mlstm.cu",
-                      "mlstm_tc5.cu", "moe.cu", "stream_norm.cu", "stream_post.cu", "stream_sandwich.cu"}
+NO_FAST_MATH: set = {"attention_fp4.cu", "attention_simt.cu", "channel_delta.cu", "gemm_f32.cu", "kv_evict.cu", "kv_fp4.cu", "latent.cu", "lightning.cu",
+                      "lightning_tc5.cu", "mlstm.cu", "mlstm_tc5.cu", "moe.cu", "stream_norm.cu", "stream_post.cu", "stream_sandwich.cu"}
 
 
 def _newer(src: str, dst: str, deps: List[str]) -> bool:

@@ -1,0 +1,217 @@
+// Four-bit (NVFP4) cache pages: what writes them and what expands them.  The page layout is in kv_fp4_common.cuh.
+//
+//   rope_kv_write_fp4  per-head RMS norm and rotation of a step's queries and keys, and the step's keys and values quantised into the pages:
+//                      a = max |r| over 16 features, s = e4m3(min(a / 6 / scale, 448)), code = e2m1(r / (s * scale)).  r is the 16-bit value
+//                      that a 16-bit cache would hold.  The products of the rotation are rounded one by one and the sum of squares is taken
+//                      in 64 bits, so that the codes, which jump at a border, are those of the formula and not of one order of additions.
+//   kv_fp4_stage       16-bit pages of the cached rows of a step's sequences, for the prompt kernels.
+#include <type_traits>
+
+#include "host_utils.h"
+#include "kv_fp4_common.cuh"
+
+namespace telb {
+
+struct Fp4WriteParams {
+    const void* qkv;
+    void* q_out;
+    uint8_t* pool;
+    const float* cos_sin;
+    const int *positions, *seq_ids, *q_start, *past_len, *page_table, *kv_offsets;
+    const void *q_norm, *k_norm;
+    const float* scales;
+    void* stage;
+    const int* stage_table;
+    int tokens, hq, hkv, rot, max_pos, page_size, max_pages, num_pages, stage_page, stage_max, stage_pages;
+    float eps;
+};
+
+// One warp per (token, head); a lane holds E neighbouring features.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) rope_kv_write_fp4_kernel(const Fp4WriteParams p) {
+    pdl_prologue();
+    constexpr int E = D / 32, kLanes = 16 / E;                 // lanes of a block of 16 features
+    const int heads = p.hq + 2 * p.hkv;
+    const long long wid = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
+    const int lane = threadIdx.x & 31;
+    if (wid >= (long long)p.tokens * heads) return;
+    const int t = (int)(wid / heads), h = (int)(wid - (long long)t * heads);
+    const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
+    alignas(16) T x[E];
+    {
+        const T* src = reinterpret_cast<const T*>(p.qkv) + ((size_t)t * heads + h) * D + lane * E;
+        if constexpr (E == 2) *reinterpret_cast<uint32_t*>(x) = *reinterpret_cast<const uint32_t*>(src);
+        else if constexpr (E == 4) *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(src);
+        else *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(src);
+    }
+    const T* nw = reinterpret_cast<const T*>(is_q ? p.q_norm : is_v ? nullptr : p.k_norm);
+    if (nw) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < E; ++i) ss += (double)Cvt<T>::to_f(x[i]) * (double)Cvt<T>::to_f(x[i]);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = (float)(1.0 / sqrt(ss / D + (double)p.eps));
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            x[i] = Cvt<T>::from_f(__fmul_rn(Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(Cvt<T>::to_f(x[i]), inv))), Cvt<T>::to_f(nw[lane * E + i])));
+    }
+    if (!is_v) {
+        // features i and i + rot / 2 turn together; rot is a multiple of 2 E, so the other one is at the same place of another lane
+        const int half = p.rot / 2, step = half / E, d0 = lane * E;
+        const bool turns = d0 < p.rot, low = d0 < half;
+        const int other = !turns ? lane : low ? lane + step : lane - step;
+        const float* cs = p.cos_sin + (size_t)min(max(p.positions[t], 0), p.max_pos - 1) * p.rot + (low ? d0 : d0 - half);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float a = Cvt<T>::to_f(x[i]);
+            const float b = __shfl_sync(0xffffffffu, a, other);
+            if (turns) {
+                const float c = cs[i], s = cs[half + i];
+                x[i] = Cvt<T>::from_f(low ? __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)) : __fadd_rn(__fmul_rn(a, c), __fmul_rn(b, s)));
+            }
+        }
+    }
+    auto put = [&](T* dst) {
+        if constexpr (E == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(x);
+        else if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(x);
+        else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
+    };
+    if (is_q) {
+        put(reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.hq + h) * D + lane * E);
+        return;
+    }
+    const int s = p.seq_ids[t];
+    const int slot = p.past_len[s] + (p.kv_offsets ? p.kv_offsets[t] : t - p.q_start[s]);
+    const int lp = slot / p.page_size, at = slot - lp * p.page_size;
+    const int page = lp < p.max_pages ? p.page_table[(size_t)s * p.max_pages + lp] : -1;
+    const int head = is_v ? h - p.hq - p.hkv : h - p.hq;
+    const float scale = p.scales[is_v];
+    // the largest magnitude of the block, compared as bit patterns so that a NaN stays one
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) m = max(m, __float_as_uint(Cvt<T>::to_f(x[i])) & 0x7fffffffu);
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float want = __fdiv_rn(__fdiv_rn(__uint_as_float(m), 6.f), scale);
+    want = want > 448.f ? 448.f : want;
+    const uint8_t sf = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
+    const float step = __fmul_rn(e4m3_to_float(sf), scale);
+    uint32_t codes = 0;
+    float back[E];
+#pragma unroll
+    for (int i = 0; i < E; i += 2) {
+        float y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const float v = Cvt<T>::to_f(x[i + j]);
+            y[j] = step > 0.f ? __fdiv_rn(v, step) : v != v ? 0.f : copysignf(0.f, v);
+        }
+        const uint32_t c = e2m1_pair(y[0], y[1]);
+        codes |= c << (4 * i);
+        uint32_t hb;
+        asm("{\n\t.reg .b8 b, z;\n\tmov.b16 {b, z}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, b;\n\t}" : "=r"(hb) : "h"((uint16_t)c));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hb));
+        back[i] = __fmul_rn(f.x, step);
+        back[i + 1] = __fmul_rn(f.y, step);
+    }
+    if ((unsigned)page < (unsigned)p.num_pages) {              // else: a row that has no page is not stored
+        uint8_t* slab = p.pool + (((size_t)page * 2 + is_v) * p.hkv + head) * fp4_slab_bytes(p.page_size, D);
+        uint8_t* row = slab + (size_t)at * (D / 2) + lane * (E / 2);
+        if constexpr (E == 2) *row = (uint8_t)codes;
+        else if constexpr (E == 4) *reinterpret_cast<uint16_t*>(row) = (uint16_t)codes;
+        else *reinterpret_cast<uint32_t*>(row) = codes;
+        if (lane % kLanes == 0) slab[(size_t)p.page_size * (D / 2) + (size_t)at * (D / 16) + lane / kLanes] = sf;
+    }
+    if (p.stage) {
+        const int sl = slot / p.stage_page;
+        const int sp = sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
+        if ((unsigned)sp >= (unsigned)p.stage_pages) return;
+#pragma unroll
+        for (int i = 0; i < E; ++i) x[i] = fp4_round<T>(back[i]);
+        put(reinterpret_cast<T*>(p.stage) + ((((size_t)sp * 2 + is_v) * p.hkv + head) * p.stage_page + slot - sl * p.stage_page) * D + lane * E);
+    }
+}
+
+// A CTA per page of the 16-bit copy (64 rows; sequence blockIdx.y, logical page blockIdx.x) and plane (K|V, head) blockIdx.z.  Rows from `count` on, up
+// to the page's end, become zero.
+template <typename T>
+__global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table, const int* __restrict__ past_len,
+                                                           const int* __restrict__ q_len, const int* __restrict__ page_table,
+                                                           const float* __restrict__ scales, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d,
+                                                           int window) {
+    pdl_prologue();
+    const int seq = blockIdx.y, lp = blockIdx.x, plane = blockIdx.z;
+    if (plane == 0 && threadIdx.x == 0) stage_table[seq * stage_pages + lp] = seq * stage_pages + lp;
+    const int past = past_len[seq];
+    const int count = past + (q_len ? q_len[seq] : 0);
+    if (window > 0 && (lp + 1) * 64 + 2 * 128 <= past - window) return;        // before every tile that the windowed kernels touch
+    const size_t slab = fp4_slab_bytes(page_size, d);
+    const float scale = scales[plane >= hkv];
+    T* dst = stage + (((size_t)seq * stage_pages + lp) * 2 * hkv + plane) * 64 * d;
+    for (int i = threadIdx.x; i < 64 * d / 8; i += blockDim.x) {
+        const int r = i / (d / 8), e = (i - r * (d / 8)) * 8, slot = lp * 64 + r;
+        alignas(16) T out[8];
+        int page = -1;
+        if (slot < count && slot / page_size < max_pages) page = page_table[(size_t)seq * max_pages + slot / page_size];
+        if ((unsigned)page >= (unsigned)num_pages) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) out[j] = Cvt<T>::from_f(0.f);
+        } else {
+            const uint8_t* src = pool + ((size_t)page * 2 * hkv + plane) * slab;
+            const int at = slot % page_size;
+            uint32_t h[4];
+            e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(src + (size_t)at * (d / 2) + e / 2), h[0], h[1], h[2], h[3]);
+            const float step = __fmul_rn(e4m3_to_float(src[(size_t)page_size * (d / 2) + (size_t)at * (d / 16) + e / 16]), scale);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+                out[2 * j] = fp4_round<T>(__fmul_rn(f.x, step));
+                out[2 * j + 1] = fp4_round<T>(__fmul_rn(f.y, step));
+            }
+        }
+        *reinterpret_cast<uint4*>(dst + (size_t)r * d + e) = *reinterpret_cast<const uint4*>(out);
+    }
+}
+
+}  // namespace telb
+
+using namespace telb;
+
+extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int is_bf16, cudaStream_t stream) {
+    const Fp4WriteParams& p = *params;
+    if (p.tokens <= 0) return 0;
+    if (d != 64 && d != 128 && d != 256) return fail("telb_rope_kv_write_fp4: head_dim must be 64, 128 or 256");
+    if (p.rot < 0 || p.rot > d || p.rot % (d / 16)) return fail("telb_rope_kv_write_fp4: the rotated part must be a multiple of head_dim / 16");
+    const long long warps = (long long)p.tokens * (p.hq + 2 * p.hkv);
+    const dim3 grid((unsigned)((warps + 7) / 8)), blk(256);
+#define WRITE_FP4(T, D) TELB_LAUNCH("rope_kv_write_fp4_kernel", (rope_kv_write_fp4_kernel<T, D>), grid, blk, 0, stream, p)
+    if (is_bf16) {
+        if (d == 128) WRITE_FP4(__nv_bfloat16, 128);
+        else if (d == 64) WRITE_FP4(__nv_bfloat16, 64);
+        else WRITE_FP4(__nv_bfloat16, 256);
+    } else {
+        if (d == 128) WRITE_FP4(__half, 128);
+        else if (d == 64) WRITE_FP4(__half, 64);
+        else WRITE_FP4(__half, 256);
+    }
+    return 0;
+}
+
+// pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [num_seqs * stage_pages, 2, Hkv, 64, d], page s * stage_pages + i for rows 64 i.. of sequence s.  `q_len` null: only the
+// rows that were cached before this step.
+extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table, const int* past_len, const int* q_len, const int* page_table, const float* scales,
+                                 int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d, int window, int is_bf16,
+                                 cudaStream_t stream) {
+    if (num_seqs <= 0 || stage_pages <= 0) return 0;
+    if (d % 16 || page_size % 16) return fail("telb_kv_fp4_stage: head_dim and page size must be multiples of 16");
+    if (num_seqs > 65535 || 2 * hkv > 65535) return fail("telb_kv_fp4_stage: more than 65535 sequences or planes");
+    const dim3 grid(stage_pages, num_seqs, 2 * hkv), blk(256);
+    if (is_bf16)
+        TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<__nv_bfloat16>), grid, blk, 0, stream, (const uint8_t*)pool, (__nv_bfloat16*)stage, stage_table, past_len,
+                    q_len, page_table, scales, max_pages, num_pages, page_size, stage_pages, hkv, d, window);
+    else
+        TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<__half>), grid, blk, 0, stream, (const uint8_t*)pool, (__half*)stage, stage_table, past_len, q_len,
+                    page_table, scales, max_pages, num_pages, page_size, stage_pages, hkv, d, window);
+    return 0;
+}

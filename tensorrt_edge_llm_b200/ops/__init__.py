@@ -380,6 +380,50 @@ def kv_fp8_commit(kv_layer, stage, meta, scales):
     return ref.kv_fp8_store(kv_layer, stage, meta, scales)
 
 
+def rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, num_q_heads, num_kv_heads, head_dim, scales, q_norm_w=None, k_norm_w=None, eps=1e-6,
+                      stage=None, stage_table=None):
+    """:func:`rope_kv_write` into four-bit (NVFP4) pages: returns ``q [T, Hq, D]``; keys and values are quantised as they are written.
+
+    ``kv_layer``: ``uint8 [pages, 2, Hkv, P, 9 D / 16]``, D 64, 128 or 256, P a multiple of 16.  The part of a page that holds one head's keys or
+    values has the codes ``[P, D / 2]`` (E2M1, even feature in the low nibble) in front and the block scales ``[P, D / 16]`` (E4M3, one per
+    16 features) behind them; a value is ``code * block scale * scales[0 keys, 1 values]`` (``scales`` fp32, on the device).  A block whose
+    features hold a NaN becomes NaN.  ``stage`` (16-bit pages ``[*, 2, Hkv, P', D]``) with ``stage_table`` ``[sequences, pages]``: the
+    rows as the cache now holds them are written there too.  Rows without a page (-1) are not stored."""
+    f = cuda_ops().rope_kv_write_fp4 if qkv.is_cuda else ref.rope_kv_write_fp4
+    return f(qkv, kv_layer, meta, cos_sin, num_q_heads, num_kv_heads, head_dim, scales, q_norm_w, k_norm_w, eps, stage, stage_table)
+
+
+def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
+    """16-bit copies of the rows that the step's sequences have in a four-bit layer, for the prompt kernels: ``(stage, meta)`` with the pages
+    ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  Rows cached before the step, with ``new_rows`` the step's own too; what
+    lies behind them in a page is zero.  ``window`` > 0: pages that no row of the step can see may be left out."""
+    f = cuda_ops().kv_fp4_stage if kv_layer.is_cuda else ref.kv_fp4_stage
+    return f(kv_layer, meta, scales, dtype, window, new_rows)
+
+
+def paged_attention_fp4(q, kv_layer, meta, scale, scales, sliding_window=None, sinks=None, weights=None, decay=1.0):
+    """:func:`paged_attention` over four-bit pages (see :func:`rope_kv_write_fp4`), which hold the step's rows already.  Steps of few rows read
+    them in place; longer ones, and tree masks, go through :func:`kv_fp4_stage`.  A row that sees no key gives zeros.
+
+    ``weights`` (fp32 ``[pages, Hkv, P]``, causal steps of at most 256 rows x heads of a KV head): every key that some row of the step sees
+    gets ``decay * weights + `` the sum of its softmax weights over those rows and the query heads of the KV head; the step's own keys
+    start from zero, other entries stay as they are."""
+    f = cuda_ops().paged_attention_fp4 if q.is_cuda else ref.paged_attention_fp4
+    return f(q, kv_layer, meta, scale, scales, sliding_window, sinks, weights, decay)
+
+
+def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep, first=0, recent=0):
+    """Shorten cached sequences to ``keep`` rows a KV head: the ``first`` ones, the ``recent`` ones and, of those between, the heaviest by
+    ``weights`` ``[pages, Hkv, P]`` (equal weights: the earlier row; NaN counts as the largest).
+
+    The rows of ``kv_layer`` ``[pages, 2, Hkv, P, *]`` (any cache type) and their weights are copied, in order, to the rows 0, 1, 2 .. of the
+    pages in ``to_table`` ``[sequences, ceil(keep / P)]``, which must be none of the pages in ``page_table`` ``[sequences, pages]``.
+    Returns which rows they were, int32 ``[sequences, Hkv, keep]``, -1 behind the last row of a sequence that had fewer than ``keep`` of its
+    ``lengths`` ``[sequences]``."""
+    f = cuda_ops().kv_evict if kv_layer.is_cuda else ref.kv_evict
+    return f(kv_layer, weights, page_table, lengths, to_table, keep, first, recent)
+
+
 def argmax(logits):
     if logits.is_cuda:
         return cuda_ops().argmax(logits)

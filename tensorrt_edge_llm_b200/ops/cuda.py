@@ -7,12 +7,15 @@ nothing in this module falls back to PyTorch on a GPU.
 from __future__ import annotations
 
 import ctypes
+import dataclasses
+import functools
 import os
 import threading
 from typing import Dict, Optional, Tuple
 
 import torch
 
+from . import reference as ref_ops
 from .meta import StepMeta
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_lib", "libtelb_kernels.so")
@@ -610,6 +613,184 @@ def paged_attention_decode_fp8(q8: torch.Tensor, kv_layer: torch.Tensor, meta: S
         c_ll(ws.attn_ws.numel()), c_int(1 if out_dtype == torch.bfloat16 else 0), _p(ws.status), _p(sinks), _stream()),
         "paged_attention_decode_fp8", 2 if splits > 1 else 1)
     return out if out_scale is None else QuantActs(xq, sf, (t, hq * d), out_dtype)
+
+
+# ---- four-bit (NVFP4) cache pages --------------------------------------------------------------
+
+
+def _on_device(fn):
+    """Run ``fn`` with the device of its first tensor argument as the current one (its launches go to that device's current stream)."""
+    @functools.wraps(fn)
+    def run(t, *args, **kw):
+        if not t.is_cuda:
+            raise ValueError(f"{fn.__name__}: a tensor on {t.device}, not on the GPU")
+        if t.device.index == torch.cuda.current_device():
+            return fn(t, *args, **kw)
+        with torch.cuda.device(t.device):
+            return fn(t, *args, **kw)
+    return run
+
+
+class Fp4WriteParams(ctypes.Structure):
+    """Host mirror of ``Fp4WriteParams`` (``csrc/kernels/kv_fp4.cu``)."""
+    _fields_ = [(n, c_vp) for n in ("qkv", "q_out", "pool", "cos_sin", "positions", "seq_ids", "q_start", "past_len", "page_table", "kv_offsets", "q_norm",
+                                    "k_norm", "scales", "stage", "stage_table")] + \
+               [(n, c_int) for n in ("tokens", "hq", "hkv", "rot", "max_pos", "page_size", "max_pages", "num_pages", "stage_page", "stage_max", "stage_pages")] + \
+               [("eps", c_float)]
+
+
+class Fp4AttnParams(ctypes.Structure):
+    """Host mirror of ``Fp4AttnParams`` (``csrc/kernels/attention_fp4.cu``)."""
+    _fields_ = [(n, c_vp) for n in ("q", "pool", "out", "part_o", "part_ml", "stat", "q_start", "q_len", "past_len", "page_table", "scales", "sinks", "weights")] + \
+               [(n, c_int) for n in ("num_seqs", "tokens", "max_q_len", "num_pages", "max_pages", "page_size", "hq", "hkv", "window", "splits")] + \
+               [("scale", c_float), ("decay", c_float)]
+
+
+class EvictParams(ctypes.Structure):
+    """Host mirror of ``EvictParams`` (``csrc/kernels/kv_evict.cu``)."""
+    _fields_ = [(n, c_vp) for n in ("pool", "weights", "page_table", "lengths", "to_table", "kept")] + \
+               [(n, c_int) for n in ("num_seqs", "hkv", "num_pages", "max_pages", "to_pages", "page_size", "row_bytes", "scale_bytes", "keep", "first", "recent")]
+
+
+def _fp4_geometry(kv_layer: torch.Tensor, meta: StepMeta, scales: torch.Tensor) -> int:
+    """Head size of a four-bit layer, after the checks that all its operators share."""
+    d = ref_ops.fp4_head_dim(kv_layer)
+    if not kv_layer.is_contiguous() or kv_layer.data_ptr() % 16:
+        raise ValueError("a four-bit layer must be contiguous and start on 16 bytes")
+    if kv_layer.shape[3] != meta.page_size:
+        raise ValueError(f"a layer of {kv_layer.shape[3]}-row pages in a step of {meta.page_size}-row pages")
+    if scales.dtype != torch.float32 or scales.numel() != 2 or not scales.is_contiguous():
+        raise ValueError("scales: two contiguous fp32 numbers, of the keys and of the values")
+    return d
+
+
+@_on_device
+def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads: int, num_kv_heads: int, head_dim: int, scales, q_norm_w=None, k_norm_w=None,
+                      eps: float = 1e-6, stage=None, stage_table=None) -> torch.Tensor:
+    """See :func:`ops.rope_kv_write_fp4`."""
+    d = _fp4_geometry(kv_layer, meta, scales)
+    is_bf16 = _is_bf16(qkv)
+    t = qkv.shape[0]
+    if d != head_dim or kv_layer.shape[2] != num_kv_heads or qkv.shape != (t, (num_q_heads + 2 * num_kv_heads) * d) or t != meta.num_tokens:
+        raise ValueError(f"rope_kv_write_fp4: rows {tuple(qkv.shape)} of {num_q_heads} + 2 x {num_kv_heads} heads of {head_dim}, a layer of {kv_layer.shape[2]} heads of {d}")
+    positions = meta.positions
+    if meta.rope_rows is not None:          # multimodal RoPE: per-row cos / sin tables prepared by the model
+        cos_sin, positions = meta.rope_rows, meta.rope_pos
+    rot = cos_sin.shape[-1]
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or rot > d or rot % (d // 16):
+        raise ValueError(f"rope_kv_write_fp4: a contiguous fp32 cos | sin table of at most {d} columns, a multiple of {d // 16}")
+    for w in (q_norm_w, k_norm_w):
+        if w is not None and (w.dtype != qkv.dtype or w.numel() != d or not w.is_contiguous()):
+            raise ValueError(f"rope_kv_write_fp4: norm weights of {d} numbers in the type of the rows")
+    if (stage is None) != (stage_table is None):
+        raise ValueError("rope_kv_write_fp4: 16-bit pages come with their page table")
+    if stage is not None:
+        if stage.dtype != qkv.dtype or not stage.is_contiguous() or stage.shape[1:3] != (2, num_kv_heads) or stage.shape[4] != d:
+            raise ValueError(f"rope_kv_write_fp4: 16-bit pages {tuple(stage.shape)} {stage.dtype} for rows of {qkv.dtype}, {num_kv_heads} heads of {d}")
+        if stage_table.dtype != torch.int32 or not stage_table.is_contiguous() or stage_table.shape[0] != meta.num_seqs:
+            raise ValueError("rope_kv_write_fp4: the 16-bit pages' table is int32 [sequences, pages]")
+    qkv = _aligned(qkv)
+    q = torch.empty(t, num_q_heads, d, dtype=qkv.dtype, device=qkv.device)
+    ptr = lambda v: None if v is None else _p(v).value
+    p = Fp4WriteParams(*[ptr(v) for v in (qkv, q, kv_layer, cos_sin, positions, meta.seq_ids, meta.q_start, meta.past_len, meta.page_table, meta.kv_offsets,
+                                          q_norm_w, k_norm_w, scales, stage, stage_table)],
+                       t, num_q_heads, num_kv_heads, rot, cos_sin.shape[0], meta.page_size, meta.page_table.shape[1], kv_layer.shape[0],
+                       1 if stage is None else stage.shape[3], 0 if stage is None else stage_table.shape[1], 0 if stage is None else stage.shape[0], eps)
+    _check(lib().telb_rope_kv_write_fp4(ctypes.byref(p), c_int(d), c_int(is_bf16), _stream()), "rope_kv_write_fp4")
+    return q
+
+
+@_on_device
+def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int = 0, new_rows: bool = False):
+    """See :func:`ops.kv_fp4_stage`."""
+    d = _fp4_geometry(kv_layer, meta, scales)
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"kv_fp4_stage: pages of fp16 or bf16, not {dtype}")
+    hkv, n = kv_layer.shape[2], meta.num_seqs
+    per = max(1, (meta.max_seq_len + 63) // 64)
+    stage = torch.empty(n * per, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
+    table = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device)
+    _check(lib().telb_kv_fp4_stage(_p(kv_layer), _p(stage), _p(table), _p(meta.past_len), _p(meta.q_len if new_rows else None), _p(meta.page_table), _p(scales), c_int(n),
+                                   c_int(meta.page_table.shape[1]), c_int(kv_layer.shape[0]), c_int(meta.page_size), c_int(per), c_int(hkv), c_int(d),
+                                   c_int(window or 0), c_int(int(dtype == torch.bfloat16)), _stream()), "kv_fp4_stage")
+    return stage, dataclasses.replace(meta, page_table=table, page_size=64)
+
+
+FP4_DIRECT_COLUMNS = 64      # rows x heads of a KV head up to which a step reads four-bit pages in place
+FP4_WEIGHT_COLUMNS = 256     # and up to which it keeps account of the attention weights
+
+
+def _fp4_splits(items: int, keys: int) -> int:
+    return max(1, min(4 * 148 // max(1, items), (keys + 127) // 128, 64))
+
+
+@_on_device
+def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, sliding_window=None, sinks=None, weights=None, decay: float = 1.0,
+                        direct: Optional[bool] = None, splits: Optional[int] = None) -> torch.Tensor:
+    """See :func:`ops.paged_attention_fp4`.  ``direct`` forces the kernel that reads the pages in place (True), or the expansion to 16 bits and
+    the prompt kernels (False); ``splits``: parts of a sequence's keys."""
+    d = _fp4_geometry(kv_layer, meta, scales)
+    is_bf16 = _is_bf16(q)
+    t, hq = q.shape[:2]
+    hkv = kv_layer.shape[2]
+    if q.dim() != 3 or q.shape[2] != d or hq % hkv or t != meta.num_tokens:
+        raise ValueError(f"paged_attention_fp4: queries {tuple(q.shape)} over {hkv} heads of {d}, {meta.num_tokens} rows")
+    if not scale > 0:
+        raise ValueError("paged_attention_fp4: the score scale must be positive")
+    window = sliding_window if sliding_window and sliding_window > 0 else 0
+    columns = meta.max_q_len * (hq // hkv)
+    if weights is not None:
+        if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (kv_layer.shape[0], hkv, meta.page_size):
+            raise ValueError(f"paged_attention_fp4: weights are contiguous fp32 {(kv_layer.shape[0], hkv, meta.page_size)}")
+        if meta.tree_mask is not None or columns > FP4_WEIGHT_COLUMNS:
+            raise ValueError(f"paged_attention_fp4: weights are kept for causal steps of at most {FP4_WEIGHT_COLUMNS} rows x heads of a KV head, not {columns}")
+        if direct is False:
+            raise ValueError("paged_attention_fp4: weights come from the kernel that reads the pages in place")
+    if sinks is not None:
+        if sinks.numel() != hq:
+            raise ValueError(f"paged_attention_fp4: {sinks.numel()} sinks for {hq} heads")
+        sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
+    if direct is None:
+        direct = weights is not None or (meta.tree_mask is None and columns <= FP4_DIRECT_COLUMNS)
+    if not direct or meta.tree_mask is not None:
+        if direct:
+            raise ValueError("paged_attention_fp4: tree masks are read by the prompt kernels only")
+        stage, staged = kv_fp4_stage(kv_layer, meta, scales, q.dtype, window, True)
+        return paged_attention(q, stage, staged, scale, sliding_window, sinks)
+    q = _aligned(q)
+    out = torch.empty_like(q)
+    if splits is None:
+        splits = _fp4_splits(meta.num_seqs * hkv * ((columns + 15) // 16), min(meta.max_seq_len, window + meta.max_q_len) if window else meta.max_seq_len)
+    part_o = part_ml = stat = None
+    if splits > 1:
+        part_o = torch.empty(t * hq * splits, d, dtype=torch.float32, device=q.device)
+        part_ml = torch.empty(t * hq * splits, 2, dtype=torch.float32, device=q.device)
+    if weights is not None:
+        stat = torch.empty(t * hq, 2, dtype=torch.float32, device=q.device)
+    ptr = lambda v: None if v is None else _p(v).value
+    p = Fp4AttnParams(*[ptr(v) for v in (q, kv_layer, out, part_o, part_ml, stat, meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
+                      meta.num_seqs, t, meta.max_q_len, kv_layer.shape[0], meta.page_table.shape[1], meta.page_size, hq, hkv, window, splits, scale, decay)
+    _check(lib().telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(splits), c_int(is_bf16), _stream()), "paged_attention_fp4",
+           1 + (splits > 1) + (weights is not None))
+    return out
+
+
+@_on_device
+def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep: int, first: int = 0, recent: int = 0) -> torch.Tensor:
+    """See :func:`ops.kv_evict`."""
+    row, sf = ref_ops.evict_geometry(kv_layer, weights, page_table, lengths, to_table, keep, first, recent)
+    if not (kv_layer.is_contiguous() and weights.is_contiguous()) or kv_layer.data_ptr() % 16 or row % 16 or sf % 4:
+        raise ValueError("kv_evict: a contiguous layer that starts on 16 bytes, rows of a multiple of 16 bytes, contiguous weights")
+    if any(v.device != kv_layer.device for v in (weights, page_table, lengths, to_table)):
+        raise ValueError("kv_evict: all tensors on one device")
+    pages, _, hkv, psz = kv_layer.shape[:4]
+    n = page_table.shape[0]
+    kept = torch.empty(n, hkv, keep, dtype=torch.int32, device=kv_layer.device)
+    page_table, lengths, to_table = (v.to(torch.int32).contiguous() for v in (page_table, lengths, to_table))
+    p = EvictParams(*[_p(v).value for v in (kv_layer, weights, page_table, lengths, to_table, kept)], n, hkv, pages, page_table.shape[1], to_table.shape[1],
+                    psz, row, sf, keep, first, recent)
+    _check(lib().telb_kv_evict(ctypes.byref(p), _stream()), "kv_evict", 2)
+    return kept
 
 
 def _visible_len(meta: StepMeta, chunk: int, window: int = 0) -> int:

@@ -13,6 +13,7 @@ GQA attention (``unittests/support/references.h:29-65``), NVFP4 math
 """
 from __future__ import annotations
 
+import dataclasses
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -1344,6 +1345,202 @@ def kv_fp8_store(kv_layer: torch.Tensor, stage: torch.Tensor, meta, scales: torc
         q = (rows / sc).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
         kv_layer[page, :, :, slot % psz] = q
         stage[page, :, :, slot % psz] = (q.float() * sc).to(stage.dtype)
+
+
+# ------------------------------------------------------------------------------------------
+# Four-bit (NVFP4) cache pages: host formulation of csrc/kernels/{kv_fp4,attention_fp4,kv_evict}.cu
+
+
+def fp4_head_dim(kv_layer: torch.Tensor) -> int:
+    """Head size of a four-bit layer ``uint8 [pages, 2, Hkv, P, 9 D / 16]``."""
+    if kv_layer.dtype != torch.uint8 or kv_layer.dim() != 5 or kv_layer.shape[1] != 2 or kv_layer.shape[4] not in (36, 72, 144):
+        raise ValueError(f"a four-bit layer is uint8 [pages, 2, heads, rows, 9 D / 16] with heads of 64, 128 or 256, not {kv_layer.dtype} {tuple(kv_layer.shape)}")
+    if kv_layer.shape[3] % 16 or kv_layer.shape[3] == 0:
+        raise ValueError("four-bit pages hold a multiple of 16 rows")
+    return kv_layer.shape[4] * 16 // 9
+
+
+def fp4_page_parts(kv_layer: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Views of a four-bit layer: codes ``[pages, 2, Hkv, P, D / 2]`` and block scales (E4M3 bytes) ``[pages, 2, Hkv, P, D / 16]``."""
+    d = fp4_head_dim(kv_layer)
+    n, two, hkv, p, _ = kv_layer.shape
+    flat = kv_layer.view(n, two, hkv, p * (d // 2 + d // 16))
+    return flat[..., :p * d // 2].unflatten(-1, (p, d // 2)), flat[..., p * d // 2:].unflatten(-1, (p, d // 16))
+
+
+def fp4_encode_rows(x: torch.Tensor, scale: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(packed codes, block scale bytes, values)`` of fp32 rows ``[..., D]`` with the global scale ``scale``."""
+    b = x.unflatten(-1, (-1, 16))
+    sf = (b.abs().amax(-1) / FP4_MAX / scale).clamp(max=E4M3_MAX).to(torch.float8_e4m3fn)
+    step = (sf.float() * scale)[..., None]
+    codes = fp4_encode(torch.where(step > 0, b / step, torch.copysign(torch.zeros_like(b), b.nan_to_num(0.0))))
+    values = (_e2m1_table(x.device)[codes.long()] * step).flatten(-2)
+    return fp4_pack(codes.flatten(-2)), sf.view(torch.uint8), values
+
+
+def _fp4_rows(kv_layer: torch.Tensor, table_row: torch.Tensor, rows: int, scales: torch.Tensor) -> torch.Tensor:
+    """fp32 keys and values ``[2, Hkv, rows, D]`` of one sequence; rows without a page are zero."""
+    codes, sf = fp4_page_parts(kv_layer)
+    p = kv_layer.shape[3]
+    slot = torch.arange(rows, device=kv_layer.device)
+    page = torch.full_like(slot, -1)
+    inside = slot // p < table_row.numel()
+    page[inside] = table_row.long()[slot[inside] // p]
+    there = (page >= 0) & (page < kv_layer.shape[0])
+    page = torch.where(there, page, torch.zeros_like(page))
+    step = sf[page, :, :, slot % p].view(torch.float8_e4m3fn).float() * scales.float().view(1, 2, 1, 1)
+    vals = _e2m1_table(kv_layer.device)[fp4_unpack(codes[page, :, :, slot % p]).long()].unflatten(-1, (-1, 16)) * step[..., None]
+    return torch.where(there[:, None, None, None], vals.flatten(-2), torch.zeros(())).permute(1, 2, 0, 3)
+
+
+def _fp4_round(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    if dtype == torch.float16:          # stops at its largest number
+        x = torch.where(x.abs() < float("inf"), x.clamp(-65504.0, 65504.0), x)
+    return x.to(dtype)
+
+
+def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads, num_kv_heads, head_dim, scales, q_norm_w=None, k_norm_w=None, eps=1e-6,
+                      stage=None, stage_table=None):
+    d, t = fp4_head_dim(kv_layer), qkv.shape[0]
+    if d != head_dim or kv_layer.shape[2] != num_kv_heads:
+        raise ValueError(f"rope_kv_write_fp4: {num_kv_heads} heads of {head_dim}, a layer of {kv_layer.shape[2]} heads of {d}")
+    if (stage is None) != (stage_table is None):
+        raise ValueError("rope_kv_write_fp4: 16-bit pages come with their page table")
+    q, k, v = qkv.view(t, -1, d).split([num_q_heads, num_kv_heads, num_kv_heads], dim=1)
+    pos = meta.positions
+    if meta.rope_rows is not None:
+        cos_sin, pos = meta.rope_rows, meta.rope_pos
+
+    def turn(x, w):
+        if w is not None:               # the mean square in 64 bits: codes jump at a border
+            inv = (1.0 / torch.sqrt(x.double().square().mean(-1, keepdim=True) + eps)).float()
+            x = ((x.float() * inv).to(x.dtype).float() * w.float()).to(x.dtype)
+        return apply_rope(x, pos, cos_sin)
+
+    q, k = turn(q, q_norm_w), turn(k, k_norm_w)
+    codes, sf, values = fp4_encode_rows(torch.stack([k, v], dim=1).float(), scales.float().view(2, 1, 1))
+    cv, sv = fp4_page_parts(kv_layer)
+    sid = meta.seq_ids.long()
+    slot = meta.past_len.long()[sid] + (meta.kv_offsets.long() if meta.kv_offsets is not None else torch.arange(t, device=qkv.device) - meta.q_start.long()[sid])
+    for parts, table, p, pages in (((cv, codes), (sv, sf)), meta.page_table, meta.page_size, kv_layer.shape[0]), (((stage, _fp4_round(values, qkv.dtype)),), stage_table, 0, 0):
+        if table is None:
+            continue
+        p, pages = p or stage.shape[3], pages or stage.shape[0]
+        lp = slot // p
+        page = torch.where(lp < table.shape[1], table.long()[sid, lp.clamp(max=table.shape[1] - 1)], torch.full_like(lp, -1))
+        ok = (page >= 0) & (page < pages)
+        for dst, src in parts:
+            dst[page[ok], :, :, slot[ok] % p] = src[ok]
+    return q
+
+
+def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype, window=0, new_rows=False):
+    d = fp4_head_dim(kv_layer)
+    n, per = meta.num_seqs, max(1, (meta.max_seq_len + 63) // 64)
+    stage = torch.zeros(n * per, 2, kv_layer.shape[2], 64, d, dtype=dtype, device=kv_layer.device)
+    table = torch.arange(n * per, dtype=torch.int32, device=kv_layer.device).view(n, per)
+    for s in range(n):
+        rows = int(meta.past_len[s]) + (int(meta.q_len[s]) if new_rows else 0)
+        v = _fp4_round(_fp4_rows(kv_layer, meta.page_table[s], rows, scales), dtype)
+        v = F.pad(v, (0, 0, 0, per * 64 - rows)).unflatten(2, (per, 64))
+        stage[s * per:(s + 1) * per] = v.permute(2, 0, 1, 3, 4)
+    return stage, dataclasses.replace(meta, page_table=table, page_size=64)
+
+
+def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale, scales, sliding_window=None, sinks=None, weights=None, decay=1.0):
+    t, hq, d = q.shape
+    hkv, p = kv_layer.shape[2], kv_layer.shape[3]
+    if d != fp4_head_dim(kv_layer) or hq % hkv:
+        raise ValueError(f"paged_attention_fp4: queries {tuple(q.shape)} over {hkv} heads of {fp4_head_dim(kv_layer)}")
+    if not scale > 0:
+        raise ValueError("paged_attention_fp4: the score scale must be positive")
+    g = hq // hkv
+    if weights is not None and (meta.tree_mask is not None or meta.max_q_len * g > 256):
+        raise ValueError("paged_attention_fp4: weights are kept for causal steps of at most 256 rows x heads of a KV head")
+    if meta.tree_mask is not None:
+        stage, staged = kv_fp4_stage(kv_layer, meta, scales, q.dtype, 0, True)
+        return paged_attention(q, stage, staged, scale, sliding_window, sinks)
+    window = sliding_window if sliding_window and sliding_window > 0 else 0
+    out = torch.empty_like(q)
+    for s in range(meta.num_seqs):
+        r0, ql, past = int(meta.q_start[s]), int(meta.q_len[s]), int(meta.past_len[s])
+        total = past + ql
+        if ql == 0:
+            continue
+        kv = _fp4_rows(kv_layer, meta.page_table[s], total, scales)
+        cols, rows = torch.arange(total, device=q.device), past + torch.arange(ql, device=q.device)[:, None]
+        page = F.pad(meta.page_table[s].long(), (0, (total + p - 1) // p), value=-1)[cols // p]
+        there = (page >= 0) & (page < kv_layer.shape[0])
+        seen = (cols <= rows) & there
+        if window:
+            seen = seen & (cols > rows - window)
+        sc = (q[r0:r0 + ql].float().view(ql, hkv, g, d).permute(1, 2, 0, 3) @ kv[0].transpose(-1, -2)[:, None]) * scale
+        sc = sc.masked_fill(~seen, float("-inf"))
+        if sinks is not None:
+            sc = torch.cat([sc, sinks.float().view(hkv, g, 1, 1).expand(hkv, g, ql, 1)], dim=-1)
+        elif not bool(seen.any(-1).all()):
+            sc = torch.where(seen.any(-1)[:, None], sc, torch.zeros(()))
+        pr = torch.softmax(sc, dim=-1)[..., :total].masked_fill(~seen, 0.0)
+        v = torch.where(seen.any(0)[:, None], kv[1], torch.zeros(()))
+        out[r0:r0 + ql] = (pr @ v[:, None]).permute(2, 0, 1, 3).reshape(ql, hq, d).to(q.dtype)
+        if weights is not None:
+            live = seen.any(0)
+            pg, at = page[live], cols[live] % p
+            old = torch.where((cols[live] < past)[:, None], weights[pg, :, at] * decay, torch.zeros(()))
+            weights[pg, :, at] = old + pr.sum((1, 2)).t()[live]
+    return out
+
+
+def evict_geometry(kv_layer, weights, page_table, lengths, to_table, keep: int, first: int, recent: int) -> Tuple[int, int]:
+    """``(bytes of a row, bytes of its block scales)`` of a cache layer of any type, after the checks of :func:`kv_evict`."""
+    if kv_layer.dim() != 5 or kv_layer.shape[1] != 2:
+        raise ValueError(f"kv_evict: a layer [pages, 2, heads, rows, *], not {tuple(kv_layer.shape)}")
+    pages, _, hkv, p, width = kv_layer.shape
+    if weights.dtype != torch.float32 or weights.shape != (pages, hkv, p):
+        raise ValueError(f"kv_evict: weights are fp32 {(pages, hkv, p)}")
+    n = page_table.shape[0]
+    if page_table.dim() != 2 or lengths.shape != (n,) or to_table.dim() != 2 or to_table.shape[0] != n:
+        raise ValueError("kv_evict: page tables [sequences, pages] and lengths [sequences]")
+    if keep < 1 or first < 0 or recent < 0 or first + recent > keep:
+        raise ValueError(f"kv_evict: {first} first and {recent} recent rows of {keep}")
+    if to_table.shape[1] * p < keep:
+        raise ValueError(f"kv_evict: {to_table.shape[1]} pages of {p} rows for {keep}")
+    if kv_layer.dtype == torch.uint8:
+        d = fp4_head_dim(kv_layer)
+        return d // 2, d // 16
+    return width * kv_layer.element_size(), 0
+
+
+def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep, first=0, recent=0):
+    _, sf = evict_geometry(kv_layer, weights, page_table, lengths, to_table, keep, first, recent)
+    parts = [v.view(torch.uint8) for v in fp4_page_parts(kv_layer)] if sf else [kv_layer.view(torch.uint8)]
+    pages, _, hkv, p = kv_layer.shape[:4]
+    n = page_table.shape[0]
+    kept = torch.full((n, hkv, keep), -1, dtype=torch.int32, device=kv_layer.device)
+    for s in range(n):
+        total = min(max(int(lengths[s]), 0), page_table.shape[1] * p)
+        slot = torch.arange(total, device=kv_layer.device)
+        page = page_table[s].long()[slot // p]
+        there = (page >= 0) & (page < pages)
+        for h in range(hkv):
+            pick = slot
+            if total > keep:
+                mid = slot[first:total - recent]
+                w = weights[page.clamp(0, pages - 1), h, slot % p][first:total - recent]
+                w = torch.where(w.isnan(), torch.full_like(w, float("inf")), w)
+                rank = torch.where(there[mid], 0, 2) - weights[page.clamp(0, pages - 1), h, slot % p][mid].isnan().int()     # NaN, numbers, no page
+                order = torch.sort(-w, stable=True).indices
+                order = order[torch.sort(rank[order], stable=True).indices][:keep - first - recent]
+                pick = torch.cat([slot[:first], mid[order].sort().values, slot[total - recent:]])
+            kept[s, h, :pick.numel()] = pick.int()
+            j = torch.arange(pick.numel(), device=kv_layer.device)
+            to = to_table[s].long()[j // p]
+            ok = there[pick] & (to >= 0) & (to < pages)
+            src, dst, at, j = page[pick][ok], to[ok], (pick % p)[ok], (j % p)[ok]
+            for part in parts:
+                part[dst, :, h, j] = part[src, :, h, at]
+            weights[dst, h, j] = weights[src, h, at]
+    return kept
 
 
 # ---- block-draft verification trees ---------------------------------------------------------------------------------
