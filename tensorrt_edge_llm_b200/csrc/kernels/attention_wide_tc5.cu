@@ -34,6 +34,7 @@ struct AttnWideParams {
     int splits, total_tokens, num_seqs;
     int window;                // sliding window, 0 = none, -1 = every row sees every cached and new token
     float scale_log2;          // softmax scale * log2(e), positive
+    const float* kv_scales;    // [2], of the scaled form: factors of the keys and of the values
     int* status;
 };
 
@@ -83,7 +84,7 @@ __device__ __forceinline__ bool wide_find_block(const int* __restrict__ q_len, i
     return false;
 }
 
-template <typename T>
+template <typename T, bool kScaled>
 __global__ void __launch_bounds__(kWideThreads, 1)
 attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constant__ CUtensorMap tma_kv, AttnWideParams p) {
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
@@ -255,6 +256,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
         const int* mask_row = p.tree_mask ? p.tree_mask + (size_t)(qrow0 + min(qi, qlen - 1)) * p.mask_words : nullptr;
         const int last_vis = p.window < 0 ? past + qlen - 1 : past + min(qi, qlen - 1);       // last visible cache slot (no tree mask)
         const int first_vis = p.window > 0 ? past + qi - p.window + 1 : 0;
+        const float scale_log2 = kScaled ? p.scale_log2 * p.kv_scales[0] : p.scale_log2;
         float m_used = -INFINITY, l_sum = 0.f;
         bool ok = true;
         for (int j = 0; j < ntiles; ++j) {
@@ -310,7 +312,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
                 for (int i = 1; i < 31; i += 2) mx[c] = fmaxf(fmaxf(mx[c], __uint_as_float(s[c][i])), __uint_as_float(s[c][i + 1]));
                 mx[c] = fmaxf(mx[c], __uint_as_float(s[c][31]));
             }
-            const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);
+            const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2);
             if (j == 0) {
                 m_used = m_new;
             } else {
@@ -334,7 +336,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
                 }
             }
             const float mref = m_used == -INFINITY ? 0.f : m_used;
-            const float2 sc = make_float2(p.scale_log2, p.scale_log2), mm = make_float2(-mref, -mref);
+            const float2 sc = make_float2(scale_log2, scale_log2), mm = make_float2(-mref, -mref);
             float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -361,7 +363,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
             tc_fence_after_sync();
             const size_t tok = (size_t)qrow0 + qi;
             const int head = kvh * p.group + g;
-            const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+            const float inv = (l_sum > 0.f ? 1.f / l_sum : 0.f) * (kScaled ? p.kv_scales[1] : 1.f);
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 float v[32];
@@ -410,17 +412,17 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
     }
 }
 
-template <typename T>
+template <typename T, bool kScaled>
 static int launch_wide(const CUtensorMap& tq, const CUtensorMap& tkv, const AttnWideParams& p, cudaStream_t stream) {
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attn_wide_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
+        cudaError_t e = cudaFuncSetAttribute(attn_wide_kernel<T, kScaled>, cudaFuncAttributeMaxDynamicSharedMemorySize, kWideSmem);
         if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attn_wide)", e);
         configured = true;
     }
     // no more blocks than whole ones and one remainder per sequence
     const long long blocks = p.total_tokens / (2 * p.tq) + p.num_seqs;
-    TELB_LAUNCH("attn_wide_kernel", (attn_wide_kernel<T>), dim3((unsigned)(blocks * p.hkv * p.splits)), dim3(kWideThreads), kWideSmem, stream, tq, tkv, p);
+    TELB_LAUNCH("attn_wide_kernel", (attn_wide_kernel<T, kScaled>), dim3((unsigned)(blocks * p.hkv * p.splits)), dim3(kWideThreads), kWideSmem, stream, tq, tkv, p);
     TELB_CHECK_LAUNCH("attn_wide_kernel");
     return 0;
 }
@@ -436,7 +438,8 @@ extern "C" int telb_attn_combine_dense(const float* ws_o, const float* ws_lse, v
 extern "C" int telb_paged_attention_wide(const void* q, const void* kv_layer, void* out, const int* q_start, const int* q_len,
                                          const int* past_len, const int* page_table, const int* tree_mask, int mask_words, int num_seqs,
                                          int total_tokens, int num_pages, int max_pages, int page_size, int hq, int hkv, float scale,
-                                         int window, int splits, float* ws, long long ws_floats, int is_bf16, int* status, cudaStream_t stream) {
+                                         int window, int splits, float* ws, long long ws_floats, int is_bf16, int* status, const float* kv_scales,
+                                         cudaStream_t stream) {
     AttnWideParams p{};
     p.out = out;
     p.q_start = q_start;
@@ -455,6 +458,7 @@ extern "C" int telb_paged_attention_wide(const void* q, const void* kv_layer, vo
     p.num_seqs = num_seqs;
     p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
+    p.kv_scales = kv_scales;
     p.status = status;
     if (splits < 1) splits = 1;
     while (splits > 1 && (long long)splits * total_tokens * hq * 129 > ws_floats) --splits;
@@ -468,7 +472,9 @@ extern "C" int telb_paged_attention_wide(const void* q, const void* kv_layer, vo
     const uint32_t box[3] = {64, (uint32_t)p.group, (uint32_t)p.tq};
     if (make_tmap_nd(&tq, dt, 3, q, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return -1;
     if (make_tmap_2d(&tkv, dt, 2, kv_layer, (uint64_t)num_pages * 2 * hkv * page_size, 128, 256, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B)) return -1;
-    const int rc = is_bf16 ? launch_wide<__nv_bfloat16>(tq, tkv, p, stream) : launch_wide<__half>(tq, tkv, p, stream);
+    // the form with scales is a kernel of its own: the plain one has no register to spare
+    const int rc = kv_scales ? (is_bf16 ? launch_wide<__nv_bfloat16, true>(tq, tkv, p, stream) : launch_wide<__half, true>(tq, tkv, p, stream))
+                             : (is_bf16 ? launch_wide<__nv_bfloat16, false>(tq, tkv, p, stream) : launch_wide<__half, false>(tq, tkv, p, stream));
     if (rc || splits == 1) return rc;
     return telb_attn_combine_dense(p.ws_o, p.ws_lse, out, total_tokens * hq, splits, 128, is_bf16, stream);
 }

@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __rest
     const int count = past + (q_len ? q_len[seq] : 0);
     if (window > 0 && (lp + 1) * 64 + 2 * 128 <= past - window) return;        // before every tile that the windowed kernels touch
     const size_t slab = fp4_slab_bytes(page_size, d);
-    const float scale = scales[plane >= hkv];
+    const float scale = scales ? scales[plane >= hkv] : 1.f;
     T* dst = stage + (((size_t)seq * stage_pages + lp) * 2 * hkv + plane) * 64 * d;
     for (int i = threadIdx.x; i < 64 * d / 8; i += blockDim.x) {
         const int r = i / (d / 8), e = (i - r * (d / 8)) * 8, slot = lp * 64 + r;
@@ -199,7 +199,7 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
 }
 
 // pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [num_seqs * stage_pages, 2, Hkv, 64, d], page s * stage_pages + i for rows 64 i.. of sequence s.  `q_len` null: only the
-// rows that were cached before this step.
+// rows that were cached before this step.  `scales` null: code * block scale, which both 16-bit types hold exactly.
 extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table, const int* past_len, const int* q_len, const int* page_table, const float* scales,
                                  int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d, int window, int is_bf16,
                                  cudaStream_t stream) {

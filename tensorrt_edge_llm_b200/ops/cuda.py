@@ -706,6 +706,10 @@ def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: i
     d = _fp4_geometry(kv_layer, meta, scales)
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"kv_fp4_stage: pages of fp16 or bf16, not {dtype}")
+    return _fp4_stage(kv_layer, meta, scales, dtype, window, new_rows, d)
+
+
+def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int, new_rows: bool, d: int):
     hkv, n = kv_layer.shape[2], meta.num_seqs
     per = max(1, (meta.max_seq_len + 63) // 64)
     stage = torch.empty(n * per, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
@@ -755,8 +759,9 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     if not direct or meta.tree_mask is not None:
         if direct:
             raise ValueError("paged_attention_fp4: tree masks are read by the prompt kernels only")
-        stage, staged = kv_fp4_stage(kv_layer, meta, scales, q.dtype, window, True)
-        return paged_attention(q, stage, staged, scale, sliding_window, sinks)
+        # codes times block scales, which 16 bits hold exactly; the two global scales multiply scores and outputs
+        stage, staged = _fp4_stage(kv_layer, meta, None, q.dtype, window, True, d)
+        return paged_attention(q, stage, staged, scale, sliding_window, sinks, kv_scales=scales)
     q = _aligned(q)
     out = torch.empty_like(q)
     if splits is None:
@@ -858,13 +863,14 @@ def _decode_splits(meta: StepMeta, hkv: int, chunk: int = 0, window: int = 0, fp
 def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sinks=None, splits: Optional[int] = None,
                     kernel: Optional[str] = None, trace: Optional[torch.Tensor] = None, causal: bool = True,
                     skip_thr: Optional[torch.Tensor] = None, skip_stats: Optional[torch.Tensor] = None, chunk: int = 0,
-                    fp32_weights: bool = False, back: Optional[tuple] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    fp32_weights: bool = False, back: Optional[tuple] = None, out: Optional[torch.Tensor] = None, kv_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Paged GQA attention.  Decode-shaped steps (``max_q_len * Hq/Hkv <= 16``, head_dim 128, causal)
     run the token-major XQA-style kernel; everything else the row-major tile kernel, or its two-tile form for plain steps of head size 128
     that it suits (all of them where ``splits`` is given).
     ``kernel`` forces ``"decode"`` or ``"tile"`` (one tile a CTA); ``causal=False`` lets every row see every token of its sequence; ``chunk`` > 0 limits
     a row to the keys of its own ``chunk``-token block; ``fp32_weights`` feeds the probabilities to the 16-bit P·V product as high + low
-    halves.  fp32 rows and head sizes without a tensor-core form run on the CUDA cores."""
+    halves.  ``kv_scales`` (two positive fp32 numbers on the device): keys and values are multiplied by them, in 32 bits, on the scores and the outputs (tile
+    kernels only).  fp32 rows and head sizes without a tensor-core form run on the CUDA cores."""
     wide = kernel is None
     if not causal:
         sliding_window, kernel = -1, "tile"
@@ -886,7 +892,7 @@ def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sin
     win = sliding_window if sliding_window and sliding_window > 0 else 0
     tm = meta.tree_mask
     if q.dtype == torch.float32 or d not in (64, 128, 256):
-        if tm is not None or not causal or skip_thr is not None or meta.skip_thr is not None:
+        if tm is not None or not causal or skip_thr is not None or meta.skip_thr is not None or kv_scales is not None:
             raise ValueError("fp32 / odd-sized attention covers causal, windowed and chunked masks only")
         _check(lib().telb_paged_attention_simt(
             _p(q), _p(kv_layer), _p(out), _p(meta.q_start), _p(meta.past_len), _p(meta.seq_ids), _p(meta.page_table), c_int(t),
@@ -901,7 +907,7 @@ def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sin
         skip_thr = skip_thr.to(device=q.device, dtype=torch.float32).contiguous()
         if kernel is None and meta.max_q_len * group > 16:
             kernel = "tile"
-    use_decode = decode_ok if kernel is None else (kernel == "decode")
+    use_decode = decode_ok and kv_scales is None if kernel is None else (kernel == "decode")
     if use_decode:
         if not decode_ok:
             raise ValueError("step is not decode-shaped")
@@ -925,7 +931,7 @@ def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sin
         c_int(kv_layer.shape[0]), c_int(meta.page_table.shape[1]), c_int(meta.page_size), c_int(hq), c_int(hkv),
         c_int(d), c_float(scale), c_int(sliding_window or 0), c_int(splits), _p(ws.attn_ws), c_ll(ws.attn_ws.numel()),
         c_int(_is_bf16(q)), _p(ws.status), _p(sinks), _p(skip_thr), _p(skip_stats), c_int(chunk), c_int(int(fp32_weights)),
-        _p(table), c_float(mult), _p(meta.positions), c_ll(ld_out), c_int(int(wide)), _stream()), "paged_attention", 2 if splits > 1 else 1)
+        _p(table), c_float(mult), _p(meta.positions), c_ll(ld_out), c_int(int(wide)), _p(kv_scales), _stream()), "paged_attention", 2 if splits > 1 else 1)
     return out
 
 
