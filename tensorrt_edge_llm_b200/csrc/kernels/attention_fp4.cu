@@ -22,7 +22,8 @@ struct Fp4AttnParams {
     const int *q_start, *q_len, *past_len, *page_table;
     const float *scales, *sinks;
     float* weights;
-    int num_seqs, tokens, max_q_len, num_pages, max_pages, page_size, hq, hkv, window, splits;
+    int2* spans;
+    int num_seqs, tokens, max_q_len, num_pages, max_pages, page_size, page_shift, hq, hkv, window, ctas, max_items;
     float scale, decay;
 };
 
@@ -113,14 +114,18 @@ struct KeyTile {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        uint32_t two[2][(D + 127) / 128];
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int i = 0; i < (D + 127) / 128; ++i) two[r][i] = e4m3x2_to_half(s[r][i]);
 #pragma unroll
         for (int j2 = 0; j2 < D / 32; ++j2) {                                   // a word: eight features, two steps
             uint32_t a[2][4], sc[2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 e2m1x8_to_half(w[r][j2], a[r][0], a[r][1], a[r][2], a[r][3]);
-                const uint32_t two = e4m3x2_to_half(s[r][j2 / 4]);                // the blocks of 16 features: two words each
-                sc[r] = __byte_perm(two, two, (j2 / 2) % 2 ? 0x3232 : 0x1010);
+                sc[r] = __byte_perm(two[r][j2 / 4], 0u, (j2 / 2) % 2 ? 0x3232 : 0x1010);      // the blocks of 16 features: two words each
 #pragma unroll
                 for (int i = 0; i < 4; ++i) a[r][i] = hmul2u(a[r][i], sc[r]);
             }
@@ -140,7 +145,7 @@ struct ValueTile {
     uint32_t w[4][D / 64];
     uint16_t s[4];
     __device__ __forceinline__ static int place(int i, int t) { return key_place(2 * t + (i & 1) + 8 * (i >> 1)); }
-    __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* sf, int g, int t, int live) {
+    __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* sf, int g, int t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int at = place(i, t);
@@ -152,8 +157,13 @@ struct ValueTile {
             if constexpr (D == 64) s[i] = f[g / 2];
             else if constexpr (D == 128) s[i] = f[g];
             else s[i] = *reinterpret_cast<const uint16_t*>(f + 2 * g);
-            if (at >= live) s[i] = 0;                                             // what lies behind the last key may be anything, NaN scales too
         }
+    }
+    // Keys from `live` on: what lies there may be anything, NaN scales too.
+    __device__ __forceinline__ void clear(int t, int live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (place(i, t) >= live) s[i] = 0;
     }
     template <int NT>
     __device__ __forceinline__ void add(const uint32_t (&pb)[NT][2], float (&o)[NT][D / 16][4]) const {
@@ -198,220 +208,424 @@ struct ColumnLimits {
     }
 };
 
-// grid (splits, KV heads x chunks of 8 NT columns, sequences).  Every split takes a contiguous part of the sequence's own keys, its warps every fourth tile.
+// ---- which keys a CTA takes ---------------------------------------------------------------------------------------------------
+//
+// An item is a sequence, a KV head and a chunk of C columns; its keys come in tiles of 32.  All tiles of all items stand in one line, which is cut into
+// equal parts, one per CTA, so that sequences of any lengths load the SMs alike.  A CTA meets whole items, whose results it writes, and parts
+// of an item at its ends, which the merge kernel joins in their order.
+
+struct Fp4Line {
+    int total, per;                                                             // tiles in the line; tiles of a CTA
+};
+
+__device__ __forceinline__ int fp4_first_tile(int past, int window) { return window > 0 ? max(0, past + 1 - window) / kFp4Tile : 0; }
+__device__ __forceinline__ int fp4_tiles(int past, int ql, int window) {
+    return ql > 0 ? (past + ql + kFp4Tile - 1) / kFp4Tile - fp4_first_tile(past, window) : 0;
+}
+__device__ __forceinline__ int fp4_items(int ql, int group, int hkv, int cols) { return (ql * group + cols - 1) / cols * hkv; }
+
+// Lengths of the line, by all lanes of a warp.
+__device__ __forceinline__ Fp4Line fp4_line(const Fp4AttnParams& p, int cols, int lane) {
+    int sum = 0;
+    const int group = p.hq / p.hkv;
+    for (int s = lane; s < p.num_seqs; s += 32) {
+        const int ql = p.q_len[s];
+        sum += fp4_tiles(p.past_len[s], ql, p.window) * fp4_items(ql, group, p.hkv, cols);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    return {sum, max((sum + (int)gridDim.x - 1) / (int)gridDim.x, kFp4Warps)};
+}
+
+// The sequence that holds place `at` of the line, and its first place.
+__device__ __forceinline__ int fp4_locate(const Fp4AttnParams& p, int cols, int lane, int at, int& start) {
+    const int group = p.hq / p.hkv;
+    int base = 0;
+    for (int s0 = 0; s0 < p.num_seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < p.num_seqs) {
+            const int ql = p.q_len[s];
+            n = fp4_tiles(p.past_len[s], ql, p.window) * fp4_items(ql, group, p.hkv, cols);
+        }
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, at < base + incl);
+        if (here) {
+            const int l = __ffs(here) - 1;
+            start = base + __shfl_sync(0xffffffffu, incl - n, l);
+            return s0 + l;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return -1;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {       // bytes 0: zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// The tiles of a warp on their way into its own ring in shared memory.  A stage: key codes [32][D/2], value codes, key scales [32][D/16], value scales.
+template <int D>
+struct Fp4Ring {
+    static constexpr int kStages = 3, kCodes = kFp4Tile * D / 2, kScales = kFp4Tile * D / 16, kBytes = 2 * (kCodes + kScales);
+    const uint8_t* base;                                                         // the head's keys in page 0
+    const int* table;
+    size_t page_bytes, value_at;
+    int page_shift, max_pages, num_pages, ids_at, ids, end;
+    uint32_t smem;
+    int lane;
+
+    __device__ __forceinline__ void begin(const Fp4AttnParams& p, int seq, int kvh, int end_, uint32_t smem_, int lane_) {
+        const size_t slab = fp4_slab_bytes(p.page_size, D);
+        base = p.pool + kvh * slab;
+        page_bytes = 2 * p.hkv * slab;
+        value_at = p.hkv * slab;
+        table = p.page_table + (size_t)seq * p.max_pages;
+        page_shift = p.page_shift;
+        max_pages = p.max_pages;
+        num_pages = p.num_pages;
+        ids_at = -64;
+        end = end_;
+        smem = smem_;
+        lane = lane_;
+    }
+    // Pages of the table are looked up 32 at a time.
+    __device__ __forceinline__ int page_of(int key) {
+        const int lp = key >> page_shift;
+        if (lp < ids_at || lp >= ids_at + 32) {
+            ids_at = lp;
+            const int i = lp + lane;
+            ids = i < max_pages ? table[i] : -1;
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, lp - ids_at);
+        return key < end && (unsigned)page < (unsigned)num_pages ? page : -1;
+    }
+    // Starts the copies of a tile; returns a bit per half that has a page (keys from `end` on count as having none).
+    __device__ __forceinline__ uint32_t load(int stage, int tile, bool real) {
+        uint32_t there = 0;
+        if (real) {
+            const int kb = tile * kFp4Tile, at = kb & ((1 << page_shift) - 1);
+            const uint32_t dst = smem + stage * kBytes;
+            int page[2];
+            page[0] = page_of(kb);
+            if (page_shift >= 5) page[1] = kb + 16 < end ? page[0] : -1;
+            else page[1] = page_of(kb + 16);
+            there = (page[0] >= 0 ? 1u : 0u) | (page[1] >= 0 ? 2u : 0u);
+            const int at1 = page_shift >= 5 ? at + 16 : 0;
+            const uint8_t* k0 = base + (size_t)max(page[0], 0) * page_bytes;
+            const uint8_t* k1 = base + (size_t)max(page[1], 0) * page_bytes;
+            const uint32_t n0 = page[0] >= 0 ? 16u : 0u, n1 = page[1] >= 0 ? 16u : 0u;
+            constexpr int kHalf = 16 * D / 2;                                     // bytes of 16 rows of codes
+#pragma unroll
+            for (int i = 0; i < kHalf / 512; ++i) {
+                const int o = i * 512 + lane * 16;
+                cp_async16(dst + o, k0 + (size_t)at * (D / 2) + o, n0);
+                cp_async16(dst + kCodes + o, k0 + value_at + (size_t)at * (D / 2) + o, n0);
+                cp_async16(dst + kHalf + o, k1 + (size_t)at1 * (D / 2) + o, n1);
+                cp_async16(dst + kCodes + kHalf + o, k1 + value_at + (size_t)at1 * (D / 2) + o, n1);
+            }
+            constexpr int kPieces = D / 16;                                       // of 16 bytes, in 16 rows of scales
+#pragma unroll
+            for (int i = lane; i < 4 * kPieces; i += 32) {
+                const int v = i / (2 * kPieces), h = i / kPieces % 2, o = i % kPieces * 16;
+                const uint8_t* src = (h ? k1 : k0) + (v ? value_at : 0) + ((size_t)(D / 2) << page_shift) + (size_t)(h ? at1 : at) * (D / 16) + o;
+                cp_async16(dst + 2 * kCodes + v * kScales + h * (kScales / 2) + o, src, h ? n1 : n0);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        return there;
+    }
+};
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(kFp4Warps * 32) attention_fp4_kernel(const Fp4AttnParams p) {
+struct Fp4Occupancy {
+    // CTAs an SM: registers for the accumulators (4 NT D/16) and the queries (2 NT D/16) besides some 60; three stages of a ring a warp
+    static constexpr int kCtas = D * NT <= 128 ? 4 : D * NT <= 256 && D < 256 ? 3 : 2;
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas)) attention_fp4_kernel(const Fp4AttnParams p) {
     pdl_prologue();
     constexpr int C = 8 * NT;
-    extern __shared__ float smem[];                                              // [warps][C][D] outputs, then [warps][C][2] (reference, sum)
-    const int seq = blockIdx.z, kvh = blockIdx.y % p.hkv, chunk = blockIdx.y / p.hkv;
+    using Ring = Fp4Ring<D>;
+    extern __shared__ __align__(16) uint8_t smem[];                              // rings; after a segment [warps][C][D] outputs and [warps][C][2] (reference, sum)
+    float* smem_f = reinterpret_cast<float*>(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = p.hq / p.hkv, ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
-    if (chunk * C >= columns) return;
-    const int q0 = p.q_start[seq];
-    const int* table = p.page_table + (size_t)seq * p.max_pages;
-    const size_t slab = fp4_slab_bytes(p.page_size, D);
+    const int group = p.hq / p.hkv;
+    const Fp4Line line = fp4_line(p, C, lane);
+    int at = blockIdx.x * line.per;
+    const int stop = min(line.total, at + line.per);
+    if (at >= stop) return;
+    int seq_start = 0, seq = fp4_locate(p, C, lane, at, seq_start);
+    const float base = p.scale * 1.4426950408889634f * p.scales[0], v_scale = p.scales[1];
+    const uint32_t ring_at = smem_u32(smem) + warp * Ring::kStages * Ring::kBytes;
+    const uint8_t* ring_ptr = smem + warp * Ring::kStages * Ring::kBytes;
 
-    uint32_t qb[NT][D / 16][2];
-    float factor[NT][2];
-    int low[NT][2], high[NT][2];
-    const float base = p.scale * 1.4426950408889634f * p.scales[0];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int c = chunk * C + n * 8 + g;
-        const int r = c / group, h = kvh * group + c - r * group;
-        const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + ((size_t)(q0 + r) * p.hq + h) * D + t * (D / 4), c < columns, qb[n]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            factor[n][i] = base * __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
-            const ColumnLimits lim(chunk * C + n * 8 + 2 * t + i, columns, group, past, p.window);
-            low[n][i] = lim.low;
-            high[n][i] = lim.high;
+    while (at < stop) {
+        const int ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
+        const int tiles = fp4_tiles(past, ql, p.window), items = fp4_items(ql, group, p.hkv, C);
+        if (at >= seq_start + tiles * items) {                                   // on to the next sequence
+            seq_start += tiles * items;
+            ++seq;
+            continue;
         }
-    }
-    const int r_first = chunk * C / group, r_last = (min(columns, chunk * C + C) - 1) / group;
-    const int first = p.window > 0 ? max(0, past + r_first + 1 - p.window) : 0, end = past + r_last + 1;
-    const int all_low = p.window > 0 ? max(0, past + r_last + 1 - p.window) : 0, all_high = past + r_first + 1;      // visible to every column
-    const int tile0 = first / kFp4Tile, tiles = (end + kFp4Tile - 1) / kFp4Tile - tile0;
-    const int t_begin = tile0 + (int)((long long)tiles * blockIdx.x / p.splits), t_end = tile0 + (int)((long long)tiles * (blockIdx.x + 1) / p.splits);
+        const int item = (at - seq_start) / tiles, off = (at - seq_start) - item * tiles;
+        const int count = min(tiles - off, stop - at);
+        const int chunk = item / p.hkv, kvh = item - chunk * p.hkv;
+        const int tile0 = fp4_first_tile(past, p.window) + off, tile1 = tile0 + count;
+        const int q0 = p.q_start[seq];
+        const int r_first = chunk * C / group, r_last = (min(columns, chunk * C + C) - 1) / group;
+        const int end = past + r_last + 1;
+        const int all_low = p.window > 0 ? max(0, past + r_last + 1 - p.window) : 0, all_high = past + r_first + 1;      // visible to every column
 
-    float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
+        Ring ring;
+        ring.begin(p, seq, kvh, end, ring_at, lane);
+        uint32_t flags = 0;                                                      // two bits a stage
+        int next = tile0 + warp;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
+        for (int s = 0; s < Ring::kStages - 1; ++s, next += kFp4Warps) flags |= ring.load(s, next, next < tile1) << (2 * s);
+
+        uint32_t qb[NT][D / 16][2];
+        float factor[NT][2];
+        int low[NT][2], high[NT][2];
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
+        for (int n = 0; n < NT; ++n) {
+            const int c = chunk * C + n * 8 + g;
+            const int r = c / group, h = kvh * group + c - r * group;
+            const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + ((size_t)(q0 + r) * p.hq + h) * D + t * (D / 4), c < columns, qb[n]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
-        ref[n][0] = ref[n][1] = kRefStart;
-        sum[n][0] = sum[n][1] = 0.f;
-    }
-    for (int tile = t_begin + warp; tile < t_end; tile += kFp4Warps) {
-        const int kb = tile * kFp4Tile;
-        float s[2][NT][4];
-        KeyTile<D> kt[2];
-        ValueTile<D> vt[2];
-        bool there[2];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const int k0 = kb + 16 * m, lp = k0 / p.page_size, at = k0 - lp * p.page_size;
-            const int page = k0 < end && lp < p.max_pages ? table[lp] : -1;
-            there[m] = (unsigned)page < (unsigned)p.num_pages;
-            const uint8_t* ks = p.pool + ((size_t)(there[m] ? page : 0) * 2 * p.hkv + kvh) * slab;
-            const uint8_t* vs = ks + (size_t)p.hkv * slab;
-            kt[m].load(ks + (size_t)at * (D / 2), ks + (size_t)p.page_size * (D / 2) + (size_t)at * (D / 16), g, t);
-            vt[m].load(vs + (size_t)at * (D / 2), vs + (size_t)p.page_size * (D / 2) + (size_t)at * (D / 16), g, t, there[m] ? end - k0 : 0);
+            for (int i = 0; i < 2; ++i) {
+                factor[n][i] = base * __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
+                const ColumnLimits lim(chunk * C + n * 8 + 2 * t + i, columns, group, past, p.window);
+                low[n][i] = lim.low;
+                high[n][i] = lim.high;
+            }
         }
+        float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) kt[m].template scores<NT>(qb, s[m]);
-        const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there[0] && there[1];
-        uint32_t pb[2][NT][2];
-        float x[2][NT][4];
-        auto shifted = [&]() {
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+            for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
+            ref[n][0] = ref[n][1] = kRefStart;
+            sum[n][0] = sum[n][1] = 0.f;
+        }
+        int stage = 0;
+        for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
+            const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
+            __syncwarp();                                                        // the stage to be filled has been read by all lanes
+            const uint32_t more = ring.load(ahead, next, next < tile1);
+            flags = (flags & ~(3u << (2 * ahead))) | (more << (2 * ahead));
+            next += kFp4Warps;
+            asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
+            __syncwarp();
+            const uint8_t* st = ring_ptr + stage * Ring::kBytes;
+            const uint32_t there = (flags >> (2 * stage)) & 3u;
+            const int kb = tile * kFp4Tile;
+            float s[2][NT][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[m][n][i] = fmaf(s[m][n][i], factor[n][i & 1], -ref[n][i & 1]);
-                        if (!open) {
-                            const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1);
-                            if (!there[m] || key < low[n][i & 1] || key >= high[n][i & 1]) x[m][n][i] = -INFINITY;
-                        }
-                    }
-        };
-        shifted();
-        bool over = false;
+            for (int m = 0; m < 2; ++m) {
+                KeyTile<D> kt;
+                kt.load(st + m * (16 * D / 2), st + 2 * Ring::kCodes + m * D, g, t);
+                kt.template scores<NT>(qb, s[m]);
+            }
+            const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there == 3u;
+            float x[2][NT][4];
+            auto shifted = [&]() {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+                for (int m = 0; m < 2; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) over = over || x[0][n][i] > 15.f || x[1][n][i] > 15.f;
-        if (__any_sync(0xffffffffu, over)) {
-            float up[NT][2];
+                    for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    // scores themselves: x has lost them where the reference is the first one
-                    float top = -INFINITY;
+                        for (int i = 0; i < 4; ++i) x[m][n][i] = fmaf(s[m][n][i], factor[n][i & 1], -ref[n][i & 1]);
+                if (!open) {
 #pragma unroll
                     for (int m = 0; m < 2; ++m)
 #pragma unroll
-                        for (int i = c; i < 4; i += 2)
-                            if (x[m][n][i] > -INFINITY) top = fmaxf(top, s[m][n][i] * factor[n][c]);
+                        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const float next = top - ref[n][c] > 15.f ? top - 8.f : ref[n][c];
-                    up[n][c] = exp2_approx(ref[n][c] - next);
-                    ref[n][c] = next;
-                    sum[n][c] *= up[n][c];
+                            for (int i = 0; i < 4; ++i) {
+                                const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1);
+                                if (!((there >> m) & 1u) || key < low[n][i & 1] || key >= high[n][i & 1]) x[m][n][i] = -INFINITY;
+                            }
                 }
+            };
+            shifted();
+            float most = -INFINITY;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(x[0][n][i], x[1][n][i]));
+            if (__any_sync(0xffffffffu, most > 15.f)) {
+                float up[NT][2];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) o[n][i][k] *= up[n][k & 1];
-            shifted();
-        }
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+                    for (int c = 0; c < 2; ++c) {
+                        // scores themselves: x has lost them where the reference is the first one
+                        float top = -INFINITY;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+                        for (int m = 0; m < 2; ++m)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[m][n][i] = exp2_approx(x[m][n][i]);
-                    sum[n][i & 1] += x[m][n][i];
+                            for (int i = c; i < 4; i += 2)
+                                if (x[m][n][i] > -INFINITY) top = fmaxf(top, s[m][n][i] * factor[n][c]);
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        const float next_ref = top - ref[n][c] > 15.f ? top - 8.f : ref[n][c];
+                        up[n][c] = exp2_approx(ref[n][c] - next_ref);
+                        ref[n][c] = next_ref;
+                        sum[n][c] *= up[n][c];
+                    }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[n][i][k] *= up[n][k & 1];
+                shifted();
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[m][n][i] = exp2_approx(x[m][n][i]);
+                        sum[n][i & 1] += x[m][n][i];
+                    }
+                    pb[n][0] = transpose8(Cvt<__half>::pack2(x[m][n][0], x[m][n][1]));
+                    pb[n][1] = transpose8(Cvt<__half>::pack2(x[m][n][2], x[m][n][3]));
                 }
-                pb[m][n][0] = transpose8(Cvt<__half>::pack2(x[m][n][0], x[m][n][1]));
-                pb[m][n][1] = transpose8(Cvt<__half>::pack2(x[m][n][2], x[m][n][3]));
+                ValueTile<D> vt;
+                vt.load(st + Ring::kCodes + m * (16 * D / 2), st + 2 * Ring::kCodes + Ring::kScales + m * D, g, t);
+                if (!open) vt.clear(t, end - kb - 16 * m);
+                vt.template add<NT>(pb, o);
             }
+            stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();                                                         // the rings have been read: their place takes the warps' results
+        float* so = smem_f + warp * C * D;
+        float* sml = smem_f + kFp4Warps * C * D;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) vt[m].template add<NT>(pb[m], o);
-    }
-    // join the warps
-    float* so = smem + warp * C * D;
-    float* sml = smem + kFp4Warps * C * D;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+            for (int c = 0; c < 2; ++c) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+                for (int d = 4; d < 32; d *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], d);
+                const int col = n * 8 + 2 * t + c;
+                if (g == 0) {
+                    sml[(warp * C + col) * 2] = ref[n][c];
+                    sml[(warp * C + col) * 2 + 1] = sum[n][c];
+                }
 #pragma unroll
-            for (int d = 4; d < 32; d *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], d);
-            const int col = n * 8 + 2 * t + c;
-            if (g == 0) {
-                sml[(warp * C + col) * 2] = ref[n][c];
-                sml[(warp * C + col) * 2 + 1] = sum[n][c];
+                for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(so + col * D + g * (D / 8) + 2 * i) = make_float2(o[n][i][c], o[n][i][c + 2]);
             }
+        __syncthreads();
+        const int live = min(C, columns - chunk * C);
+        const bool whole = count == tiles;
+        const size_t slot = (size_t)blockIdx.x * 2 + (off == 0);                 // parts: [0] what began in an earlier CTA, [1] what goes on in a later one
+        if (threadIdx.x == 0 && off == 0 && p.spans && item < p.max_items)
+            p.spans[(size_t)seq * p.max_items + item] = make_int2(blockIdx.x, (at + tiles - 1) / line.per);
+        for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
+            const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
+            float top = kRefStart;
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(so + col * D + g * (D / 8) + 2 * i) = make_float2(o[n][i][c], o[n][i][c + 2]);
-        }
-    __syncthreads();
-    const int live = min(C, columns - chunk * C);
-    for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
-        const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
-        float top = kRefStart;
+            for (int w = 0; w < kFp4Warps; ++w) top = fmaxf(top, sml[(w * C + col) * 2]);
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kFp4Warps; ++w) top = fmaxf(top, sml[(w * C + col) * 2]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kFp4Warps; ++w) {
-            const float f = exp2_approx(sml[(w * C + col) * 2] - top);
-            const float4 v = *reinterpret_cast<const float4*>(smem + (w * C + col) * D + d);
-            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-            l += f * sml[(w * C + col) * 2 + 1];
-        }
-        const int c = chunk * C + col, r = c / group, h = kvh * group + c - r * group;
-        const size_t row = (size_t)(q0 + r) * p.hq + h;
-        if (p.splits > 1) {
-            const size_t at = row * p.splits + blockIdx.x;
-            *reinterpret_cast<float4*>(p.part_o + at * D + d) = acc;
-            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + at * 2) = make_float2(top, l);
-        } else {
-            if (p.sinks) {
-                const float z = p.sinks[h] * 1.4426950408889634f, m = fmaxf(top, z), f = exp2_approx(top - m);
-                acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-                l = l * f + exp2_approx(z - m);
-                top = m;
+            for (int w = 0; w < kFp4Warps; ++w) {
+                const float f = exp2_approx(sml[(w * C + col) * 2] - top);
+                const float4 v = *reinterpret_cast<const float4*>(smem_f + (w * C + col) * D + d);
+                acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+                l += f * sml[(w * C + col) * 2 + 1];
             }
-            const float inv = l == 0.f ? 0.f : 1.f / l, f = inv * p.scales[1];                 // a row that sees nothing gives zeros
-            *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + row * D + d) = make_uint2(Cvt<T>::pack2(acc.x * f, acc.y * f), Cvt<T>::pack2(acc.z * f, acc.w * f));
-            if (p.stat && d == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
+            if (!whole) {
+                *reinterpret_cast<float4*>(p.part_o + (slot * C + col) * D + d) = acc;
+                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C + col) * 2) = make_float2(top, l);
+            } else {
+                const int c = chunk * C + col, r = c / group, h = kvh * group + c - r * group;
+                const size_t row = (size_t)(q0 + r) * p.hq + h;
+                if (p.sinks) {
+                    const float z = p.sinks[h] * 1.4426950408889634f, m = fmaxf(top, z), f = exp2_approx(top - m);
+                    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+                    l = l * f + exp2_approx(z - m);
+                    top = m;
+                }
+                const float inv = l == 0.f ? 0.f : 1.f / l, f = inv * v_scale;                 // a row that sees nothing gives zeros
+                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + row * D + d) = make_uint2(Cvt<T>::pack2(acc.x * f, acc.y * f), Cvt<T>::pack2(acc.z * f, acc.w * f));
+                if (p.stat && d == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
+            }
         }
+        at += count;
+        if (at < stop) __syncthreads();                                          // the next segment's tiles go where the results were
     }
 }
 
-// One warp per (row, head): the splits' parts joined in their order.
-template <typename T, int D>
+// grid (items of a sequence, sequences, columns of an item): the parts of a column joined in their order, a fourth of them a warp.
+template <typename T, int D, int NT>
 __global__ void __launch_bounds__(128) attention_fp4_merge_kernel(const Fp4AttnParams p) {
+    constexpr int C = 8 * NT, E = D / 32;
+    __shared__ float s_o[4][D], s_ml[4][2];
+    const int item = blockIdx.x, seq = blockIdx.y, col = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_prologue();
-    const long long row = (blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (row >= (long long)p.tokens * p.hq) return;
-    const int h = (int)(row % p.hq);
-    const float* ml = p.part_ml + (size_t)row * p.splits * 2;
-    const float z = p.sinks ? p.sinks[h] * 1.4426950408889634f : kRefStart;
-    float top = z;
-    for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, ml[2 * s]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    constexpr int E = D / 32;
-    float acc[E], l = p.sinks ? exp2_approx(z - top) : 0.f;
+    const int group = p.hq / p.hkv, chunk = item / p.hkv, kvh = item - chunk * p.hkv;
+    const int c = chunk * C + col, ql = p.q_len[seq];
+    if (c >= ql * group) return;
+    const int2 span = p.spans[(size_t)seq * p.max_items + item];
+    if (span.x >= span.y) return;                                                // whole: written already
+    const int parts = span.y - span.x + 1;
+    float top = kRefStart, l = 0.f, acc[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float f = exp2_approx(ml[2 * s] - top);
-        l += f * ml[2 * s + 1];
-        const float* src = p.part_o + ((size_t)row * p.splits + s) * D + lane * E;
+    // the first part is slot 1 of its CTA, the others slot 0
+    auto slot_of = [&](int i) { return ((size_t)(span.x + i) * 2 + (i == 0)) * C + col; };
+    for (int i = warp + 4 * lane; i < parts; i += 128) top = fmaxf(top, p.part_ml[slot_of(i) * 2]);
 #pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] += f * src[i];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 4
+    for (int i = warp; i < parts; i += 4) {
+        const size_t s = slot_of(i);
+        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
+        const float f = exp2_approx(ml.x - top);
+        l += f * ml.y;
+        const float* src = p.part_o + s * D + lane * E;
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] += f * src[k];
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l, f = inv * p.scales[1];
-    T* dst = reinterpret_cast<T*>(p.out) + (size_t)row * D + lane * E;
 #pragma unroll
-    for (int i = 0; i < E; i += 2) *reinterpret_cast<uint32_t*>(dst + i) = Cvt<T>::pack2(acc[i] * f, acc[i + 1] * f);
-    if (p.stat && lane == 0) *reinterpret_cast<float2*>(p.stat + (size_t)row * 2) = make_float2(top, inv);
+    for (int k = 0; k < E; ++k) s_o[warp][lane * E + k] = acc[k];
+    if (lane == 0) s_ml[warp][0] = top, s_ml[warp][1] = l;
+    __syncthreads();
+    const int r = c / group, h = kvh * group + c - r * group;
+    const size_t row = (size_t)(p.q_start[seq] + r) * p.hq + h;
+    const float z = p.sinks ? p.sinks[h] * 1.4426950408889634f : kRefStart;
+    top = z;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][0]);
+    l = p.sinks ? exp2_approx(z - top) : 0.f;
+    float f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        f[w] = exp2_approx(s_ml[w][0] - top);
+        l += f[w] * s_ml[w][1];
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    for (int d = threadIdx.x * 2; d < D; d += 256) {
+        float v[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[k] = (f[0] * s_o[0][d + k] + f[1] * s_o[1][d + k] + f[2] * s_o[2][d + k] + f[3] * s_o[3][d + k]) * inv * p.scales[1];
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row * D + d) = Cvt<T>::pack2(v[0], v[1]);
+    }
+    if (p.stat && threadIdx.x == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
 }
 
 // Accumulated attention weights: weights[page, head, slot] = decay * weights + the sum over the step's rows and the group's heads of
@@ -428,7 +642,7 @@ __global__ void __launch_bounds__(kFp4Warps * 32) attention_fp4_weights_kernel(c
     const size_t slab = fp4_slab_bytes(p.page_size, D);
     const int first = p.window > 0 ? max(0, past + 1 - p.window) : 0, end = past + ql;
     const int tile0 = first / kFp4Tile, tiles = (end + kFp4Tile - 1) / kFp4Tile - tile0;
-    const int t_begin = tile0 + (int)((long long)tiles * blockIdx.x / p.splits), t_end = tile0 + (int)((long long)tiles * (blockIdx.x + 1) / p.splits);
+    const int t_begin = tile0 + (int)((long long)tiles * blockIdx.x / gridDim.x), t_end = tile0 + (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x);
     const float base = p.scale * 1.4426950408889634f * p.scales[0];
     for (int tile = t_begin + warp; tile < t_end; tile += kFp4Warps) {
         const int kb = tile * kFp4Tile;
@@ -487,30 +701,31 @@ __global__ void __launch_bounds__(kFp4Warps * 32) attention_fp4_weights_kernel(c
     }
 }
 
-template <typename T, int D>
-int launch_attention_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
-    const int columns = p.max_q_len * (p.hq / p.hkv);
-    constexpr int kMost = D == 256 ? 1 : 2;
-    const int nt = columns > 8 ? kMost : 1;
-    const int chunks = (columns + 8 * nt - 1) / (8 * nt);
-    if ((long long)chunks * p.hkv > 65535 || p.num_seqs > 65535) return fail("telb_paged_attention_fp4: too many sequences or columns");
-    const int smem = kFp4Warps * 8 * nt * (D + 2) * 4;
-    const dim3 grid(p.splits, chunks * p.hkv, p.num_seqs), blk(kFp4Warps * 32);
-    if (nt == 1) {
-        TELB_LAUNCH("attention_fp4_kernel", (attention_fp4_kernel<T, D, 1>), grid, blk, smem, stream, p);
-    } else {
-        TELB_LAUNCH("attention_fp4_kernel", (attention_fp4_kernel<T, D, kMost>), grid, blk, smem, stream, p);
+template <typename T, int D, int NT>
+int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t stream) {
+    constexpr int C = 8 * NT;
+    constexpr int kSmem = kFp4Warps * Fp4Ring<D>::kStages * Fp4Ring<D>::kBytes;
+    static_assert(kSmem >= kFp4Warps * C * (D + 2) * 4, "the warps' results fit where their rings were");
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(attention_fp4_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4)", e);
+        if (dev >= 0 && dev < 64) configured[dev] = true;
     }
-    if (p.splits > 1) {
-        const long long rows = (long long)p.tokens * p.hq;
-        TELB_LAUNCH("attention_fp4_merge_kernel", (attention_fp4_merge_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, stream, p);
-    }
+    TELB_LAUNCH("attention_fp4_kernel", (attention_fp4_kernel<T, D, NT>), dim3(p.ctas), dim3(kFp4Warps * 32), kSmem, stream, p);
+    if (p.spans) TELB_LAUNCH("attention_fp4_merge_kernel", (attention_fp4_merge_kernel<T, D, NT>), dim3(p.max_items, p.num_seqs, min(columns, C)), dim3(128), 0, stream, p);
     return 0;
 }
 
 template <typename T, int D>
-int launch_weights_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
-    TELB_LAUNCH("attention_fp4_weights_kernel", (attention_fp4_weights_kernel<T, D>), dim3(p.splits, p.hkv, p.num_seqs), dim3(kFp4Warps * 32), 0, stream, p);
+int launch_attention_fp4(const Fp4AttnParams& p, int weight_splits, cudaStream_t stream) {
+    const int columns = p.max_q_len * (p.hq / p.hkv);
+    constexpr int kMost = D == 256 ? 1 : 2;
+    const int rc = columns <= 8 ? launch_attention_fp4_nt<T, D, 1>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost>(p, columns, stream);
+    if (rc || !p.weights) return rc;
+    TELB_LAUNCH("attention_fp4_weights_kernel", (attention_fp4_weights_kernel<T, D>), dim3(weight_splits, p.hkv, p.num_seqs), dim3(kFp4Warps * 32), 0, stream, p);
     return 0;
 }
 
@@ -518,27 +733,32 @@ int launch_weights_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
 
 using namespace telb;
 
-// `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and `weight_splits` parts of every sequence's keys run at once.
+// Columns (rows x heads of a KV head) that an item takes, of a step with `columns` of them.
+extern "C" int telb_attention_fp4_columns(int columns, int d) { return columns <= 8 || d == 256 ? 8 : 16; }
+// CTAs that run at once.
+extern "C" int telb_attention_fp4_ctas(int columns, int d) {
+    const int nt = telb_attention_fp4_columns(columns, d) / 8;
+    return sm_count() * (d * nt <= 128 ? 4 : d * nt <= 256 && d < 256 ? 3 : 2);
+}
+
+// part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C of telb_attention_fp4_columns, max_items = KV heads x chunks of the longest
+// sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and `weight_splits` parts of every
+// sequence's keys run at once.
 extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int weight_splits, int is_bf16, cudaStream_t stream) {
     const Fp4AttnParams& p = *params;
     if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
     if (d != 64 && d != 128 && d != 256) return fail("telb_paged_attention_fp4: head_dim must be 64, 128 or 256");
-    if (p.page_size <= 0 || p.page_size % 16) return fail("telb_paged_attention_fp4: the page size must be a multiple of 16");
+    if (p.page_size < 16 || p.page_size != 1 << p.page_shift) return fail("telb_paged_attention_fp4: the page size must be a power of two, at least 16");
     if (p.hkv <= 0 || p.hq % p.hkv) return fail("telb_paged_attention_fp4: query heads must be a multiple of the KV heads");
-    if (p.splits < 1 || (p.splits > 1 && (!p.part_o || !p.part_ml))) return fail("telb_paged_attention_fp4: splits without room for their parts");
-    if (p.weights && (!p.stat || weight_splits < 1)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
-    int rc;
-    Fp4AttnParams w = p;
-    w.splits = weight_splits;
-#define ATTN_FP4(T, D) rc = launch_attention_fp4<T, D>(p, stream); if (rc == 0 && p.weights) rc = launch_weights_fp4<T, D>(w, stream)
+    if (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans) return fail("telb_paged_attention_fp4: no room for the parts");
+    if (p.num_seqs > 65535) return fail("telb_paged_attention_fp4: more than 65535 sequences");
+    if (p.weights && (!p.stat || weight_splits < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
     if (is_bf16) {
-        if (d == 128) { ATTN_FP4(__nv_bfloat16, 128); }
-        else if (d == 64) { ATTN_FP4(__nv_bfloat16, 64); }
-        else { ATTN_FP4(__nv_bfloat16, 256); }
-    } else {
-        if (d == 128) { ATTN_FP4(__half, 128); }
-        else if (d == 64) { ATTN_FP4(__half, 64); }
-        else { ATTN_FP4(__half, 256); }
+        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, weight_splits, stream);
+        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, weight_splits, stream);
+        return launch_attention_fp4<__nv_bfloat16, 256>(p, weight_splits, stream);
     }
-    return rc;
+    if (d == 128) return launch_attention_fp4<__half, 128>(p, weight_splits, stream);
+    if (d == 64) return launch_attention_fp4<__half, 64>(p, weight_splits, stream);
+    return launch_attention_fp4<__half, 256>(p, weight_splits, stream);
 }

@@ -384,7 +384,7 @@ def rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, num_q_heads, num_kv_heads, h
                       stage=None, stage_table=None):
     """:func:`rope_kv_write` into four-bit (NVFP4) pages: returns ``q [T, Hq, D]``; keys and values are quantised as they are written.
 
-    ``kv_layer``: ``uint8 [pages, 2, Hkv, P, 9 D / 16]``, D 64, 128 or 256, P a multiple of 16.  The part of a page that holds one head's keys or
+    ``kv_layer``: ``uint8 [pages, 2, Hkv, P, 9 D / 16]``, D 64, 128 or 256, P a power of two from 16 on.  The part of a page that holds one head's keys or
     values has the codes ``[P, D / 2]`` (E2M1, even feature in the low nibble) in front and the block scales ``[P, D / 16]`` (E4M3, one per
     16 features) behind them; a value is ``code * block scale * scales[0 keys, 1 values]`` (``scales`` fp32, on the device).  A block whose
     features hold a NaN becomes NaN.  ``stage`` (16-bit pages ``[*, 2, Hkv, P', D]``) with ``stage_table`` ``[sequences, pages]``: the

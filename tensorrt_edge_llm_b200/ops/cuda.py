@@ -641,8 +641,8 @@ class Fp4WriteParams(ctypes.Structure):
 
 class Fp4AttnParams(ctypes.Structure):
     """Host mirror of ``Fp4AttnParams`` (``csrc/kernels/attention_fp4.cu``)."""
-    _fields_ = [(n, c_vp) for n in ("q", "pool", "out", "part_o", "part_ml", "stat", "q_start", "q_len", "past_len", "page_table", "scales", "sinks", "weights")] + \
-               [(n, c_int) for n in ("num_seqs", "tokens", "max_q_len", "num_pages", "max_pages", "page_size", "hq", "hkv", "window", "splits")] + \
+    _fields_ = [(n, c_vp) for n in ("q", "pool", "out", "part_o", "part_ml", "stat", "q_start", "q_len", "past_len", "page_table", "scales", "sinks", "weights", "spans")] + \
+               [(n, c_int) for n in ("num_seqs", "tokens", "max_q_len", "num_pages", "max_pages", "page_size", "page_shift", "hq", "hkv", "window", "ctas", "max_items")] + \
                [("scale", c_float), ("decay", c_float)]
 
 
@@ -724,15 +724,11 @@ FP4_DIRECT_COLUMNS = 64      # rows x heads of a KV head up to which a step read
 FP4_WEIGHT_COLUMNS = 256     # and up to which it keeps account of the attention weights
 
 
-def _fp4_splits(items: int, keys: int) -> int:
-    return max(1, min(4 * 148 // max(1, items), (keys + 127) // 128, 64))
-
-
 @_on_device
 def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, sliding_window=None, sinks=None, weights=None, decay: float = 1.0,
-                        direct: Optional[bool] = None, splits: Optional[int] = None) -> torch.Tensor:
+                        direct: Optional[bool] = None, ctas: Optional[int] = None) -> torch.Tensor:
     """See :func:`ops.paged_attention_fp4`.  ``direct`` forces the kernel that reads the pages in place (True), or the expansion to 16 bits and
-    the prompt kernels (False); ``splits``: parts of a sequence's keys."""
+    the prompt kernels (False); ``ctas``: into how many parts that kernel cuts its work."""
     d = _fp4_geometry(kv_layer, meta, scales)
     is_bf16 = _is_bf16(q)
     t, hq = q.shape[:2]
@@ -764,19 +760,23 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
         return paged_attention(q, stage, staged, scale, sliding_window, sinks, kv_scales=scales)
     q = _aligned(q)
     out = torch.empty_like(q)
-    if splits is None:
-        splits = _fp4_splits(meta.num_seqs * hkv * ((columns + 15) // 16), min(meta.max_seq_len, window + meta.max_q_len) if window else meta.max_seq_len)
-    part_o = part_ml = stat = None
-    if splits > 1:
-        part_o = torch.empty(t * hq * splits, d, dtype=torch.float32, device=q.device)
-        part_ml = torch.empty(t * hq * splits, 2, dtype=torch.float32, device=q.device)
-    if weights is not None:
-        stat = torch.empty(t * hq, 2, dtype=torch.float32, device=q.device)
+    n, L = meta.num_seqs, lib()
+    cols = L.telb_attention_fp4_columns(c_int(columns), c_int(d))
+    items = hkv * -(-columns // cols)
+    if ctas is None:            # as many as run at once, of four tiles of 32 keys or more
+        tiles = n * items * (-(-min(meta.max_seq_len, window + meta.max_q_len if window else meta.max_seq_len) // 32) + 1)
+        ctas = max(1, min(L.telb_attention_fp4_ctas(c_int(columns), c_int(d)), tiles // 4))
+    # parts of outputs, their references and sums, (first, last) CTA of every item, softmax statistics of the rows
+    room = [2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items, 2 * t * hq if weights is not None else 0]
+    ws = torch.empty(sum(room), dtype=torch.float32, device=q.device)
+    at = _p(ws).value
+    part_o, part_ml, spans, stat = at, at + 4 * room[0], at + 4 * (room[0] + room[1]), at + 4 * sum(room[:3]) if weights is not None else None
     ptr = lambda v: None if v is None else _p(v).value
-    p = Fp4AttnParams(*[ptr(v) for v in (q, kv_layer, out, part_o, part_ml, stat, meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
-                      meta.num_seqs, t, meta.max_q_len, kv_layer.shape[0], meta.page_table.shape[1], meta.page_size, hq, hkv, window, splits, scale, decay)
-    _check(lib().telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(splits), c_int(is_bf16), _stream()), "paged_attention_fp4",
-           1 + (splits > 1) + (weights is not None))
+    p = Fp4AttnParams(ptr(q), ptr(kv_layer), ptr(out), part_o, part_ml, stat, *[ptr(v) for v in (meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
+                      spans, n, t, meta.max_q_len, kv_layer.shape[0], meta.page_table.shape[1], meta.page_size, meta.page_size.bit_length() - 1, hq, hkv, window, ctas,
+                      items, scale, decay)
+    splits = max(1, min(4 * 148 // (n * hkv), -(-meta.max_seq_len // 128), 64))
+    _check(L.telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(splits), c_int(is_bf16), _stream()), "paged_attention_fp4", 2 + (weights is not None))
     return out
 
 

@@ -75,14 +75,14 @@ def test_attention_in_place(q_lens, past, hq, hkv, d, page, window, dtype, sunk)
     top = 6 * 448 * float(scales[1])
     m, lg, qg, sg = meta.to("cuda"), layer.cuda(), q.cuda(), scales.cuda()
     zg = sinks.cuda() if sunk else None
-    for splits in (None, 1, 3):
+    for ctas in (None, 1, 3):
         wg = w.cuda()
-        got = ops.cuda_ops().paged_attention_fp4(qg, lg, m, d ** -0.5, sg, window or None, zg, wg, 0.75, splits=splits)
-        again = ops.cuda_ops().paged_attention_fp4(qg, lg, m, d ** -0.5, sg, window or None, zg, direct=True, splits=splits)
+        got = ops.cuda_ops().paged_attention_fp4(qg, lg, m, d ** -0.5, sg, window or None, zg, wg, 0.75, ctas=ctas)
+        again = ops.cuda_ops().paged_attention_fp4(qg, lg, m, d ** -0.5, sg, window or None, zg, direct=True, ctas=ctas)
         assert torch.equal(got, again)
-        assert ((got.cpu().double() - want).abs() <= bound(want, top, dtype)).all(), splits
+        assert ((got.cpu().double() - want).abs() <= bound(want, top, dtype)).all(), ctas
         # a probability is off by the 32-bit error of its score and of the sum: 2^-15 of it, up to group * rows of them a key
-        assert ((wg.cpu().double() - want_w).abs() <= 2 ** -15 * want_w + 1e-6).all(), splits
+        assert ((wg.cpu().double() - want_w).abs() <= 2 ** -15 * want_w + 1e-6).all(), ctas
     if not sunk:
         assert torch.equal(ops.paged_attention_fp4(qg, lg, m, d ** -0.5, sg, sliding_window=window or None, weights=w.cuda(), decay=0.75),
                            ops.paged_attention_fp4(qg, lg, m, d ** -0.5, sg, sliding_window=window or None, weights=torch.zeros_like(w).cuda()))
