@@ -649,7 +649,7 @@ class Fp4AttnParams(ctypes.Structure):
 class EvictParams(ctypes.Structure):
     """Host mirror of ``EvictParams`` (``csrc/kernels/kv_evict.cu``)."""
     _fields_ = [(n, c_vp) for n in ("pool", "weights", "page_table", "lengths", "to_table", "kept")] + \
-               [(n, c_int) for n in ("num_seqs", "hkv", "num_pages", "max_pages", "to_pages", "page_size", "row_bytes", "scale_bytes", "keep", "first", "recent")]
+               [(n, c_int) for n in ("num_seqs", "hkv", "num_pages", "max_pages", "to_pages", "page_size", "page_shift", "row_bytes", "scale_bytes", "keep", "first", "recent")]
 
 
 def _fp4_geometry(kv_layer: torch.Tensor, meta: StepMeta, scales: torch.Tensor) -> int:
@@ -784,8 +784,8 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
 def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep: int, first: int = 0, recent: int = 0) -> torch.Tensor:
     """See :func:`ops.kv_evict`."""
     row, sf = ref_ops.evict_geometry(kv_layer, weights, page_table, lengths, to_table, keep, first, recent)
-    if not (kv_layer.is_contiguous() and weights.is_contiguous()) or kv_layer.data_ptr() % 16 or row % 16 or sf % 4:
-        raise ValueError("kv_evict: a contiguous layer that starts on 16 bytes, rows of a multiple of 16 bytes, contiguous weights")
+    if not (kv_layer.is_contiguous() and weights.is_contiguous()) or (kv_layer.data_ptr() | weights.data_ptr()) % 16 or row % 16 or sf % 4:
+        raise ValueError("kv_evict: a contiguous layer that starts on 16 bytes, rows of a multiple of 16 bytes, contiguous weights that start on 16 bytes")
     if any(v.device != kv_layer.device for v in (weights, page_table, lengths, to_table)):
         raise ValueError("kv_evict: all tensors on one device")
     pages, _, hkv, psz = kv_layer.shape[:4]
@@ -793,7 +793,7 @@ def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep: int, first:
     kept = torch.empty(n, hkv, keep, dtype=torch.int32, device=kv_layer.device)
     page_table, lengths, to_table = (v.to(torch.int32).contiguous() for v in (page_table, lengths, to_table))
     p = EvictParams(*[_p(v).value for v in (kv_layer, weights, page_table, lengths, to_table, kept)], n, hkv, pages, page_table.shape[1], to_table.shape[1],
-                    psz, row, sf, keep, first, recent)
+                    psz, psz.bit_length() - 1 if psz & (psz - 1) == 0 else -1, row, sf, keep, first, recent)
     _check(lib().telb_kv_evict(ctypes.byref(p), _stream()), "kv_evict", 2)
     return kept
 
