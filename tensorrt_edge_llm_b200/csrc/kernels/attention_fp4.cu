@@ -28,6 +28,7 @@ struct Fp4AttnParams {
 };
 
 constexpr int kFp4Warps = 4, kFp4Tile = 32;               // warps of a CTA; keys that a warp takes at a time
+constexpr int kFp4WeightSmem = 200 << 10;
 constexpr float kRefStart = -1e30f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -108,34 +109,38 @@ struct KeyTile {
             }
         }
     }
-    template <int NT>
-    __device__ __forceinline__ void scores(const uint32_t (&b)[NT][D / 16][2], float (&acc)[NT][4]) const {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+    // A operands: of word j, [0..3] of the step over its features 0..3 of every lane, [4..7] of the step over its features 4..7.
+    __device__ __forceinline__ void operands(uint32_t (&a)[D / 32][8]) const {
         uint32_t two[2][(D + 127) / 128];
 #pragma unroll
         for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int i = 0; i < (D + 127) / 128; ++i) two[r][i] = e4m3x2_to_half(s[r][i]);
 #pragma unroll
-        for (int j2 = 0; j2 < D / 32; ++j2) {                                   // a word: eight features, two steps
-            uint32_t a[2][4], sc[2];
+        for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                e2m1x8_to_half(w[r][j2], a[r][0], a[r][1], a[r][2], a[r][3]);
-                sc[r] = __byte_perm(two[r][j2 / 4], 0u, (j2 / 2) % 2 ? 0x3232 : 0x1010);      // the blocks of 16 features: two words each
+                e2m1x8_to_half(w[r][j], a[j][r], a[j][2 + r], a[j][4 + r], a[j][6 + r]);
+                const uint32_t sc = __byte_perm(two[r][j / 4], 0u, (j / 2) % 2 ? 0x3232 : 0x1010);       // blocks of 16 features: two words each
 #pragma unroll
-                for (int i = 0; i < 4; ++i) a[r][i] = hmul2u(a[r][i], sc[r]);
+                for (int i = 0; i < 4; ++i) a[j][2 * i + r] = hmul2u(a[j][2 * i + r], sc);
             }
+    }
+    template <int NT>
+    __device__ __forceinline__ void scores(const uint32_t (&b)[NT][D / 16][2], float (&acc)[NT][4]) const {
+        uint32_t a[D / 32][8];
+        operands(a);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const uint32_t lo[4] = {a[0][0], a[1][0], a[0][1], a[1][1]}, hi[4] = {a[0][2], a[1][2], a[0][3], a[1][3]};
-                mma_f16(acc[n], lo, b[n][2 * j2][0], b[n][2 * j2][1]);
-                mma_f16(acc[n], hi, b[n][2 * j2 + 1][0], b[n][2 * j2 + 1][1]);
+                mma_f16(acc[n], *reinterpret_cast<const uint32_t(*)[4]>(&a[j][0]), b[n][2 * j][0], b[n][2 * j][1]);
+                mma_f16(acc[n], *reinterpret_cast<const uint32_t(*)[4]>(&a[j][4]), b[n][2 * j + 1][0], b[n][2 * j + 1][1]);
             }
-        }
     }
 };
 
@@ -269,10 +274,11 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// The tiles of a warp on their way into its own ring in shared memory.  A stage: key codes [32][D/2], value codes, key scales [32][D/16], value scales.
-template <int D>
+// The tiles of a warp on their way into its own ring in shared memory.  A stage: key codes [32][D/2], value codes, key scales [32][D/16], value scales; with one
+// plane the keys' alone.
+template <int D, int kPlanes = 2>
 struct Fp4Ring {
-    static constexpr int kStages = 3, kCodes = kFp4Tile * D / 2, kScales = kFp4Tile * D / 16, kBytes = 2 * (kCodes + kScales);
+    static constexpr int kStages = 3, kCodes = kFp4Tile * D / 2, kScales = kFp4Tile * D / 16, kBytes = kPlanes * (kCodes + kScales);
     const uint8_t* base;                                                         // the head's keys in page 0
     const int* table;
     size_t page_bytes, value_at;
@@ -325,16 +331,18 @@ struct Fp4Ring {
             for (int i = 0; i < kHalf / 512; ++i) {
                 const int o = i * 512 + lane * 16;
                 cp_async16(dst + o, k0 + (size_t)at * (D / 2) + o, n0);
-                cp_async16(dst + kCodes + o, k0 + value_at + (size_t)at * (D / 2) + o, n0);
                 cp_async16(dst + kHalf + o, k1 + (size_t)at1 * (D / 2) + o, n1);
-                cp_async16(dst + kCodes + kHalf + o, k1 + value_at + (size_t)at1 * (D / 2) + o, n1);
+                if constexpr (kPlanes == 2) {
+                    cp_async16(dst + kCodes + o, k0 + value_at + (size_t)at * (D / 2) + o, n0);
+                    cp_async16(dst + kCodes + kHalf + o, k1 + value_at + (size_t)at1 * (D / 2) + o, n1);
+                }
             }
             constexpr int kPieces = D / 16;                                       // of 16 bytes, in 16 rows of scales
 #pragma unroll
-            for (int i = lane; i < 4 * kPieces; i += 32) {
+            for (int i = lane; i < 2 * kPlanes * kPieces; i += 32) {
                 const int v = i / (2 * kPieces), h = i / kPieces % 2, o = i % kPieces * 16;
                 const uint8_t* src = (h ? k1 : k0) + (v ? value_at : 0) + ((size_t)(D / 2) << page_shift) + (size_t)(h ? at1 : at) * (D / 16) + o;
-                cp_async16(dst + 2 * kCodes + v * kScales + h * (kScales / 2) + o, src, h ? n1 : n0);
+                cp_async16(dst + kPlanes * kCodes + v * kScales + h * (kScales / 2) + o, src, h ? n1 : n0);
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -629,75 +637,131 @@ __global__ void __launch_bounds__(128) attention_fp4_merge_kernel(const Fp4AttnP
 }
 
 // Accumulated attention weights: weights[page, head, slot] = decay * weights + the sum over the step's rows and the group's heads of
-// exp2(score - top) / sum, for keys that some row sees; the step's own keys start from zero.  A warp owns its keys, so the sum has one order.
+// exp2(score - top) / sum, for keys that some row sees; the step's own keys start from zero.  The scores are made again: that reads the keys, half of what
+// the step has read, where keeping them would write and read 4 bytes for each (key, column).  A CTA takes a part of the line of all (sequence, KV
+// head, tile); the queries of its item stand in shared memory as the operands that the products take.  A warp owns its keys, so that every sum has one order.
 template <typename T, int D>
-__global__ void __launch_bounds__(kFp4Warps * 32) attention_fp4_weights_kernel(const Fp4AttnParams p) {
+__global__ void __launch_bounds__(kFp4Warps * 32, D == 256 ? 2 : 3) attention_fp4_weights_kernel(const Fp4AttnParams p) {
     pdl_prologue();
-    const int seq = blockIdx.z, kvh = blockIdx.y;
+    using Ring = Fp4Ring<D, 1>;
+    constexpr int kAll = 1 << 24, kOperand = D * 16;                             // columns of an item: all; bytes of 8 columns' operands
+    extern __shared__ __align__(16) uint8_t smem[];                              // rings, operands [chunks][D/32][32 lanes] uint4, columns [chunks][8] float4
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = p.hq / p.hkv, ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
-    if (columns == 0) return;
-    const int q0 = p.q_start[seq];
-    const int* table = p.page_table + (size_t)seq * p.max_pages;
-    const size_t slab = fp4_slab_bytes(p.page_size, D);
-    const int first = p.window > 0 ? max(0, past + 1 - p.window) : 0, end = past + ql;
-    const int tile0 = first / kFp4Tile, tiles = (end + kFp4Tile - 1) / kFp4Tile - tile0;
-    const int t_begin = tile0 + (int)((long long)tiles * blockIdx.x / gridDim.x), t_end = tile0 + (int)((long long)tiles * (blockIdx.x + 1) / gridDim.x);
+    const int group = p.hq / p.hkv, most_chunks = (p.max_q_len * group + 7) / 8;
+    uint8_t* operands = smem + kFp4Warps * Ring::kStages * Ring::kBytes;
+    float4* params = reinterpret_cast<float4*>(operands + (size_t)most_chunks * kOperand);       // factor, top, 1 / sum, limit (as an int)
+    const Fp4Line line = fp4_line(p, kAll, lane);
+    int at = blockIdx.x * line.per;
+    const int stop = min(line.total, at + line.per);
+    if (at >= stop) return;
+    int seq_start = 0, seq = fp4_locate(p, kAll, lane, at, seq_start);
     const float base = p.scale * 1.4426950408889634f * p.scales[0];
-    for (int tile = t_begin + warp; tile < t_end; tile += kFp4Warps) {
-        const int kb = tile * kFp4Tile;
-        KeyTile<D> kt[2];
-        int pages[2];
-        float given[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            const int k0 = kb + 16 * m, lp = k0 / p.page_size, at = k0 - lp * p.page_size;
-            pages[m] = k0 < end && lp < p.max_pages ? table[lp] : -1;
-            if ((unsigned)pages[m] >= (unsigned)p.num_pages) pages[m] = -1;
-            const uint8_t* ks = p.pool + ((size_t)max(pages[m], 0) * 2 * p.hkv + kvh) * slab;
-            kt[m].load(ks + (size_t)at * (D / 2), ks + (size_t)p.page_size * (D / 2) + (size_t)at * (D / 16), g, t);
+    const uint32_t ring_at = smem_u32(smem) + warp * Ring::kStages * Ring::kBytes;
+    const uint8_t* ring_ptr = smem + warp * Ring::kStages * Ring::kBytes;
+    while (at < stop) {
+        const int ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
+        const int tiles = fp4_tiles(past, ql, p.window);
+        if (at >= seq_start + tiles * p.hkv) {
+            seq_start += tiles * p.hkv;
+            ++seq;
+            continue;
         }
-        for (int c0 = 0; c0 < columns; c0 += 8) {
-            uint32_t qb[1][D / 16][2];
-            const int c = c0 + g, r = c / group, h = kvh * group + c - r * group;
-            const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + ((size_t)(q0 + r) * p.hq + h) * D + t * (D / 4), c < columns, qb[0]);
-            float factor[2], top[2], inv[2];
-            int low[2], high[2];
+        const int kvh = (at - seq_start) / tiles, off = (at - seq_start) - kvh * tiles;
+        const int count = min(tiles - off, stop - at);
+        const int tile0 = fp4_first_tile(past, p.window) + off, tile1 = tile0 + count;
+        const int q0 = p.q_start[seq], chunks = min((columns + 7) / 8, most_chunks);
+        const int first = p.window > 0 ? max(0, past + 1 - p.window) : 0, end = past + ql;
+        const int all_low = p.window > 0 ? max(0, end - p.window) : 0, all_high = past + 1;       // visible to every row
+
+        Ring ring;
+        ring.begin(p, seq, kvh, end, ring_at, lane);
+        uint32_t flags = 0;
+        int next = tile0 + warp;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                factor[i] = base * __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
-                const int cc = c0 + 2 * t + i, rr = cc / group;
-                const ColumnLimits lim(cc, columns, group, past, p.window);
-                low[i] = lim.low;
-                high[i] = lim.high;
-                const float2 st = cc < columns ? *reinterpret_cast<const float2*>(p.stat + ((size_t)(q0 + rr) * p.hq + kvh * group + cc - rr * group) * 2)
-                                               : make_float2(0.f, 0.f);
-                top[i] = st.x;
-                inv[i] = st.y;
+        for (int s = 0; s < Ring::kStages - 1; ++s, next += kFp4Warps) flags |= ring.load(s, next, next < tile1) << (2 * s);
+        for (int ch = warp; ch < chunks; ch += kFp4Warps) {
+            const int c = ch * 8 + g, r = c / group, h = kvh * group + c - r * group;
+            uint32_t qb[D / 16][2];
+            const size_t row = (size_t)(q0 + r) * p.hq + h;
+            const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + row * D + t * (D / 4), c < columns, qb);
+#pragma unroll
+            for (int j = 0; j < D / 32; ++j)
+                *reinterpret_cast<uint4*>(operands + (size_t)ch * kOperand + (j * 32 + lane) * 16) = make_uint4(qb[2 * j][0], qb[2 * j][1], qb[2 * j + 1][0], qb[2 * j + 1][1]);
+            if (t == 0) {
+                const float2 st = c < columns ? *reinterpret_cast<const float2*>(p.stat + row * 2) : make_float2(0.f, 0.f);
+                params[ch * 8 + g] = make_float4(base * up, st.x, st.y, __int_as_float(c < columns ? past + r + 1 : 0));
             }
+        }
+        __syncthreads();
+        int stage = 0;
+        for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
+            const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
+            __syncwarp();
+            const uint32_t more = ring.load(ahead, next, next < tile1);
+            flags = (flags & ~(3u << (2 * ahead))) | (more << (2 * ahead));
+            next += kFp4Warps;
+            const uint32_t there = (flags >> (2 * stage)) & 3u;
+            const int kb = tile * kFp4Tile;
+            // a lane's own key: half t / 2, row g or g + 8 of it
+            const int mine = kb + 16 * (t >> 1) + key_place(g) + 8 * (t & 1);
+            const int page = ((there >> (t >> 1)) & 1u) && mine >= first && mine < end ? ring.table[mine >> p.page_shift] : -1;
+            float* w = page >= 0 ? p.weights + ((size_t)page * p.hkv + kvh) * p.page_size + (mine & (p.page_size - 1)) : nullptr;
+            const float old = w && mine < past ? p.decay * *w : 0.f;
+            asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
+            __syncwarp();
+            const uint8_t* st = ring_ptr + stage * Ring::kBytes;
+            KeyTile<D> kt[2];
+            uint32_t a[2][D / 32][8];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                float s[1][4];
-                kt[m].template scores<1>(qb, s);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1);
-                    if (key >= low[i & 1] && key < high[i & 1]) given[m][i >> 1] += exp2_approx(fmaf(s[0][i], factor[i & 1], -top[i & 1])) * inv[i & 1];
-                }
+                kt[m].load(st + m * (16 * D / 2), st + Ring::kCodes + m * D, g, t);
+                kt[m].operands(a[m]);
             }
+            const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there == 3u;
+            float given[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+            for (int ch = 0; ch < chunks; ++ch) {
+                float s[2][4];
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[m][i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < D / 32; ++j) {
+                    const uint4 b = *reinterpret_cast<const uint4*>(operands + (size_t)ch * kOperand + (j * 32 + lane) * 16);
+#pragma unroll
+                    for (int m = 0; m < 2; ++m) {
+                        mma_f16(s[m], *reinterpret_cast<const uint32_t(*)[4]>(&a[m][j][0]), b.x, b.y);
+                        mma_f16(s[m], *reinterpret_cast<const uint32_t(*)[4]>(&a[m][j][4]), b.z, b.w);
+                    }
+                }
+                const float4 col[2] = {params[ch * 8 + 2 * t], params[ch * 8 + 2 * t + 1]};
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float4 c = col[i & 1];
+                        float e = exp2_approx(fmaf(s[m][i], c.x, -c.y));
+                        if (!open) {
+                            const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1), high = __float_as_int(c.w);
+                            if (key >= high || (p.window > 0 && key < high - p.window)) e = 0.f;
+                        }
+                        given[m][i >> 1] = fmaf(e, c.z, given[m][i >> 1]);
+                    }
+            }
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 1);
+                    given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 2);
+                }
+            const float sum = t & 2 ? (t & 1 ? given[1][1] : given[1][0]) : (t & 1 ? given[0][1] : given[0][0]);
+            if (w) *w = old + sum;
+            stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
         }
-#pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 1);
-                given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 2);
-                const int key = kb + 16 * m + key_place(g) + 8 * r;
-                if (t == 0 && pages[m] >= 0 && key >= first && key < end) {
-                    float* w = p.weights + ((size_t)pages[m] * p.hkv + kvh) * p.page_size + key % p.page_size;
-                    *w = (key >= past ? 0.f : p.decay * *w) + given[m][r];
-                }
-            }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        at += count;
+        if (at < stop) __syncthreads();                                          // the operands make room for the next item's
     }
 }
 
@@ -720,12 +784,23 @@ int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t st
 }
 
 template <typename T, int D>
-int launch_attention_fp4(const Fp4AttnParams& p, int weight_splits, cudaStream_t stream) {
+int launch_attention_fp4(const Fp4AttnParams& p, int weight_ctas, cudaStream_t stream) {
     const int columns = p.max_q_len * (p.hq / p.hkv);
     constexpr int kMost = D == 256 ? 1 : 2;
     const int rc = columns <= 8 ? launch_attention_fp4_nt<T, D, 1>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost>(p, columns, stream);
     if (rc || !p.weights) return rc;
-    TELB_LAUNCH("attention_fp4_weights_kernel", (attention_fp4_weights_kernel<T, D>), dim3(weight_splits, p.hkv, p.num_seqs), dim3(kFp4Warps * 32), 0, stream, p);
+    using Ring = Fp4Ring<D, 1>;
+    const int chunks = (columns + 7) / 8, smem = kFp4Warps * Ring::kStages * Ring::kBytes + chunks * (D * 16 + 128);
+    if (smem > kFp4WeightSmem) return fail("telb_paged_attention_fp4: too many rows x heads of a KV head for accumulated weights");
+    static bool configured[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(attention_fp4_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp4WeightSmem);
+        if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4_weights)", e);
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    TELB_LAUNCH("attention_fp4_weights_kernel", (attention_fp4_weights_kernel<T, D>), dim3(weight_ctas), dim3(kFp4Warps * 32), smem, stream, p);
     return 0;
 }
 
@@ -742,9 +817,9 @@ extern "C" int telb_attention_fp4_ctas(int columns, int d) {
 }
 
 // part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C of telb_attention_fp4_columns, max_items = KV heads x chunks of the longest
-// sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and `weight_splits` parts of every
-// sequence's keys run at once.
-extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int weight_splits, int is_bf16, cudaStream_t stream) {
+// sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and its keys are cut
+// into `weight_ctas` parts.
+extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int weight_ctas, int is_bf16, cudaStream_t stream) {
     const Fp4AttnParams& p = *params;
     if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
     if (d != 64 && d != 128 && d != 256) return fail("telb_paged_attention_fp4: head_dim must be 64, 128 or 256");
@@ -752,13 +827,13 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (p.hkv <= 0 || p.hq % p.hkv) return fail("telb_paged_attention_fp4: query heads must be a multiple of the KV heads");
     if (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans) return fail("telb_paged_attention_fp4: no room for the parts");
     if (p.num_seqs > 65535) return fail("telb_paged_attention_fp4: more than 65535 sequences");
-    if (p.weights && (!p.stat || weight_splits < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
+    if (p.weights && (!p.stat || weight_ctas < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
     if (is_bf16) {
-        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, weight_splits, stream);
-        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, weight_splits, stream);
-        return launch_attention_fp4<__nv_bfloat16, 256>(p, weight_splits, stream);
+        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, weight_ctas, stream);
+        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, weight_ctas, stream);
+        return launch_attention_fp4<__nv_bfloat16, 256>(p, weight_ctas, stream);
     }
-    if (d == 128) return launch_attention_fp4<__half, 128>(p, weight_splits, stream);
-    if (d == 64) return launch_attention_fp4<__half, 64>(p, weight_splits, stream);
-    return launch_attention_fp4<__half, 256>(p, weight_splits, stream);
+    if (d == 128) return launch_attention_fp4<__half, 128>(p, weight_ctas, stream);
+    if (d == 64) return launch_attention_fp4<__half, 64>(p, weight_ctas, stream);
+    return launch_attention_fp4<__half, 256>(p, weight_ctas, stream);
 }

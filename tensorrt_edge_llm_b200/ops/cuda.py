@@ -763,8 +763,8 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     n, L = meta.num_seqs, lib()
     cols = L.telb_attention_fp4_columns(c_int(columns), c_int(d))
     items = hkv * -(-columns // cols)
+    tiles = n * items * (-(-min(meta.max_seq_len, window + meta.max_q_len if window else meta.max_seq_len) // 32) + 1)
     if ctas is None:            # as many as run at once, of four tiles of 32 keys or more
-        tiles = n * items * (-(-min(meta.max_seq_len, window + meta.max_q_len if window else meta.max_seq_len) // 32) + 1)
         ctas = max(1, min(L.telb_attention_fp4_ctas(c_int(columns), c_int(d)), tiles // 4))
     # parts of outputs, their references and sums, (first, last) CTA of every item, softmax statistics of the rows
     room = [2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items, 2 * t * hq if weights is not None else 0]
@@ -775,8 +775,8 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     p = Fp4AttnParams(ptr(q), ptr(kv_layer), ptr(out), part_o, part_ml, stat, *[ptr(v) for v in (meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
                       spans, n, t, meta.max_q_len, kv_layer.shape[0], meta.page_table.shape[1], meta.page_size, meta.page_size.bit_length() - 1, hq, hkv, window, ctas,
                       items, scale, decay)
-    splits = max(1, min(4 * 148 // (n * hkv), -(-meta.max_seq_len // 128), 64))
-    _check(L.telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(splits), c_int(is_bf16), _stream()), "paged_attention_fp4", 2 + (weights is not None))
+    weight_ctas = max(1, min(2 * 148 if columns > 64 else 3 * 148, tiles // 4))
+    _check(L.telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(weight_ctas), c_int(is_bf16), _stream()), "paged_attention_fp4", 2 + (weights is not None))
     return out
 
 
