@@ -23,7 +23,7 @@ struct Fp4AttnParams {
     const float *scales, *sinks;
     float* weights;
     int2* spans;
-    int num_seqs, tokens, max_q_len, num_pages, max_pages, page_size, page_shift, hq, hkv, window, ctas, max_items;
+    int num_seqs, tokens, max_q_len, num_pages, max_pages, page_size, page_shift, hq, hkv, window, ctas, ranks, max_items;
     float scale, decay;
 };
 
@@ -270,6 +270,9 @@ __device__ __forceinline__ int fp4_locate(const Fp4AttnParams& p, int cols, int 
     return -1;
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {       // bytes 0: zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -315,34 +318,42 @@ struct Fp4Ring {
     __device__ __forceinline__ uint32_t load(int stage, int tile, bool real) {
         uint32_t there = 0;
         if (real) {
-            const int kb = tile * kFp4Tile, at = kb & ((1 << page_shift) - 1);
-            const uint32_t dst = smem + stage * kBytes;
-            int page[2];
-            page[0] = page_of(kb);
-            if (page_shift >= 5) page[1] = kb + 16 < end ? page[0] : -1;
-            else page[1] = page_of(kb + 16);
-            there = (page[0] >= 0 ? 1u : 0u) | (page[1] >= 0 ? 2u : 0u);
-            const int at1 = page_shift >= 5 ? at + 16 : 0;
-            const uint8_t* k0 = base + (size_t)max(page[0], 0) * page_bytes;
-            const uint8_t* k1 = base + (size_t)max(page[1], 0) * page_bytes;
-            const uint32_t n0 = page[0] >= 0 ? 16u : 0u, n1 = page[1] >= 0 ? 16u : 0u;
+            const int kb = tile * kFp4Tile;
+            const uint32_t dst = smem + stage * kBytes + lane * 16;
             constexpr int kHalf = 16 * D / 2;                                     // bytes of 16 rows of codes
-#pragma unroll
-            for (int i = 0; i < kHalf / 512; ++i) {
-                const int o = i * 512 + lane * 16;
-                cp_async16(dst + o, k0 + (size_t)at * (D / 2) + o, n0);
-                cp_async16(dst + kHalf + o, k1 + (size_t)at1 * (D / 2) + o, n1);
-                if constexpr (kPlanes == 2) {
-                    cp_async16(dst + kCodes + o, k0 + value_at + (size_t)at * (D / 2) + o, n0);
-                    cp_async16(dst + kCodes + kHalf + o, k1 + value_at + (size_t)at1 * (D / 2) + o, n1);
-                }
-            }
             constexpr int kPieces = D / 16;                                       // of 16 bytes, in 16 rows of scales
+            const int page0 = page_of(kb);
+            if (page_shift >= 5 && page0 >= 0 && kb + 16 < end) {                 // the whole tile lies in one page
+                const int at = kb & ((1 << page_shift) - 1);
+                const uint8_t* k = base + (size_t)page0 * page_bytes;
+                const uint8_t* c = k + at * (D / 2) + lane * 16;
 #pragma unroll
-            for (int i = lane; i < 2 * kPlanes * kPieces; i += 32) {
-                const int v = i / (2 * kPieces), h = i / kPieces % 2, o = i % kPieces * 16;
-                const uint8_t* src = (h ? k1 : k0) + (v ? value_at : 0) + ((size_t)(D / 2) << page_shift) + (size_t)(h ? at1 : at) * (D / 16) + o;
-                cp_async16(dst + kPlanes * kCodes + v * kScales + h * (kScales / 2) + o, src, h ? n1 : n0);
+                for (int i = 0; i < 2 * kHalf / 512; ++i) cp_async16(dst + i * 512, c + i * 512);
+                if constexpr (kPlanes == 2) {
+#pragma unroll
+                    for (int i = 0; i < 2 * kHalf / 512; ++i) cp_async16(dst + kCodes + i * 512, c + value_at + i * 512);
+                }
+                const uint8_t* f = k + ((size_t)(D / 2) << page_shift) + at * (D / 16);
+#pragma unroll
+                for (int i = lane; i < 2 * kPlanes * kPieces; i += 32)
+                    cp_async16(dst - lane * 16 + kPlanes * kCodes + i * 16, f + (i >= 2 * kPieces ? value_at - 2 * kPieces * 16 : 0) + i * 16);
+                there = 3u;
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int key = kb + 16 * h, page = page_of(key), at = key & ((1 << page_shift) - 1);
+                    const uint8_t* k = base + (size_t)max(page, 0) * page_bytes;
+                    const uint32_t n = page >= 0 ? 16u : 0u;
+                    if (page >= 0) there |= 1u << h;
+#pragma unroll
+                    for (int v = 0; v < kPlanes; ++v) {
+#pragma unroll
+                        for (int i = 0; i < kHalf / 512; ++i)
+                            cp_async16(dst + v * kCodes + h * kHalf + i * 512, k + v * value_at + (size_t)at * (D / 2) + i * 512 + lane * 16, n);
+                        if (lane < kPieces)
+                            cp_async16(dst + kPlanes * kCodes + v * kScales + h * (kScales / 2), k + v * value_at + ((size_t)(D / 2) << page_shift) + (size_t)at * (D / 16) + lane * 16, n);
+                    }
+                }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -356,6 +367,275 @@ struct Fp4Occupancy {
     static constexpr int kCtas = D * NT <= 128 ? 4 : D * NT <= 256 && D < 256 ? 3 : 2;
 };
 
+// One item's tiles [tile0, tile1), every fourth of them this warp's: outputs of the warp over its keys, the references of their probabilities and their sums.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kvh, int chunk, int q0, int past, int columns, int tile0, int tile1, uint32_t ring_at,
+                                         const uint8_t* ring_ptr, float base, float (&o)[NT][D / 16][4], float (&ref)[NT][2], float (&sum)[NT][2]) {
+    constexpr int C = 8 * NT;
+    using Ring = Fp4Ring<D>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = p.hq / p.hkv;
+    const int r_first = chunk * C / group, r_last = (min(columns, chunk * C + C) - 1) / group;
+    const int end = past + r_last + 1;
+    const int all_low = p.window > 0 ? max(0, past + r_last + 1 - p.window) : 0, all_high = past + r_first + 1;      // visible to every column
+    Ring ring;
+    ring.begin(p, seq, kvh, end, ring_at, lane);
+    uint32_t flags = 0;                                                      // two bits a stage
+    int next = tile0 + warp;
+#pragma unroll
+    for (int s = 0; s < Ring::kStages - 1; ++s, next += kFp4Warps) flags |= ring.load(s, next, next < tile1) << (2 * s);
+
+    uint32_t qb[NT][D / 16][2];
+    float factor[NT][2];
+    int low[NT][2], high[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int c = chunk * C + n * 8 + g;
+        const int r = c / group, h = kvh * group + c - r * group;
+        const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + ((size_t)(q0 + r) * p.hq + h) * D + t * (D / 4), c < columns, qb[n]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            factor[n][i] = base * __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
+            const ColumnLimits lim(chunk * C + n * 8 + 2 * t + i, columns, group, past, p.window);
+            low[n][i] = lim.low;
+            high[n][i] = lim.high;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
+        ref[n][0] = ref[n][1] = kRefStart;
+        sum[n][0] = sum[n][1] = 0.f;
+    }
+    int stage = 0;
+    for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
+        const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
+        __syncwarp();                                                        // the stage to be filled has been read by all lanes
+        const uint32_t more = ring.load(ahead, next, next < tile1);
+        flags = (flags & ~(3u << (2 * ahead))) | (more << (2 * ahead));
+        next += kFp4Warps;
+        asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
+        __syncwarp();
+        const uint8_t* st = ring_ptr + stage * Ring::kBytes;
+        const uint32_t there = (flags >> (2 * stage)) & 3u;
+        const int kb = tile * kFp4Tile;
+        float s[2][NT][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            KeyTile<D> kt;
+            kt.load(st + m * (16 * D / 2), st + 2 * Ring::kCodes + m * D, g, t);
+            kt.template scores<NT>(qb, s[m]);
+        }
+        const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there == 3u;
+        float x[2][NT][4];
+        auto shifted = [&]() {
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[m][n][i] = fmaf(s[m][n][i], factor[n][i & 1], -ref[n][i & 1]);
+            if (!open) {
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1);
+                            if (!((there >> m) & 1u) || key < low[n][i & 1] || key >= high[n][i & 1]) x[m][n][i] = -INFINITY;
+                        }
+            }
+        };
+        shifted();
+        float most = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(x[0][n][i], x[1][n][i]));
+        if (__any_sync(0xffffffffu, most > 15.f)) {
+            float up[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    // scores themselves: x has lost them where the reference is the first one
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int m = 0; m < 2; ++m)
+#pragma unroll
+                        for (int i = c; i < 4; i += 2)
+                            if (x[m][n][i] > -INFINITY) top = fmaxf(top, s[m][n][i] * factor[n][c]);
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float next_ref = top - ref[n][c] > 15.f ? top - 8.f : ref[n][c];
+                    up[n][c] = exp2_approx(ref[n][c] - next_ref);
+                    ref[n][c] = next_ref;
+                    sum[n][c] *= up[n][c];
+                }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[n][i][k] *= up[n][k & 1];
+            shifted();
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    x[m][n][i] = exp2_approx(x[m][n][i]);
+                    sum[n][i & 1] += x[m][n][i];
+                }
+                pb[n][0] = transpose8(Cvt<__half>::pack2(x[m][n][0], x[m][n][1]));
+                pb[n][1] = transpose8(Cvt<__half>::pack2(x[m][n][2], x[m][n][3]));
+            }
+            ValueTile<D> vt;
+            vt.load(st + Ring::kCodes + m * (16 * D / 2), st + 2 * Ring::kCodes + Ring::kScales + m * D, g, t);
+            if (!open) vt.clear(t, end - kb - 16 * m);
+            vt.template add<NT>(pb, o);
+        }
+        stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// The warps' results joined where their rings were: smem [warps][C][D] outputs and [warps][C][2]; `use(column, first feature, four outputs, reference, sum)`.
+template <int D, int NT, typename Use>
+__device__ __forceinline__ void fp4_join(float* smem_f, int live, float (&o)[NT][D / 16][4], float (&ref)[NT][2], float (&sum)[NT][2], Use use) {
+    constexpr int C = 8 * NT;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float* so = smem_f + warp * C * D;
+    float* sml = smem_f + kFp4Warps * C * D;
+    __syncthreads();                                                             // the rings have been read
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], d);
+            const int col = n * 8 + 2 * t + c;
+            if (col >= live) continue;
+            if (g == 0) *reinterpret_cast<float2*>(sml + (warp * C + col) * 2) = make_float2(ref[n][c], sum[n][c]);
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(so + col * D + g * (D / 8) + 2 * i) = make_float2(o[n][i][c], o[n][i][c + 2]);
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
+        const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
+        float2 ml[kFp4Warps];
+        float top = kRefStart, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kFp4Warps; ++w) {
+            ml[w] = *reinterpret_cast<const float2*>(sml + (w * C + col) * 2);
+            top = fmaxf(top, ml[w].x);
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kFp4Warps; ++w) {
+            const float f = exp2_approx(ml[w].x - top);
+            const float4 v = *reinterpret_cast<const float4*>(smem_f + (w * C + col) * D + d);
+            acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+            l += f * ml[w].y;
+        }
+        use(col, d, acc, top, l);
+    }
+}
+
+// Four outputs of a column whose keys have all been joined: the sink, the sum and the values' scale, then the one rounding.
+template <typename T, int D>
+__device__ __forceinline__ void fp4_finish(const Fp4AttnParams& p, size_t row, int h, int d, float4 acc, float top, float l) {
+    if (p.sinks) {
+        const float z = p.sinks[h] * 1.4426950408889634f, m = fmaxf(top, z), f = exp2_approx(top - m);
+        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+        l = l * f + exp2_approx(z - m);
+        top = m;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l, f = inv * p.scales[1];           // a row that sees nothing gives zeros
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + row * D + d) = make_uint2(Cvt<T>::pack2(acc.x * f, acc.y * f), Cvt<T>::pack2(acc.z * f, acc.w * f));
+    if (p.stat && d == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
+}
+
+__device__ __forceinline__ float4 cluster_load_f4(const void* at, uint32_t rank) {
+    uint32_t a;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(at)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void fp4_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Many items: a cluster per item, its CTAs take equal parts of the item's tiles and join their results through shared memory.
+// grid (CTAs of a cluster, items of a sequence, sequences)
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas)) attention_fp4_cluster_kernel(const Fp4AttnParams p) {
+    pdl_prologue();
+    constexpr int C = 8 * NT;
+    using Ring = Fp4Ring<D>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, ranks = gridDim.x, rank = blockIdx.x, seq = blockIdx.z;
+    const int chunk = blockIdx.y / p.hkv, kvh = blockIdx.y - chunk * p.hkv;
+    const int group = p.hq / p.hkv, ql = p.q_len[seq], past = p.past_len[seq], q0 = p.q_start[seq], columns = ql * group;
+    if (chunk * C >= columns) return;                                            // the whole cluster
+    const int first = fp4_first_tile(past, p.window), tiles = fp4_tiles(past, ql, p.window);
+    const int tile0 = first + tiles * rank / ranks, tile1 = first + tiles * (rank + 1) / ranks;
+    float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
+    fp4_keys<T, D, NT>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, smem_u32(smem) + warp * Ring::kStages * Ring::kBytes,
+                       smem + warp * Ring::kStages * Ring::kBytes, p.scale * 1.4426950408889634f * p.scales[0], o, ref, sum);
+    float* smem_f = reinterpret_cast<float*>(smem);
+    const int live = min(C, columns - chunk * C);
+    auto finish = [&](int col, int d, float4 acc, float top, float l) {
+        const int c = chunk * C + col, r = c / group, h = kvh * group + c - r * group;
+        fp4_finish<T, D>(p, (size_t)(q0 + r) * p.hq + h, h, d, acc, top, l);
+    };
+    if (ranks == 1) {
+        fp4_join<D, NT>(smem_f, live, o, ref, sum, finish);
+        return;
+    }
+    // the CTA's own results take the first warp's place (a thread reads what it replaces), references and sums lie behind all of them
+    float4* own_ml = reinterpret_cast<float4*>(smem_f + kFp4Warps * C * (D + 2));
+    fp4_join<D, NT>(smem_f, live, o, ref, sum, [&](int col, int d, float4 acc, float top, float l) {
+        *reinterpret_cast<float4*>(smem_f + col * D + d) = acc;
+        if (d == 0) own_ml[col] = make_float4(top, l, 0.f, 0.f);
+    });
+    fp4_cluster_sync();
+    for (int i = rank * blockDim.x + threadIdx.x; i < live * (D / 4); i += ranks * blockDim.x) {
+        const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
+        float top = kRefStart, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r0 = 0; r0 < ranks; r0 += 4) {
+            float4 ml[4], v[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                ml[r] = r0 + r < ranks ? cluster_load_f4(own_ml + col, r0 + r) : make_float4(kRefStart, 0.f, 0.f, 0.f);
+                v[r] = r0 + r < ranks ? cluster_load_f4(smem_f + col * D + d, r0 + r) : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            const float next = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), keep = exp2_approx(top - next);
+            acc.x *= keep, acc.y *= keep, acc.z *= keep, acc.w *= keep;
+            l *= keep;
+            top = next;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float f = exp2_approx(ml[r].x - top);
+                acc.x += f * v[r].x, acc.y += f * v[r].y, acc.z += f * v[r].z, acc.w += f * v[r].w;
+                l += f * ml[r].y;
+            }
+        }
+        finish(col, d, acc, top, l);
+    }
+    fp4_cluster_sync();                                                          // nobody leaves while its results may be read
+}
+
+// Few items and many keys: the line.
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas)) attention_fp4_kernel(const Fp4AttnParams p) {
     pdl_prologue();
@@ -370,7 +650,7 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
     const int stop = min(line.total, at + line.per);
     if (at >= stop) return;
     int seq_start = 0, seq = fp4_locate(p, C, lane, at, seq_start);
-    const float base = p.scale * 1.4426950408889634f * p.scales[0], v_scale = p.scales[1];
+    const float base = p.scale * 1.4426950408889634f * p.scales[0];
     const uint32_t ring_at = smem_u32(smem) + warp * Ring::kStages * Ring::kBytes;
     const uint8_t* ring_ptr = smem + warp * Ring::kStages * Ring::kBytes;
 
@@ -387,202 +667,32 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
         const int chunk = item / p.hkv, kvh = item - chunk * p.hkv;
         const int tile0 = fp4_first_tile(past, p.window) + off, tile1 = tile0 + count;
         const int q0 = p.q_start[seq];
-        const int r_first = chunk * C / group, r_last = (min(columns, chunk * C + C) - 1) / group;
-        const int end = past + r_last + 1;
-        const int all_low = p.window > 0 ? max(0, past + r_last + 1 - p.window) : 0, all_high = past + r_first + 1;      // visible to every column
-
-        Ring ring;
-        ring.begin(p, seq, kvh, end, ring_at, lane);
-        uint32_t flags = 0;                                                      // two bits a stage
-        int next = tile0 + warp;
-#pragma unroll
-        for (int s = 0; s < Ring::kStages - 1; ++s, next += kFp4Warps) flags |= ring.load(s, next, next < tile1) << (2 * s);
-
-        uint32_t qb[NT][D / 16][2];
-        float factor[NT][2];
-        int low[NT][2], high[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int c = chunk * C + n * 8 + g;
-            const int r = c / group, h = kvh * group + c - r * group;
-            const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + ((size_t)(q0 + r) * p.hq + h) * D + t * (D / 4), c < columns, qb[n]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                factor[n][i] = base * __shfl_sync(0xffffffffu, up, (2 * t + i) * 4);
-                const ColumnLimits lim(chunk * C + n * 8 + 2 * t + i, columns, group, past, p.window);
-                low[n][i] = lim.low;
-                high[n][i] = lim.high;
-            }
-        }
         float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-#pragma unroll
-            for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
-            ref[n][0] = ref[n][1] = kRefStart;
-            sum[n][0] = sum[n][1] = 0.f;
-        }
-        int stage = 0;
-        for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
-            const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
-            __syncwarp();                                                        // the stage to be filled has been read by all lanes
-            const uint32_t more = ring.load(ahead, next, next < tile1);
-            flags = (flags & ~(3u << (2 * ahead))) | (more << (2 * ahead));
-            next += kFp4Warps;
-            asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
-            __syncwarp();
-            const uint8_t* st = ring_ptr + stage * Ring::kBytes;
-            const uint32_t there = (flags >> (2 * stage)) & 3u;
-            const int kb = tile * kFp4Tile;
-            float s[2][NT][4];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                KeyTile<D> kt;
-                kt.load(st + m * (16 * D / 2), st + 2 * Ring::kCodes + m * D, g, t);
-                kt.template scores<NT>(qb, s[m]);
-            }
-            const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there == 3u;
-            float x[2][NT][4];
-            auto shifted = [&]() {
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[m][n][i] = fmaf(s[m][n][i], factor[n][i & 1], -ref[n][i & 1]);
-                if (!open) {
-#pragma unroll
-                    for (int m = 0; m < 2; ++m)
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1);
-                                if (!((there >> m) & 1u) || key < low[n][i & 1] || key >= high[n][i & 1]) x[m][n][i] = -INFINITY;
-                            }
-                }
-            };
-            shifted();
-            float most = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most = fmaxf(most, fmaxf(x[0][n][i], x[1][n][i]));
-            if (__any_sync(0xffffffffu, most > 15.f)) {
-                float up[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        // scores themselves: x has lost them where the reference is the first one
-                        float top = -INFINITY;
-#pragma unroll
-                        for (int m = 0; m < 2; ++m)
-#pragma unroll
-                            for (int i = c; i < 4; i += 2)
-                                if (x[m][n][i] > -INFINITY) top = fmaxf(top, s[m][n][i] * factor[n][c]);
-#pragma unroll
-                        for (int d = 4; d < 32; d *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        const float next_ref = top - ref[n][c] > 15.f ? top - 8.f : ref[n][c];
-                        up[n][c] = exp2_approx(ref[n][c] - next_ref);
-                        ref[n][c] = next_ref;
-                        sum[n][c] *= up[n][c];
-                    }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) o[n][i][k] *= up[n][k & 1];
-                shifted();
-            }
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                uint32_t pb[NT][2];
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        x[m][n][i] = exp2_approx(x[m][n][i]);
-                        sum[n][i & 1] += x[m][n][i];
-                    }
-                    pb[n][0] = transpose8(Cvt<__half>::pack2(x[m][n][0], x[m][n][1]));
-                    pb[n][1] = transpose8(Cvt<__half>::pack2(x[m][n][2], x[m][n][3]));
-                }
-                ValueTile<D> vt;
-                vt.load(st + Ring::kCodes + m * (16 * D / 2), st + 2 * Ring::kCodes + Ring::kScales + m * D, g, t);
-                if (!open) vt.clear(t, end - kb - 16 * m);
-                vt.template add<NT>(pb, o);
-            }
-            stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();                                                         // the rings have been read: their place takes the warps' results
-        float* so = smem_f + warp * C * D;
-        float* sml = smem_f + kFp4Warps * C * D;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-#pragma unroll
-                for (int d = 4; d < 32; d *= 2) sum[n][c] += __shfl_xor_sync(0xffffffffu, sum[n][c], d);
-                const int col = n * 8 + 2 * t + c;
-                if (g == 0) {
-                    sml[(warp * C + col) * 2] = ref[n][c];
-                    sml[(warp * C + col) * 2 + 1] = sum[n][c];
-                }
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i) *reinterpret_cast<float2*>(so + col * D + g * (D / 8) + 2 * i) = make_float2(o[n][i][c], o[n][i][c + 2]);
-            }
-        __syncthreads();
-        const int live = min(C, columns - chunk * C);
+        fp4_keys<T, D, NT>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, ring_at, ring_ptr, base, o, ref, sum);
         const bool whole = count == tiles;
         const size_t slot = (size_t)blockIdx.x * 2 + (off == 0);                 // parts: [0] what began in an earlier CTA, [1] what goes on in a later one
-        if (threadIdx.x == 0 && off == 0 && p.spans && item < p.max_items)
+        if (threadIdx.x == 0 && off == 0 && item < p.max_items)
             p.spans[(size_t)seq * p.max_items + item] = make_int2(blockIdx.x, (at + tiles - 1) / line.per);
-        for (int i = threadIdx.x; i < live * (D / 4); i += blockDim.x) {
-            const int col = i / (D / 4), d = (i - col * (D / 4)) * 4;
-            float top = kRefStart;
-#pragma unroll
-            for (int w = 0; w < kFp4Warps; ++w) top = fmaxf(top, sml[(w * C + col) * 2]);
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kFp4Warps; ++w) {
-                const float f = exp2_approx(sml[(w * C + col) * 2] - top);
-                const float4 v = *reinterpret_cast<const float4*>(smem_f + (w * C + col) * D + d);
-                acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
-                l += f * sml[(w * C + col) * 2 + 1];
-            }
+        fp4_join<D, NT>(smem_f, min(C, columns - chunk * C), o, ref, sum, [&](int col, int d, float4 acc, float top, float l) {
             if (!whole) {
                 *reinterpret_cast<float4*>(p.part_o + (slot * C + col) * D + d) = acc;
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C + col) * 2) = make_float2(top, l);
             } else {
                 const int c = chunk * C + col, r = c / group, h = kvh * group + c - r * group;
-                const size_t row = (size_t)(q0 + r) * p.hq + h;
-                if (p.sinks) {
-                    const float z = p.sinks[h] * 1.4426950408889634f, m = fmaxf(top, z), f = exp2_approx(top - m);
-                    acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-                    l = l * f + exp2_approx(z - m);
-                    top = m;
-                }
-                const float inv = l == 0.f ? 0.f : 1.f / l, f = inv * v_scale;                 // a row that sees nothing gives zeros
-                *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + row * D + d) = make_uint2(Cvt<T>::pack2(acc.x * f, acc.y * f), Cvt<T>::pack2(acc.z * f, acc.w * f));
-                if (p.stat && d == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
+                fp4_finish<T, D>(p, (size_t)(q0 + r) * p.hq + h, h, d, acc, top, l);
             }
-        }
+        });
         at += count;
         if (at < stop) __syncthreads();                                          // the next segment's tiles go where the results were
     }
 }
 
-// grid (items of a sequence, sequences, columns of an item): the parts of a column joined in their order, a fourth of them a warp.
+// grid (items of a sequence, sequences, columns of an item): the parts of a column joined in their order, every 16th of them a warp's.
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(128) attention_fp4_merge_kernel(const Fp4AttnParams p) {
-    constexpr int C = 8 * NT, E = D / 32;
-    __shared__ float s_o[4][D], s_ml[4][2];
+__global__ void __launch_bounds__(512) attention_fp4_merge_kernel(const Fp4AttnParams p) {
+    constexpr int C = 8 * NT, W = 16, E = D / 32;
+    __shared__ __align__(16) float s_o[W][D];
+    __shared__ float s_l[W], s_top[W];
     const int item = blockIdx.x, seq = blockIdx.y, col = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_prologue();
     const int group = p.hq / p.hkv, chunk = item / p.hkv, kvh = item - chunk * p.hkv;
@@ -591,49 +701,62 @@ __global__ void __launch_bounds__(128) attention_fp4_merge_kernel(const Fp4AttnP
     const int2 span = p.spans[(size_t)seq * p.max_items + item];
     if (span.x >= span.y) return;                                                // whole: written already
     const int parts = span.y - span.x + 1;
+    // the first part is slot 1 of its CTA, the others slot 0
+    auto slot_of = [&](int i) { return ((size_t)(span.x + i) * 2 + (i == 0)) * C + col; };
     float top = kRefStart, l = 0.f, acc[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) acc[i] = 0.f;
-    // the first part is slot 1 of its CTA, the others slot 0
-    auto slot_of = [&](int i) { return ((size_t)(span.x + i) * 2 + (i == 0)) * C + col; };
-    for (int i = warp + 4 * lane; i < parts; i += 128) top = fmaxf(top, p.part_ml[slot_of(i) * 2]);
+    for (int i0 = warp; i0 < parts; i0 += 8 * W) {
+        float2 ml[8];
+        float v[8][E], next = top;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll 4
-    for (int i = warp; i < parts; i += 4) {
-        const size_t s = slot_of(i);
-        const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + s * 2);
-        const float f = exp2_approx(ml.x - top);
-        l += f * ml.y;
-        const float* src = p.part_o + s * D + lane * E;
+        for (int u = 0; u < 8; ++u) {                                            // eight parts on their way
+            const int i = i0 + u * W;
+            ml[u] = make_float2(kRefStart, 0.f);
 #pragma unroll
-        for (int k = 0; k < E; ++k) acc[k] += f * src[k];
+            for (int k = 0; k < E; ++k) v[u][k] = 0.f;
+            if (i < parts) {
+                ml[u] = *reinterpret_cast<const float2*>(p.part_ml + slot_of(i) * 2);
+                const float* src = p.part_o + slot_of(i) * D + lane * E;
+                if constexpr (E == 2) *reinterpret_cast<float2*>(v[u]) = *reinterpret_cast<const float2*>(src);
+                else
+#pragma unroll
+                    for (int k = 0; k < E; k += 4) *reinterpret_cast<float4*>(v[u] + k) = *reinterpret_cast<const float4*>(src + k);
+            }
+            next = fmaxf(next, ml[u].x);
+        }
+        const float keep = exp2_approx(top - next);
+        top = next;
+        l *= keep;
+#pragma unroll
+        for (int k = 0; k < E; ++k) acc[k] *= keep;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float f = exp2_approx(ml[u].x - top);
+            l += f * ml[u].y;
+#pragma unroll
+            for (int k = 0; k < E; ++k) acc[k] += f * v[u][k];
+        }
     }
 #pragma unroll
     for (int k = 0; k < E; ++k) s_o[warp][lane * E + k] = acc[k];
-    if (lane == 0) s_ml[warp][0] = top, s_ml[warp][1] = l;
+    if (lane == 0) s_top[warp] = top, s_l[warp] = l;
     __syncthreads();
-    const int r = c / group, h = kvh * group + c - r * group;
-    const size_t row = (size_t)(p.q_start[seq] + r) * p.hq + h;
-    const float z = p.sinks ? p.sinks[h] * 1.4426950408889634f : kRefStart;
-    top = z;
+    if (threadIdx.x >= D / 4) return;
+    const int d = threadIdx.x * 4, r = c / group, h = kvh * group + c - r * group;
+    top = kRefStart;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, s_ml[w][0]);
-    l = p.sinks ? exp2_approx(z - top) : 0.f;
-    float f[4];
+    for (int w = 0; w < W; ++w) top = fmaxf(top, s_top[w]);
+    float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+    l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        f[w] = exp2_approx(s_ml[w][0] - top);
-        l += f[w] * s_ml[w][1];
+    for (int w = 0; w < W; ++w) {
+        const float f = exp2_approx(s_top[w] - top);
+        const float4 v = *reinterpret_cast<const float4*>(&s_o[w][d]);
+        out.x += f * v.x, out.y += f * v.y, out.z += f * v.z, out.w += f * v.w;
+        l += f * s_l[w];
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    for (int d = threadIdx.x * 2; d < D; d += 256) {
-        float v[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) v[k] = (f[0] * s_o[0][d + k] + f[1] * s_o[1][d + k] + f[2] * s_o[2][d + k] + f[3] * s_o[3][d + k]) * inv * p.scales[1];
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + row * D + d) = Cvt<T>::pack2(v[0], v[1]);
-    }
-    if (p.stat && threadIdx.x == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
+    fp4_finish<T, D>(p, (size_t)(p.q_start[seq] + r) * p.hq + h, h, d, out, top, l);
 }
 
 // Accumulated attention weights: weights[page, head, slot] = decay * weights + the sum over the step's rows and the group's heads of
@@ -769,17 +892,35 @@ template <typename T, int D, int NT>
 int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t stream) {
     constexpr int C = 8 * NT;
     constexpr int kSmem = kFp4Warps * Fp4Ring<D>::kStages * Fp4Ring<D>::kBytes;
-    static_assert(kSmem >= kFp4Warps * C * (D + 2) * 4, "the warps' results fit where their rings were");
+    static_assert(kSmem >= kFp4Warps * C * (D + 2) * 4 + C * 16, "the warps' results fit where their rings were");
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !configured[dev]) {
         cudaError_t e = cudaFuncSetAttribute(attention_fp4_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4)", e);
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
+    if (p.ranks > 0) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(p.ranks, p.max_items, p.num_seqs);
+        cfg.blockDim = dim3(kFp4Warps * 32);
+        cfg.dynamicSmemBytes = kSmem;
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = p.ranks;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = pdl_enabled() ? 2 : 1;
+        cudaError_t e = cudaLaunchKernelEx(&cfg, attention_fp4_cluster_kernel<T, D, NT>, p);
+        return e == cudaSuccess ? 0 : fail("attention_fp4_cluster_kernel", e);
+    }
     TELB_LAUNCH("attention_fp4_kernel", (attention_fp4_kernel<T, D, NT>), dim3(p.ctas), dim3(kFp4Warps * 32), kSmem, stream, p);
-    if (p.spans) TELB_LAUNCH("attention_fp4_merge_kernel", (attention_fp4_merge_kernel<T, D, NT>), dim3(p.max_items, p.num_seqs, min(columns, C)), dim3(128), 0, stream, p);
+    TELB_LAUNCH("attention_fp4_merge_kernel", (attention_fp4_merge_kernel<T, D, NT>), dim3(p.max_items, p.num_seqs, min(columns, C)), dim3(512), 0, stream, p);
     return 0;
 }
 
@@ -816,6 +957,7 @@ extern "C" int telb_attention_fp4_ctas(int columns, int d) {
     return sm_count() * (d * nt <= 128 ? 4 : d * nt <= 256 && d < 256 ? 3 : 2);
 }
 
+// ranks > 0: clusters of so many CTAs per item (sequence, KV head, C columns); 0: the line of all items' tiles cut into `ctas` parts, with
 // part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C of telb_attention_fp4_columns, max_items = KV heads x chunks of the longest
 // sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and its keys are cut
 // into `weight_ctas` parts.
@@ -825,7 +967,9 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (d != 64 && d != 128 && d != 256) return fail("telb_paged_attention_fp4: head_dim must be 64, 128 or 256");
     if (p.page_size < 16 || p.page_size != 1 << p.page_shift) return fail("telb_paged_attention_fp4: the page size must be a power of two, at least 16");
     if (p.hkv <= 0 || p.hq % p.hkv) return fail("telb_paged_attention_fp4: query heads must be a multiple of the KV heads");
-    if (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans) return fail("telb_paged_attention_fp4: no room for the parts");
+    if (p.ranks < 0 || p.ranks > 8) return fail("telb_paged_attention_fp4: clusters of at most 8 CTAs");
+    if (p.ranks == 0 && (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans)) return fail("telb_paged_attention_fp4: no room for the parts");
+    if (p.max_items > 65535) return fail("telb_paged_attention_fp4: too many rows x heads");
     if (p.num_seqs > 65535) return fail("telb_paged_attention_fp4: more than 65535 sequences");
     if (p.weights && (!p.stat || weight_ctas < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
     if (is_bf16) {

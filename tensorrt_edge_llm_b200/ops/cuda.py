@@ -642,7 +642,7 @@ class Fp4WriteParams(ctypes.Structure):
 class Fp4AttnParams(ctypes.Structure):
     """Host mirror of ``Fp4AttnParams`` (``csrc/kernels/attention_fp4.cu``)."""
     _fields_ = [(n, c_vp) for n in ("q", "pool", "out", "part_o", "part_ml", "stat", "q_start", "q_len", "past_len", "page_table", "scales", "sinks", "weights", "spans")] + \
-               [(n, c_int) for n in ("num_seqs", "tokens", "max_q_len", "num_pages", "max_pages", "page_size", "page_shift", "hq", "hkv", "window", "ctas", "max_items")] + \
+               [(n, c_int) for n in ("num_seqs", "tokens", "max_q_len", "num_pages", "max_pages", "page_size", "page_shift", "hq", "hkv", "window", "ctas", "ranks", "max_items")] + \
                [("scale", c_float), ("decay", c_float)]
 
 
@@ -724,11 +724,21 @@ FP4_DIRECT_COLUMNS = 64      # rows x heads of a KV head up to which a step read
 FP4_WEIGHT_COLUMNS = 256     # and up to which it keeps account of the attention weights
 
 
+def _fp4_ranks(items: int, tiles: int) -> int:
+    """CTAs of a cluster per item, or 0 for the form that cuts the line of all tiles."""
+    if items * 8 < 148 and tiles > 2048:
+        return 0
+    ranks = 1
+    while ranks < 8 and items * ranks < 2 * 148 and items * ranks * 8 <= tiles:
+        ranks *= 2
+    return ranks
+
+
 @_on_device
 def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, sliding_window=None, sinks=None, weights=None, decay: float = 1.0,
                         direct: Optional[bool] = None, ctas: Optional[int] = None) -> torch.Tensor:
     """See :func:`ops.paged_attention_fp4`.  ``direct`` forces the kernel that reads the pages in place (True), or the expansion to 16 bits and
-    the prompt kernels (False); ``ctas``: into how many parts that kernel cuts its work."""
+    the prompt kernels (False); ``ctas``: into how many parts that kernel cuts its work (negative: CTAs of a cluster per item)."""
     d = _fp4_geometry(kv_layer, meta, scales)
     is_bf16 = _is_bf16(q)
     t, hq = q.shape[:2]
@@ -764,19 +774,25 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     cols = L.telb_attention_fp4_columns(c_int(columns), c_int(d))
     items = hkv * -(-columns // cols)
     tiles = n * items * (-(-min(meta.max_seq_len, window + meta.max_q_len if window else meta.max_seq_len) // 32) + 1)
-    if ctas is None:            # as many as run at once, of four tiles of 32 keys or more
-        ctas = max(1, min(L.telb_attention_fp4_ctas(c_int(columns), c_int(d)), tiles // 4))
+    ranks = 0
+    if ctas is None:
+        ranks = _fp4_ranks(n * items, tiles)
+        ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(c_int(columns), c_int(d)), tiles // 4))
+    elif ctas < 0:
+        ranks, ctas = -ctas, 0
     # parts of outputs, their references and sums, (first, last) CTA of every item, softmax statistics of the rows
-    room = [2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items, 2 * t * hq if weights is not None else 0]
-    ws = torch.empty(sum(room), dtype=torch.float32, device=q.device)
-    at = _p(ws).value
-    part_o, part_ml, spans, stat = at, at + 4 * room[0], at + 4 * (room[0] + room[1]), at + 4 * sum(room[:3]) if weights is not None else None
+    room = [2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items if ctas else 0, 2 * t * hq if weights is not None else 0]
+    at = part_o = part_ml = spans = stat = None
+    if sum(room):
+        at = _p(torch.empty(sum(room), dtype=torch.float32, device=q.device)).value
+        part_o, part_ml, spans, stat = at, at + 4 * room[0], at + 4 * (room[0] + room[1]), at + 4 * sum(room[:3])
     ptr = lambda v: None if v is None else _p(v).value
-    p = Fp4AttnParams(ptr(q), ptr(kv_layer), ptr(out), part_o, part_ml, stat, *[ptr(v) for v in (meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
+    p = Fp4AttnParams(ptr(q), ptr(kv_layer), ptr(out), part_o, part_ml, stat if weights is not None else None,
+                      *[ptr(v) for v in (meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
                       spans, n, t, meta.max_q_len, kv_layer.shape[0], meta.page_table.shape[1], meta.page_size, meta.page_size.bit_length() - 1, hq, hkv, window, ctas,
-                      items, scale, decay)
+                      ranks, items, scale, decay)
     weight_ctas = max(1, min(2 * 148 if columns > 64 else 3 * 148, tiles // 4))
-    _check(L.telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(weight_ctas), c_int(is_bf16), _stream()), "paged_attention_fp4", 2 + (weights is not None))
+    _check(L.telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(weight_ctas), c_int(is_bf16), _stream()), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None))
     return out
 
 

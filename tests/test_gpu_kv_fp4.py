@@ -75,7 +75,7 @@ def test_attention_in_place(q_lens, past, hq, hkv, d, page, window, dtype, sunk)
     top = 6 * 448 * float(scales[1])
     m, lg, qg, sg = meta.to("cuda"), layer.cuda(), q.cuda(), scales.cuda()
     zg = sinks.cuda() if sunk else None
-    for ctas in (None, 1, 3):
+    for ctas in (None, 1, 3, -1, -2, -8):
         wg = w.cuda()
         got = ops.cuda_ops().paged_attention_fp4(qg, lg, m, d ** -0.5, sg, window or None, zg, wg, 0.75, ctas=ctas)
         again = ops.cuda_ops().paged_attention_fp4(qg, lg, m, d ** -0.5, sg, window or None, zg, direct=True, ctas=ctas)
