@@ -950,15 +950,15 @@ int launch_attention_fp4(const Fp4AttnParams& p, int weight_ctas, cudaStream_t s
 using namespace telb;
 
 // Columns (rows x heads of a KV head) that an item takes, of a step with `columns` of them.
-extern "C" int telb_attention_fp4_columns(int columns, int d) { return columns <= 8 || d == 256 ? 8 : 16; }
+static int fp4_columns(int columns, int d) { return columns <= 8 || d == 256 ? 8 : 16; }
 // CTAs that run at once.
 extern "C" int telb_attention_fp4_ctas(int columns, int d) {
-    const int nt = telb_attention_fp4_columns(columns, d) / 8;
+    const int nt = fp4_columns(columns, d) / 8;
     return sm_count() * (d * nt <= 128 ? 4 : d * nt <= 256 && d < 256 ? 3 : 2);
 }
 
 // ranks > 0: clusters of so many CTAs per item (sequence, KV head, C columns); 0: the line of all items' tiles cut into `ctas` parts, with
-// part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C of telb_attention_fp4_columns, max_items = KV heads x chunks of the longest
+// part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C: 8, or 16 for more than 8 columns of at most 128 features; max_items = KV heads x chunks of the longest
 // sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and its keys are cut
 // into `weight_ctas` parts.
 extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int weight_ctas, int is_bf16, cudaStream_t stream) {
@@ -969,6 +969,8 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (p.hkv <= 0 || p.hq % p.hkv) return fail("telb_paged_attention_fp4: query heads must be a multiple of the KV heads");
     if (p.ranks < 0 || p.ranks > 8) return fail("telb_paged_attention_fp4: clusters of at most 8 CTAs");
     if (p.ranks == 0 && (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans)) return fail("telb_paged_attention_fp4: no room for the parts");
+    const int columns = p.max_q_len * (p.hq / p.hkv), cols = fp4_columns(columns, d);
+    if (p.max_items != p.hkv * ((columns + cols - 1) / cols)) return fail("telb_paged_attention_fp4: items of another size");
     if (p.max_items > 65535) return fail("telb_paged_attention_fp4: too many rows x heads");
     if (p.num_seqs > 65535) return fail("telb_paged_attention_fp4: more than 65535 sequences");
     if (p.weights && (!p.stat || weight_ctas < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");

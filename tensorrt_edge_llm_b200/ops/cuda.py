@@ -10,6 +10,7 @@ import ctypes
 import dataclasses
 import functools
 import os
+import struct
 import threading
 from typing import Dict, Optional, Tuple
 
@@ -618,105 +619,126 @@ def paged_attention_decode_fp8(q8: torch.Tensor, kv_layer: torch.Tensor, meta: S
 # ---- four-bit (NVFP4) cache pages --------------------------------------------------------------
 
 
+# These operators run once a layer in steps of few rows, where the host's part of a call counts as much as the kernel's: parameters are packed
+# by `struct` in the order of the C structures, and pointers are taken without a list of what they belong to (the caller's names
+# and this module's locals hold every tensor until the launch is enqueued).
+
+
 def _on_device(fn):
-    """Run ``fn`` with the device of its first tensor argument as the current one (its launches go to that device's current stream)."""
+    """Run ``fn`` with the device of its first argument as the current one (its launches go to that device's current stream)."""
     @functools.wraps(fn)
     def run(t, *args, **kw):
-        if not t.is_cuda:
-            raise ValueError(f"{fn.__name__}: a tensor on {t.device}, not on the GPU")
-        if t.device.index == torch.cuda.current_device():
+        dev = t.get_device()
+        if dev == torch.cuda.current_device():
             return fn(t, *args, **kw)
-        with torch.cuda.device(t.device):
+        if dev < 0:
+            raise ValueError(f"{fn.__name__}: a tensor on {t.device}, not on the GPU")
+        with torch.cuda.device(dev):
             return fn(t, *args, **kw)
     return run
 
 
-class Fp4WriteParams(ctypes.Structure):
-    """Host mirror of ``Fp4WriteParams`` (``csrc/kernels/kv_fp4.cu``)."""
-    _fields_ = [(n, c_vp) for n in ("qkv", "q_out", "pool", "cos_sin", "positions", "seq_ids", "q_start", "past_len", "page_table", "kv_offsets", "q_norm",
-                                    "k_norm", "scales", "stage", "stage_table")] + \
-               [(n, c_int) for n in ("tokens", "hq", "hkv", "rot", "max_pos", "page_size", "max_pages", "num_pages", "stage_page", "stage_max", "stage_pages")] + \
-               [("eps", c_float)]
+def _ptrs(what: str, dev: int, tensors) -> list:
+    """Addresses of ``tensors`` (0 for None), which must all lie on GPU ``dev``."""
+    out = []
+    for v in tensors:
+        if v is None:
+            out.append(0)
+        elif v.get_device() != dev:
+            raise ValueError(f"{what}: a tensor of shape {tuple(v.shape)} lives on {v.device}, not on GPU {dev}")
+        else:
+            out.append(v.data_ptr())
+    return out
 
 
-class Fp4AttnParams(ctypes.Structure):
-    """Host mirror of ``Fp4AttnParams`` (``csrc/kernels/attention_fp4.cu``)."""
-    _fields_ = [(n, c_vp) for n in ("q", "pool", "out", "part_o", "part_ml", "stat", "q_start", "q_len", "past_len", "page_table", "scales", "sinks", "weights", "spans")] + \
-               [(n, c_int) for n in ("num_seqs", "tokens", "max_q_len", "num_pages", "max_pages", "page_size", "page_shift", "hq", "hkv", "window", "ctas", "ranks", "max_items")] + \
-               [("scale", c_float), ("decay", c_float)]
+def _raw_stream(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)      # 0.1 us; a Stream object costs 1.3
 
 
-class EvictParams(ctypes.Structure):
-    """Host mirror of ``EvictParams`` (``csrc/kernels/kv_evict.cu``)."""
-    _fields_ = [(n, c_vp) for n in ("pool", "weights", "page_table", "lengths", "to_table", "kept")] + \
-               [(n, c_int) for n in ("num_seqs", "hkv", "num_pages", "max_pages", "to_pages", "page_size", "page_shift", "row_bytes", "scale_bytes", "keep", "first", "recent")]
+@functools.lru_cache(maxsize=None)
+def _fp4_lib():
+    """The kernel library with the argument types of these entry points."""
+    L, i, p = lib(), c_int, c_vp
+    L.telb_rope_kv_write_fp4.argtypes = [ctypes.c_char_p, i, i, p]
+    L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, i, p]
+    L.telb_attention_fp4_ctas.argtypes = [i, i]
+    L.telb_kv_fp4_stage.argtypes = [p] * 7 + [i] * 9 + [p]
+    L.telb_kv_evict.argtypes = [ctypes.c_char_p, p]
+    return L
 
 
-def _fp4_geometry(kv_layer: torch.Tensor, meta: StepMeta, scales: torch.Tensor) -> int:
-    """Head size of a four-bit layer, after the checks that all its operators share."""
+_FP4_WRITE = struct.Struct("15P11if")       # Fp4WriteParams (csrc/kernels/kv_fp4.cu)
+_FP4_ATTN = struct.Struct("14P13i2f")       # Fp4AttnParams (csrc/kernels/attention_fp4.cu)
+_EVICT = struct.Struct("6P12i")             # EvictParams (csrc/kernels/kv_evict.cu)
+
+
+def _fp4_geometry(kv_layer: torch.Tensor, meta: StepMeta, scales: torch.Tensor) -> tuple:
+    """``(pages, KV heads, head size)`` of a four-bit layer, after the checks that all its operators share."""
+    shape = kv_layer.shape
     d = ref_ops.fp4_head_dim(kv_layer)
     if not kv_layer.is_contiguous() or kv_layer.data_ptr() % 16:
         raise ValueError("a four-bit layer must be contiguous and start on 16 bytes")
-    if kv_layer.shape[3] != meta.page_size:
-        raise ValueError(f"a layer of {kv_layer.shape[3]}-row pages in a step of {meta.page_size}-row pages")
+    if shape[3] != meta.page_size:
+        raise ValueError(f"a layer of {shape[3]}-row pages in a step of {meta.page_size}-row pages")
     if scales.dtype != torch.float32 or scales.numel() != 2 or not scales.is_contiguous():
         raise ValueError("scales: two contiguous fp32 numbers, of the keys and of the values")
-    return d
+    return shape[0], shape[2], d
 
 
 @_on_device
 def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads: int, num_kv_heads: int, head_dim: int, scales, q_norm_w=None, k_norm_w=None,
                       eps: float = 1e-6, stage=None, stage_table=None) -> torch.Tensor:
     """See :func:`ops.rope_kv_write_fp4`."""
-    d = _fp4_geometry(kv_layer, meta, scales)
-    is_bf16 = _is_bf16(qkv)
-    t = qkv.shape[0]
-    if d != head_dim or kv_layer.shape[2] != num_kv_heads or qkv.shape != (t, (num_q_heads + 2 * num_kv_heads) * d) or t != meta.num_tokens:
-        raise ValueError(f"rope_kv_write_fp4: rows {tuple(qkv.shape)} of {num_q_heads} + 2 x {num_kv_heads} heads of {head_dim}, a layer of {kv_layer.shape[2]} heads of {d}")
+    pages, hkv, d = _fp4_geometry(kv_layer, meta, scales)
+    dtype, is_bf16 = qkv.dtype, _is_bf16(qkv)
+    t = meta.num_tokens
+    if d != head_dim or hkv != num_kv_heads or qkv.shape != (t, (num_q_heads + 2 * hkv) * d):
+        raise ValueError(f"rope_kv_write_fp4: rows {tuple(qkv.shape)} of {num_q_heads} + 2 x {num_kv_heads} heads of {head_dim}, {t} rows, a layer of {hkv} heads of {d}")
     positions = meta.positions
     if meta.rope_rows is not None:          # multimodal RoPE: per-row cos / sin tables prepared by the model
         cos_sin, positions = meta.rope_rows, meta.rope_pos
-    rot = cos_sin.shape[-1]
-    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or rot > d or rot % (d // 16):
+    max_pos, rot = cos_sin.shape
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or max_pos < 1 or rot > d or rot % (d // 16):
         raise ValueError(f"rope_kv_write_fp4: a contiguous fp32 cos | sin table of at most {d} columns, a multiple of {d // 16}")
     for w in (q_norm_w, k_norm_w):
-        if w is not None and (w.dtype != qkv.dtype or w.numel() != d or not w.is_contiguous()):
-            raise ValueError(f"rope_kv_write_fp4: norm weights of {d} numbers in the type of the rows")
+        if w is not None and (w.dtype != dtype or w.numel() != d or not w.is_contiguous() or w.data_ptr() % 16):
+            raise ValueError(f"rope_kv_write_fp4: norm weights of {d} numbers in the type of the rows, which start on 16 bytes")
     if (stage is None) != (stage_table is None):
         raise ValueError("rope_kv_write_fp4: 16-bit pages come with their page table")
+    staged = (1, 0, 0)
     if stage is not None:
-        if stage.dtype != qkv.dtype or not stage.is_contiguous() or stage.shape[1:3] != (2, num_kv_heads) or stage.shape[4] != d:
-            raise ValueError(f"rope_kv_write_fp4: 16-bit pages {tuple(stage.shape)} {stage.dtype} for rows of {qkv.dtype}, {num_kv_heads} heads of {d}")
-        if stage_table.dtype != torch.int32 or not stage_table.is_contiguous() or stage_table.shape[0] != meta.num_seqs:
+        if stage.dtype != dtype or not stage.is_contiguous() or stage.data_ptr() % 16 or stage.dim() != 5 or stage.shape[1:3] != (2, hkv) or stage.shape[4] != d:
+            raise ValueError(f"rope_kv_write_fp4: 16-bit pages {tuple(stage.shape)} {stage.dtype} for rows of {dtype}, {hkv} heads of {d}")
+        if stage_table.dtype != torch.int32 or not stage_table.is_contiguous() or stage_table.dim() != 2 or stage_table.shape[0] != meta.num_seqs:
             raise ValueError("rope_kv_write_fp4: the 16-bit pages' table is int32 [sequences, pages]")
+        staged = (stage.shape[3], stage_table.shape[1], stage.shape[0])
     qkv = _aligned(qkv)
-    q = torch.empty(t, num_q_heads, d, dtype=qkv.dtype, device=qkv.device)
-    ptr = lambda v: None if v is None else _p(v).value
-    p = Fp4WriteParams(*[ptr(v) for v in (qkv, q, kv_layer, cos_sin, positions, meta.seq_ids, meta.q_start, meta.past_len, meta.page_table, meta.kv_offsets,
-                                          q_norm_w, k_norm_w, scales, stage, stage_table)],
-                       t, num_q_heads, num_kv_heads, rot, cos_sin.shape[0], meta.page_size, meta.page_table.shape[1], kv_layer.shape[0],
-                       1 if stage is None else stage.shape[3], 0 if stage is None else stage_table.shape[1], 0 if stage is None else stage.shape[0], eps)
-    _check(lib().telb_rope_kv_write_fp4(ctypes.byref(p), c_int(d), c_int(is_bf16), _stream()), "rope_kv_write_fp4")
+    q = qkv.new_empty((t, num_q_heads, d))
+    dev = qkv.get_device()
+    p = _FP4_WRITE.pack(*_ptrs("rope_kv_write_fp4", dev, (qkv, q, kv_layer, cos_sin, positions, meta.seq_ids, meta.q_start, meta.past_len, meta.page_table,
+                                                          meta.kv_offsets, q_norm_w, k_norm_w, scales, stage, stage_table)),
+                        t, num_q_heads, hkv, rot, max_pos, meta.page_size, meta.page_table.shape[1], pages, *staged, eps)
+    _check(_fp4_lib().telb_rope_kv_write_fp4(p, d, is_bf16, _raw_stream(dev)), "rope_kv_write_fp4")
     return q
 
 
 @_on_device
 def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int = 0, new_rows: bool = False):
     """See :func:`ops.kv_fp4_stage`."""
-    d = _fp4_geometry(kv_layer, meta, scales)
+    pages, hkv, d = _fp4_geometry(kv_layer, meta, scales)
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"kv_fp4_stage: pages of fp16 or bf16, not {dtype}")
-    return _fp4_stage(kv_layer, meta, scales, dtype, window, new_rows, d)
+    return _fp4_stage(kv_layer, meta, scales, dtype, window, new_rows, pages, hkv, d)
 
 
-def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int, new_rows: bool, d: int):
-    hkv, n = kv_layer.shape[2], meta.num_seqs
-    per = max(1, (meta.max_seq_len + 63) // 64)
+def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int, new_rows: bool, pages: int, hkv: int, d: int):
+    """Without ``scales``: codes times block scales, which both 16-bit types hold exactly."""
+    n, per, dev = meta.num_seqs, max(1, (meta.max_seq_len + 63) // 64), kv_layer.get_device()
     stage = torch.empty(n * per, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
     table = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device)
-    _check(lib().telb_kv_fp4_stage(_p(kv_layer), _p(stage), _p(table), _p(meta.past_len), _p(meta.q_len if new_rows else None), _p(meta.page_table), _p(scales), c_int(n),
-                                   c_int(meta.page_table.shape[1]), c_int(kv_layer.shape[0]), c_int(meta.page_size), c_int(per), c_int(hkv), c_int(d),
-                                   c_int(window or 0), c_int(int(dtype == torch.bfloat16)), _stream()), "kv_fp4_stage")
+    _check(_fp4_lib().telb_kv_fp4_stage(
+        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, meta.past_len, meta.q_len if new_rows else None, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
+        meta.page_size, per, hkv, d, window or 0, int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
     return stage, dataclasses.replace(meta, page_table=table, page_size=64)
 
 
@@ -739,19 +761,19 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
                         direct: Optional[bool] = None, ctas: Optional[int] = None) -> torch.Tensor:
     """See :func:`ops.paged_attention_fp4`.  ``direct`` forces the kernel that reads the pages in place (True), or the expansion to 16 bits and
     the prompt kernels (False); ``ctas``: into how many parts that kernel cuts its work (negative: CTAs of a cluster per item)."""
-    d = _fp4_geometry(kv_layer, meta, scales)
+    pages, hkv, d = _fp4_geometry(kv_layer, meta, scales)
     is_bf16 = _is_bf16(q)
-    t, hq = q.shape[:2]
-    hkv = kv_layer.shape[2]
-    if q.dim() != 3 or q.shape[2] != d or hq % hkv or t != meta.num_tokens:
-        raise ValueError(f"paged_attention_fp4: queries {tuple(q.shape)} over {hkv} heads of {d}, {meta.num_tokens} rows")
+    shape = q.shape
+    if len(shape) != 3 or shape[2] != d or shape[1] % hkv or shape[0] != meta.num_tokens:
+        raise ValueError(f"paged_attention_fp4: queries {tuple(shape)} over {hkv} heads of {d}, {meta.num_tokens} rows")
+    t, hq, _ = shape
     if not scale > 0:
         raise ValueError("paged_attention_fp4: the score scale must be positive")
     window = sliding_window if sliding_window and sliding_window > 0 else 0
     columns = meta.max_q_len * (hq // hkv)
     if weights is not None:
-        if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (kv_layer.shape[0], hkv, meta.page_size):
-            raise ValueError(f"paged_attention_fp4: weights are contiguous fp32 {(kv_layer.shape[0], hkv, meta.page_size)}")
+        if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (pages, hkv, meta.page_size):
+            raise ValueError(f"paged_attention_fp4: weights are contiguous fp32 {(pages, hkv, meta.page_size)}")
         if meta.tree_mask is not None or columns > FP4_WEIGHT_COLUMNS:
             raise ValueError(f"paged_attention_fp4: weights are kept for causal steps of at most {FP4_WEIGHT_COLUMNS} rows x heads of a KV head, not {columns}")
         if direct is False:
@@ -759,40 +781,42 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     if sinks is not None:
         if sinks.numel() != hq:
             raise ValueError(f"paged_attention_fp4: {sinks.numel()} sinks for {hq} heads")
-        sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
+        if sinks.dtype != torch.float32 or not sinks.is_contiguous() or not sinks.is_cuda:
+            sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     if direct is None:
         direct = weights is not None or (meta.tree_mask is None and columns <= FP4_DIRECT_COLUMNS)
     if not direct or meta.tree_mask is not None:
         if direct:
             raise ValueError("paged_attention_fp4: tree masks are read by the prompt kernels only")
-        # codes times block scales, which 16 bits hold exactly; the two global scales multiply scores and outputs
-        stage, staged = _fp4_stage(kv_layer, meta, None, q.dtype, window, True, d)
+        # the two global scales multiply scores and outputs, in 32 bits
+        stage, staged = _fp4_stage(kv_layer, meta, None, q.dtype, window, True, pages, hkv, d)
         return paged_attention(q, stage, staged, scale, sliding_window, sinks, kv_scales=scales)
     q = _aligned(q)
     out = torch.empty_like(q)
-    n, L = meta.num_seqs, lib()
-    cols = L.telb_attention_fp4_columns(c_int(columns), c_int(d))
+    dev, n, L = q.get_device(), meta.num_seqs, _fp4_lib()
+    cols = 8 if columns <= 8 or d == 256 else 16          # columns of an item, as the launcher has it
     items = hkv * -(-columns // cols)
     tiles = n * items * (-(-min(meta.max_seq_len, window + meta.max_q_len if window else meta.max_seq_len) // 32) + 1)
     ranks = 0
     if ctas is None:
         ranks = _fp4_ranks(n * items, tiles)
-        ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(c_int(columns), c_int(d)), tiles // 4))
+        ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(columns, d), tiles // 4))
     elif ctas < 0:
         ranks, ctas = -ctas, 0
-    # parts of outputs, their references and sums, (first, last) CTA of every item, softmax statistics of the rows
-    room = [2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items if ctas else 0, 2 * t * hq if weights is not None else 0]
-    at = part_o = part_ml = spans = stat = None
-    if sum(room):
-        at = _p(torch.empty(sum(room), dtype=torch.float32, device=q.device)).value
-        part_o, part_ml, spans, stat = at, at + 4 * room[0], at + 4 * (room[0] + room[1]), at + 4 * sum(room[:3])
-    ptr = lambda v: None if v is None else _p(v).value
-    p = Fp4AttnParams(ptr(q), ptr(kv_layer), ptr(out), part_o, part_ml, stat if weights is not None else None,
-                      *[ptr(v) for v in (meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights)],
-                      spans, n, t, meta.max_q_len, kv_layer.shape[0], meta.page_table.shape[1], meta.page_size, meta.page_size.bit_length() - 1, hq, hkv, window, ctas,
-                      ranks, items, scale, decay)
+    part_o = part_ml = spans = stat = 0
+    if ctas or weights is not None:
+        # parts of outputs, their references and sums, (first, last) CTA of every item; softmax statistics of the rows
+        room = (2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items if ctas else 0, 2 * t * hq if weights is not None else 0)
+        ws = torch.empty(sum(room), dtype=torch.float32, device=q.device)
+        part_o = ws.data_ptr()
+        part_ml = part_o + 4 * room[0]
+        spans = part_ml + 4 * room[1]
+        stat = spans + 4 * room[2] if weights is not None else 0
+    ptr = _ptrs("paged_attention_fp4", dev, (q, kv_layer, out, meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights))
+    p = _FP4_ATTN.pack(*ptr[:3], part_o, part_ml, stat, *ptr[3:], spans, n, t, meta.max_q_len, pages, meta.page_table.shape[1], meta.page_size,
+                       meta.page_size.bit_length() - 1, hq, hkv, window, ctas, ranks, items, scale, decay)
     weight_ctas = max(1, min(2 * 148 if columns > 64 else 3 * 148, tiles // 4))
-    _check(L.telb_paged_attention_fp4(ctypes.byref(p), c_int(d), c_int(weight_ctas), c_int(is_bf16), _stream()), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None))
+    _check(L.telb_paged_attention_fp4(p, d, weight_ctas, is_bf16, _raw_stream(dev)), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None))
     return out
 
 
@@ -802,15 +826,13 @@ def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep: int, first:
     row, sf = ref_ops.evict_geometry(kv_layer, weights, page_table, lengths, to_table, keep, first, recent)
     if not (kv_layer.is_contiguous() and weights.is_contiguous()) or (kv_layer.data_ptr() | weights.data_ptr()) % 16 or row % 16 or sf % 4:
         raise ValueError("kv_evict: a contiguous layer that starts on 16 bytes, rows of a multiple of 16 bytes, contiguous weights that start on 16 bytes")
-    if any(v.device != kv_layer.device for v in (weights, page_table, lengths, to_table)):
-        raise ValueError("kv_evict: all tensors on one device")
     pages, _, hkv, psz = kv_layer.shape[:4]
-    n = page_table.shape[0]
+    n, dev = page_table.shape[0], kv_layer.get_device()
     kept = torch.empty(n, hkv, keep, dtype=torch.int32, device=kv_layer.device)
-    page_table, lengths, to_table = (v.to(torch.int32).contiguous() for v in (page_table, lengths, to_table))
-    p = EvictParams(*[_p(v).value for v in (kv_layer, weights, page_table, lengths, to_table, kept)], n, hkv, pages, page_table.shape[1], to_table.shape[1],
-                    psz, psz.bit_length() - 1 if psz & (psz - 1) == 0 else -1, row, sf, keep, first, recent)
-    _check(lib().telb_kv_evict(ctypes.byref(p), _stream()), "kv_evict", 2)
+    page_table, lengths, to_table = (v if v.dtype == torch.int32 and v.is_contiguous() else v.to(torch.int32).contiguous() for v in (page_table, lengths, to_table))
+    p = _EVICT.pack(*_ptrs("kv_evict", dev, (kv_layer, weights, page_table, lengths, to_table, kept)), n, hkv, pages, page_table.shape[1], to_table.shape[1], psz,
+                    psz.bit_length() - 1 if psz & (psz - 1) == 0 else -1, row, sf, keep, first, recent)
+    _check(_fp4_lib().telb_kv_evict(p, _raw_stream(dev)), "kv_evict", 2)
     return kept
 
 

@@ -1353,12 +1353,13 @@ def kv_fp8_store(kv_layer: torch.Tensor, stage: torch.Tensor, meta, scales: torc
 
 def fp4_head_dim(kv_layer: torch.Tensor) -> int:
     """Head size of a four-bit layer ``uint8 [pages, 2, Hkv, P, 9 D / 16]``."""
-    if kv_layer.dtype != torch.uint8 or kv_layer.dim() != 5 or kv_layer.shape[1] != 2 or kv_layer.shape[4] not in (36, 72, 144):
-        raise ValueError(f"a four-bit layer is uint8 [pages, 2, heads, rows, 9 D / 16] with heads of 64, 128 or 256, not {kv_layer.dtype} {tuple(kv_layer.shape)}")
-    p = kv_layer.shape[3]
+    shape = kv_layer.shape
+    if kv_layer.dtype != torch.uint8 or len(shape) != 5 or shape[1] != 2 or shape[4] not in (36, 72, 144):
+        raise ValueError(f"a four-bit layer is uint8 [pages, 2, heads, rows, 9 D / 16] with heads of 64, 128 or 256, not {kv_layer.dtype} {tuple(shape)}")
+    p = shape[3]
     if p < 16 or p & (p - 1):
         raise ValueError(f"four-bit pages hold a power of two of rows, at least 16, not {p}")
-    return kv_layer.shape[4] * 16 // 9
+    return shape[4] * 16 // 9
 
 
 def fp4_page_parts(kv_layer: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
