@@ -26,9 +26,174 @@ struct Fp4WriteParams {
     float eps;
 };
 
-// One warp per (token, head); a lane holds E neighbouring features.
+// Eight values of a block of 16, whose other eight lie in the neighbouring lane: their codes, the block's scale byte and what the codes stand for.
+__device__ __forceinline__ uint32_t fp4_block_half(const float (&v)[8], float scale, uint8_t& sf, float (&back)[8]) {
+    uint32_t m = 0;                                             // the largest magnitude, compared as bit patterns so that a NaN stays one
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    float want = __fdiv_rn(__fdiv_rn(__uint_as_float(m), 6.f), scale);
+    want = want > 448.f ? 448.f : want;
+    sf = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
+    const float step = __fmul_rn(e4m3_to_float(sf), scale);
+    float y[8];
+    if (m < 0x7f800000u && step > 1e-30f && step < 1e30f) {
+        // Quotients by the reciprocal and one correction (Markstein 1990): rounded as a division rounds them, for all of the block one division
+        const float inv = __frcp_rn(step);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float q = __fmul_rn(v[i], inv);
+            y[i] = __fmaf_rn(__fmaf_rn(-q, step, v[i]), inv, q);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = step > 0.f ? __fdiv_rn(v[i], step) : v[i] != v[i] ? 0.f : copysignf(0.f, v[i]);
+    }
+    uint32_t codes = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) codes |= e2m1_pair(y[i], y[i + 1]) << (4 * i);
+    uint32_t h[4];
+    e2m1x8_to_half(codes, h[0], h[1], h[2], h[3]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        back[2 * i] = __fmul_rn(f.x, step);
+        back[2 * i + 1] = __fmul_rn(f.y, step);
+    }
+    return codes;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    return make_uint4(Cvt<T>::pack2(v[0], v[1]), Cvt<T>::pack2(v[2], v[3]), Cvt<T>::pack2(v[4], v[5]), Cvt<T>::pack2(v[6], v[7]));
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Cvt<T>::to_f(e[i]);
+}
+
+// Whole heads turn: D/16 lanes a head, a lane holds features 8 l .. and D/2 + 8 l .., which turn together; a warp takes every `parts`-th group of 512 / D heads
+// of a token, whose cos / sin row, norm weights and page look-up it fetches once.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) rope_kv_write_fp4_kernel(const Fp4WriteParams p) {
+__global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WriteParams p, int parts) {
+    pdl_prologue();
+    constexpr int L = D / 16, H = 32 / L;                       // lanes of a head, heads of a warp
+    const int unit = (int)((blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5);
+    const int t = unit / parts, part = unit - t * parts, lane = threadIdx.x & 31, l = lane % L, hh = lane / L;
+    if (t >= p.tokens) return;
+    const int heads = p.hq + 2 * p.hkv, groups = (heads + H - 1) / H;
+    const T* row = reinterpret_cast<const T*>(p.qkv) + (size_t)t * heads * D;
+    uint4 next[2];
+    auto fetch = [&](int grp) {
+        const int h = min(grp * H + hh, heads - 1);
+        const T* src = row + (size_t)h * D + 8 * l;
+        next[0] = *reinterpret_cast<const uint4*>(src);
+        next[1] = *reinterpret_cast<const uint4*>(src + D / 2);
+    };
+    fetch(part);
+    float c[8], sn[8];
+    {
+        const float* cs = p.cos_sin + (size_t)min(max(p.positions[t], 0), p.max_pos - 1) * D + 8 * l;
+        *reinterpret_cast<float4*>(c) = *reinterpret_cast<const float4*>(cs);
+        *reinterpret_cast<float4*>(c + 4) = *reinterpret_cast<const float4*>(cs + 4);
+        *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(cs + D / 2);
+        *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(cs + D / 2 + 4);
+    }
+    uint4 wq[2], wk[2];
+    wq[0] = wq[1] = wk[0] = wk[1] = make_uint4(0, 0, 0, 0);
+    if (p.q_norm) {
+        wq[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q_norm) + 8 * l);
+        wq[1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q_norm) + D / 2 + 8 * l);
+    }
+    if (p.k_norm) {
+        wk[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k_norm) + 8 * l);
+        wk[1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k_norm) + D / 2 + 8 * l);
+    }
+    const int s = p.seq_ids[t];
+    const int slot = p.past_len[s] + (p.kv_offsets ? p.kv_offsets[t] : t - p.q_start[s]);
+    const int lp = slot / p.page_size, at = slot - lp * p.page_size;
+    const int page = lp < p.max_pages ? p.page_table[(size_t)s * p.max_pages + lp] : -1;
+    int sp = -1, stage_at = 0;
+    if (p.stage) {
+        const int sl = slot / p.stage_page;
+        stage_at = slot - sl * p.stage_page;
+        sp = sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
+    }
+    const float scale_k = p.scales[0], scale_v = p.scales[1];
+    for (int grp = part; grp < groups; grp += parts) {
+        const int h = grp * H + hh;
+        float lo[8], hi[8];
+        unpack8<T>(next[0], lo);
+        unpack8<T>(next[1], hi);
+        if (grp + parts < groups) fetch(grp + parts);
+        const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
+        const bool norm = is_q ? p.q_norm != nullptr : !is_v && p.k_norm != nullptr;
+        if (__any_sync(0xffffffffu, norm)) {
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss += (double)lo[i] * (double)lo[i] + (double)hi[i] * (double)hi[i];
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (norm) {
+                const float inv = (float)(1.0 / sqrt(ss / D + (double)p.eps));
+                float w[2][8];
+                unpack8<T>(is_q ? wq[0] : wk[0], w[0]);
+                unpack8<T>(is_q ? wq[1] : wk[1], w[1]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    lo[i] = Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(lo[i], inv))), w[0][i])));
+                    hi[i] = Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(hi[i], inv))), w[1][i])));
+                }
+            }
+        }
+        if (!is_v) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float a = lo[i], b = hi[i];
+                lo[i] = __fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, sn[i]));
+                hi[i] = __fadd_rn(__fmul_rn(b, c[i]), __fmul_rn(a, sn[i]));
+            }
+        }
+        const uint4 plo = pack8<T>(lo), phi = pack8<T>(hi);
+        if (is_q) {
+            T* dst = reinterpret_cast<T*>(p.q_out) + ((size_t)t * p.hq + h) * D + 8 * l;
+            *reinterpret_cast<uint4*>(dst) = plo;
+            *reinterpret_cast<uint4*>(dst + D / 2) = phi;
+        }
+        if (__all_sync(0xffffffffu, is_q)) continue;
+        unpack8<T>(plo, lo);                                    // what a 16-bit cache would hold
+        unpack8<T>(phi, hi);
+        uint8_t sf[2];
+        float back[2][8];
+        const uint32_t codes_lo = fp4_block_half(lo, is_v ? scale_v : scale_k, sf[0], back[0]), codes_hi = fp4_block_half(hi, is_v ? scale_v : scale_k, sf[1], back[1]);
+        if (is_q || h >= heads) continue;
+        const int head = is_v ? h - p.hq - p.hkv : h - p.hq;
+        if ((unsigned)page < (unsigned)p.num_pages) {           // else: a row that has no page is not stored
+            uint8_t* slab = p.pool + (((size_t)page * 2 + is_v) * p.hkv + head) * fp4_slab_bytes(p.page_size, D);
+            uint8_t* dst = slab + (size_t)at * (D / 2) + 4 * l;
+            *reinterpret_cast<uint32_t*>(dst) = codes_lo;
+            *reinterpret_cast<uint32_t*>(dst + D / 4) = codes_hi;
+            if (!(l & 1)) {
+                uint8_t* f = slab + (size_t)p.page_size * (D / 2) + (size_t)at * (D / 16) + l / 2;
+                f[0] = sf[0];
+                f[D / 32] = sf[1];
+            }
+        }
+        if ((unsigned)sp < (unsigned)p.stage_pages) {
+            T* dst = reinterpret_cast<T*>(p.stage) + ((((size_t)sp * 2 + is_v) * p.hkv + head) * p.stage_page + stage_at) * D + 8 * l;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) back[0][i] = Cvt<T>::to_f(fp4_round<T>(back[0][i])), back[1][i] = Cvt<T>::to_f(fp4_round<T>(back[1][i]));
+            *reinterpret_cast<uint4*>(dst) = pack8<T>(back[0]);
+            *reinterpret_cast<uint4*>(dst + D / 2) = pack8<T>(back[1]);
+        }
+    }
+}
+
+// A part of a head turns: one warp per (token, head); a lane holds E neighbouring features.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4WriteParams p) {
     pdl_prologue();
     constexpr int E = D / 32, kLanes = 16 / E;                 // lanes of a block of 16 features
     const int heads = p.hq + 2 * p.hkv;
@@ -183,9 +348,28 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
     if (p.tokens <= 0) return 0;
     if (d != 64 && d != 128 && d != 256) return fail("telb_rope_kv_write_fp4: head_dim must be 64, 128 or 256");
     if (p.rot < 0 || p.rot > d || p.rot % (d / 16)) return fail("telb_rope_kv_write_fp4: the rotated part must be a multiple of head_dim / 16");
+    if (p.rot == d) {
+        // A warp for all heads of a token where that fills the device, else one for every group of heads
+        const int groups = (p.hq + 2 * p.hkv + 512 / d - 1) / (512 / d);
+        const int parts = (int)min((long long)groups, max(1LL, (16LL * 4 * sm_count() + p.tokens - 1) / p.tokens));
+        const long long warps = (long long)p.tokens * parts;
+        const dim3 grid((unsigned)((warps + 3) / 4)), blk(128);
+#define WRITE_FP4(T, D) TELB_LAUNCH("rope_kv_write_fp4_kernel", (rope_kv_write_fp4_kernel<T, D>), grid, blk, 0, stream, p, parts)
+        if (is_bf16) {
+            if (d == 128) WRITE_FP4(__nv_bfloat16, 128);
+            else if (d == 64) WRITE_FP4(__nv_bfloat16, 64);
+            else WRITE_FP4(__nv_bfloat16, 256);
+        } else {
+            if (d == 128) WRITE_FP4(__half, 128);
+            else if (d == 64) WRITE_FP4(__half, 64);
+            else WRITE_FP4(__half, 256);
+        }
+#undef WRITE_FP4
+        return 0;
+    }
     const long long warps = (long long)p.tokens * (p.hq + 2 * p.hkv);
     const dim3 grid((unsigned)((warps + 7) / 8)), blk(256);
-#define WRITE_FP4(T, D) TELB_LAUNCH("rope_kv_write_fp4_kernel", (rope_kv_write_fp4_kernel<T, D>), grid, blk, 0, stream, p)
+#define WRITE_FP4(T, D) TELB_LAUNCH("rope_part_kv_write_fp4_kernel", (rope_part_kv_write_fp4_kernel<T, D>), grid, blk, 0, stream, p)
     if (is_bf16) {
         if (d == 128) WRITE_FP4(__nv_bfloat16, 128);
         else if (d == 64) WRITE_FP4(__nv_bfloat16, 64);
@@ -195,6 +379,7 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
         else if (d == 64) WRITE_FP4(__half, 64);
         else WRITE_FP4(__half, 256);
     }
+#undef WRITE_FP4
     return 0;
 }
 

@@ -698,7 +698,7 @@ def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads: int, 
     if meta.rope_rows is not None:          # multimodal RoPE: per-row cos / sin tables prepared by the model
         cos_sin, positions = meta.rope_rows, meta.rope_pos
     max_pos, rot = cos_sin.shape
-    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or max_pos < 1 or rot > d or rot % (d // 16):
+    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16 or max_pos < 1 or rot > d or rot % (d // 16):
         raise ValueError(f"rope_kv_write_fp4: a contiguous fp32 cos | sin table of at most {d} columns, a multiple of {d // 16}")
     for w in (q_norm_w, k_norm_w):
         if w is not None and (w.dtype != dtype or w.numel() != d or not w.is_contiguous() or w.data_ptr() % 16):
