@@ -26,25 +26,40 @@ struct Fp4WriteParams {
     float eps;
 };
 
+// 1 / sqrt(x), rounded to 32 bits from a value that two Newton steps in 64 bits have brought to some 2^-50; the full root where 32 bits cannot hold x.
+__device__ __forceinline__ float inverse_root(double x) {
+    const float f = (float)x;
+    if (!(f > 1e-30f && f < 1e30f)) return (float)(1.0 / sqrt(x));
+    double y = (double)rsqrtf(f);
+    y = y * (1.5 - 0.5 * x * y * y);
+    y = y * (1.5 - 0.5 * x * y * y);
+    return (float)y;
+}
+
 // Eight values of a block of 16, whose other eight lie in the neighbouring lane: their codes, the block's scale byte and what the codes stand for.
-__device__ __forceinline__ uint32_t fp4_block_half(const float (&v)[8], float scale, uint8_t& sf, float (&back)[8]) {
+// Quotients by a reciprocal and one correction (Markstein 1990) are rounded as a division rounds them, away from the ends of the range.
+__device__ __forceinline__ float quotient(float a, float b, float inv_b) {
+    const float q = __fmul_rn(a, inv_b);
+    return __fmaf_rn(__fmaf_rn(-q, b, a), inv_b, q);
+}
+__device__ __forceinline__ bool middling(float x) { return x > 1e-18f && x < 1e18f; }
+
+__device__ __forceinline__ uint32_t fp4_block_half(const float (&v)[8], float scale, float inv_scale, uint8_t& sf, float (&back)[8]) {
     uint32_t m = 0;                                             // the largest magnitude, compared as bit patterns so that a NaN stays one
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
     m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    float want = __fdiv_rn(__fdiv_rn(__uint_as_float(m), 6.f), scale);
+    const float most = __uint_as_float(m);
+    const bool plain = middling(most) && middling(scale);
+    float want = plain ? quotient(quotient(most, 6.f, 1.f / 6.f), scale, inv_scale) : __fdiv_rn(__fdiv_rn(most, 6.f), scale);
     want = want > 448.f ? 448.f : want;
     sf = __nv_cvt_float_to_fp8(want, __NV_SATFINITE, __NV_E4M3);
     const float step = __fmul_rn(e4m3_to_float(sf), scale);
     float y[8];
-    if (m < 0x7f800000u && step > 1e-30f && step < 1e30f) {
-        // Quotients by the reciprocal and one correction (Markstein 1990): rounded as a division rounds them, for all of the block one division
+    if (plain && middling(step)) {
         const float inv = __frcp_rn(step);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q = __fmul_rn(v[i], inv);
-            y[i] = __fmaf_rn(__fmaf_rn(-q, step, v[i]), inv, q);
-        }
+        for (int i = 0; i < 8; ++i) y[i] = quotient(v[i], step, inv);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = step > 0.f ? __fdiv_rn(v[i], step) : v[i] != v[i] ? 0.f : copysignf(0.f, v[i]);
@@ -74,10 +89,23 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&v)[8]) {
     for (int i = 0; i < 8; ++i) v[i] = Cvt<T>::to_f(e[i]);
 }
 
+// round(round(v * inv) * w), both to the 16-bit type: the second product of two 16-bit numbers rounds once, as it does from 32 bits.
+template <typename T>
+__device__ __forceinline__ void scale_rows(float (&v)[8], float inv, const uint4& w) {
+    uint4 u = make_uint4(Cvt<T>::pack2(__fmul_rn(v[0], inv), __fmul_rn(v[1], inv)), Cvt<T>::pack2(__fmul_rn(v[2], inv), __fmul_rn(v[3], inv)),
+                         Cvt<T>::pack2(__fmul_rn(v[4], inv), __fmul_rn(v[5], inv)), Cvt<T>::pack2(__fmul_rn(v[6], inv), __fmul_rn(v[7], inv)));
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2* a = reinterpret_cast<T2*>(&u);
+    const T2* b = reinterpret_cast<const T2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = __hmul2_rn(a[i], b[i]);
+    unpack8<T>(u, v);
+}
+
 // Whole heads turn: D/16 lanes a head, a lane holds features 8 l .. and D/2 + 8 l .., which turn together; a warp takes every `parts`-th group of 512 / D heads
 // of a token, whose cos / sin row, norm weights and page look-up it fetches once.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WriteParams p, int parts) {
+__global__ void __launch_bounds__(128, 6) rope_kv_write_fp4_kernel(const Fp4WriteParams p, int parts) {
     pdl_prologue();
     constexpr int L = D / 16, H = 32 / L;                       // lanes of a head, heads of a warp
     const int unit = (int)((blockIdx.x * (long long)blockDim.x + threadIdx.x) >> 5);
@@ -101,16 +129,6 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WritePa
         *reinterpret_cast<float4*>(sn) = *reinterpret_cast<const float4*>(cs + D / 2);
         *reinterpret_cast<float4*>(sn + 4) = *reinterpret_cast<const float4*>(cs + D / 2 + 4);
     }
-    uint4 wq[2], wk[2];
-    wq[0] = wq[1] = wk[0] = wk[1] = make_uint4(0, 0, 0, 0);
-    if (p.q_norm) {
-        wq[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q_norm) + 8 * l);
-        wq[1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q_norm) + D / 2 + 8 * l);
-    }
-    if (p.k_norm) {
-        wk[0] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k_norm) + 8 * l);
-        wk[1] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k_norm) + D / 2 + 8 * l);
-    }
     const int s = p.seq_ids[t];
     const int slot = p.past_len[s] + (p.kv_offsets ? p.kv_offsets[t] : t - p.q_start[s]);
     const int lp = slot / p.page_size, at = slot - lp * p.page_size;
@@ -121,7 +139,7 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WritePa
         stage_at = slot - sl * p.stage_page;
         sp = sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
     }
-    const float scale_k = p.scales[0], scale_v = p.scales[1];
+    const float scale_k = p.scales[0], scale_v = p.scales[1], inv_k = __frcp_rn(scale_k), inv_v = __frcp_rn(scale_v);
     for (int grp = part; grp < groups; grp += parts) {
         const int h = grp * H + hh;
         float lo[8], hi[8];
@@ -137,15 +155,10 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WritePa
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
             if (norm) {
-                const float inv = (float)(1.0 / sqrt(ss / D + (double)p.eps));
-                float w[2][8];
-                unpack8<T>(is_q ? wq[0] : wk[0], w[0]);
-                unpack8<T>(is_q ? wq[1] : wk[1], w[1]);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    lo[i] = Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(lo[i], inv))), w[0][i])));
-                    hi[i] = Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(Cvt<T>::to_f(Cvt<T>::from_f(__fmul_rn(hi[i], inv))), w[1][i])));
-                }
+                const float inv = inverse_root(ss / D + (double)p.eps);
+                const T* nw = reinterpret_cast<const T*>(is_q ? p.q_norm : p.k_norm) + 8 * l;
+                scale_rows<T>(lo, inv, *reinterpret_cast<const uint4*>(nw));
+                scale_rows<T>(hi, inv, *reinterpret_cast<const uint4*>(nw + D / 2));
             }
         }
         if (!is_v) {
@@ -167,7 +180,8 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WritePa
         unpack8<T>(phi, hi);
         uint8_t sf[2];
         float back[2][8];
-        const uint32_t codes_lo = fp4_block_half(lo, is_v ? scale_v : scale_k, sf[0], back[0]), codes_hi = fp4_block_half(hi, is_v ? scale_v : scale_k, sf[1], back[1]);
+        const uint32_t codes_lo = fp4_block_half(lo, is_v ? scale_v : scale_k, is_v ? inv_v : inv_k, sf[0], back[0]);
+        const uint32_t codes_hi = fp4_block_half(hi, is_v ? scale_v : scale_k, is_v ? inv_v : inv_k, sf[1], back[1]);
         if (is_q || h >= heads) continue;
         const int head = is_v ? h - p.hq - p.hkv : h - p.hq;
         if ((unsigned)page < (unsigned)p.num_pages) {           // else: a row that has no page is not stored
@@ -184,7 +198,7 @@ __global__ void __launch_bounds__(128) rope_kv_write_fp4_kernel(const Fp4WritePa
         if ((unsigned)sp < (unsigned)p.stage_pages) {
             T* dst = reinterpret_cast<T*>(p.stage) + ((((size_t)sp * 2 + is_v) * p.hkv + head) * p.stage_page + stage_at) * D + 8 * l;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) back[0][i] = Cvt<T>::to_f(fp4_round<T>(back[0][i])), back[1][i] = Cvt<T>::to_f(fp4_round<T>(back[1][i]));
+            for (int i = 0; i < 8; ++i) back[0][i] = fp4_bound<T>(back[0][i]), back[1][i] = fp4_bound<T>(back[1][i]);
             *reinterpret_cast<uint4*>(dst) = pack8<T>(back[0]);
             *reinterpret_cast<uint4*>(dst + D / 2) = pack8<T>(back[1]);
         }

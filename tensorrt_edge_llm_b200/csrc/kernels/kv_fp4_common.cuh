@@ -32,12 +32,14 @@ __device__ __forceinline__ uint32_t e2m1_pair(float lo, float hi) {
     return r;
 }
 
-// A rounded value in the type of the 16-bit copies: fp16 stops at its largest number.
+// A value before it is rounded to the type of the 16-bit copies: fp16 stops at its largest number.
 template <typename T>
-__device__ __forceinline__ T fp4_round(float v) {
+__device__ __forceinline__ float fp4_bound(float v) {
     if constexpr (std::is_same<T, __half>::value)
         if (fabsf(v) > 65504.f && fabsf(v) < INFINITY) v = copysignf(65504.f, v);
-    return Cvt<T>::from_f(v);
+    return v;
 }
+template <typename T>
+__device__ __forceinline__ T fp4_round(float v) { return Cvt<T>::from_f(fp4_bound<T>(v)); }
 
 }  // namespace telb
