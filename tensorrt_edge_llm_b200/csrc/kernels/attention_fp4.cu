@@ -35,6 +35,10 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -131,14 +135,11 @@ struct KeyTile {
         uint32_t a[D / 32][8];
         operands(a);
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
-#pragma unroll
         for (int j = 0; j < D / 32; ++j)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                mma_f16(acc[n], *reinterpret_cast<const uint32_t(*)[4]>(&a[j][0]), b[n][2 * j][0], b[n][2 * j][1]);
+                if (j == 0) mma_f16_first(acc[n], *reinterpret_cast<const uint32_t(*)[4]>(&a[j][0]), b[n][2 * j][0], b[n][2 * j][1]);
+                else mma_f16(acc[n], *reinterpret_cast<const uint32_t(*)[4]>(&a[j][0]), b[n][2 * j][0], b[n][2 * j][1]);
                 mma_f16(acc[n], *reinterpret_cast<const uint32_t(*)[4]>(&a[j][4]), b[n][2 * j + 1][0], b[n][2 * j + 1][1]);
             }
     }
@@ -148,7 +149,7 @@ struct KeyTile {
 template <int D>
 struct ValueTile {
     uint32_t w[4][D / 64];
-    uint16_t s[4];
+    uint32_t s[4];
     __device__ __forceinline__ static int place(int i, int t) { return key_place(2 * t + (i & 1) + 8 * (i >> 1)); }
     __device__ __forceinline__ void load(const uint8_t* codes, const uint8_t* sf, int g, int t) {
 #pragma unroll
@@ -164,7 +165,7 @@ struct ValueTile {
             else s[i] = *reinterpret_cast<const uint16_t*>(f + 2 * g);
         }
     }
-    // Keys from `live` on: what lies there may be anything, NaN scales too.
+    // Keys from `live` on: what lies there may be anything, NaN scales too (a zero scale takes them out).
     __device__ __forceinline__ void clear(int t, int live) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -174,8 +175,8 @@ struct ValueTile {
     __device__ __forceinline__ void add(const uint32_t (&pb)[NT][2], float (&o)[NT][D / 16][4]) const {
 #pragma unroll
         for (int half = 0; half < (D == 256 ? 2 : 1); ++half) {                  // D = 256: two blocks of 16 features a lane
-            const uint32_t s01 = e4m3x2_to_half((uint16_t)(((s[0] >> (8 * half)) & 0xff) | ((s[1] >> (8 * half)) << 8)));
-            const uint32_t s23 = e4m3x2_to_half((uint16_t)(((s[2] >> (8 * half)) & 0xff) | ((s[3] >> (8 * half)) << 8)));
+            const uint32_t s01 = e4m3x2_to_half((uint16_t)__byte_perm(s[0], s[1], half ? 0x4451 : 0x4440));
+            const uint32_t s23 = e4m3x2_to_half((uint16_t)__byte_perm(s[2], s[3], half ? 0x4451 : 0x4440));
 #pragma unroll
             for (int ww = 0; ww < (D == 64 ? 1 : 2); ++ww) {
                 const int word = half * 2 + ww;
@@ -273,27 +274,25 @@ __device__ __forceinline__ int fp4_locate(const Fp4AttnParams& p, int cols, int 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {       // bytes 0: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 // The tiles of a warp on their way into its own ring in shared memory.  A stage: key codes [32][D/2], value codes, key scales [32][D/16], value scales; with one
 // plane the keys' alone.
 template <int D, int kPlanes = 2>
 struct Fp4Ring {
     static constexpr int kStages = 3, kCodes = kFp4Tile * D / 2, kScales = kFp4Tile * D / 16, kBytes = kPlanes * (kCodes + kScales);
-    const uint8_t* base;                                                         // the head's keys in page 0
+    static constexpr int kScaleLanes = kScales / 16 < 32 ? kScales / 16 : 32;    // lanes that copy one plane's scales
+    // A lane copies its 16 bytes of every 512 of codes, and 16 bytes of scales (or, of wide heads, of every 512): where they lie in page 0, row 0.
+    const uint8_t *keys, *values, *scales;
     const int* table;
-    size_t page_bytes, value_at;
-    int page_shift, max_pages, num_pages, ids_at, ids, end;
-    uint32_t smem;
-    int lane;
+    uint32_t page_bytes, smem;
+    int page_shift, max_pages, num_pages, ids_at, ids, end, lane;
 
     __device__ __forceinline__ void begin(const Fp4AttnParams& p, int seq, int kvh, int end_, uint32_t smem_, int lane_) {
         const size_t slab = fp4_slab_bytes(p.page_size, D);
-        base = p.pool + kvh * slab;
-        page_bytes = 2 * p.hkv * slab;
-        value_at = p.hkv * slab;
+        lane = lane_;
+        keys = p.pool + kvh * slab + lane * 16;
+        values = keys + p.hkv * slab;
+        scales = p.pool + (kvh + (lane / kScaleLanes) * p.hkv) * slab + (size_t)p.page_size * (D / 2) + lane % kScaleLanes * 16;
+        page_bytes = (uint32_t)(2 * p.hkv * slab);
         table = p.page_table + (size_t)seq * p.max_pages;
         page_shift = p.page_shift;
         max_pages = p.max_pages;
@@ -301,7 +300,6 @@ struct Fp4Ring {
         ids_at = -64;
         end = end_;
         smem = smem_;
-        lane = lane_;
     }
     // Pages of the table are looked up 32 at a time.
     __device__ __forceinline__ int page_of(int key) {
@@ -314,50 +312,49 @@ struct Fp4Ring {
         const int page = __shfl_sync(0xffffffffu, ids, lp - ids_at);
         return key < end && (unsigned)page < (unsigned)num_pages ? page : -1;
     }
-    // Starts the copies of a tile; returns a bit per half that has a page (keys from `end` on count as having none).
+    // Starts the copies of a tile; returns a bit per half that has no page (keys from `end` on count as having none).
     __device__ __forceinline__ uint32_t load(int stage, int tile, bool real) {
-        uint32_t there = 0;
+        uint32_t missing = 0;
         if (real) {
-            const int kb = tile * kFp4Tile;
+            const int kb = tile * kFp4Tile, page0 = page_of(kb), at = kb & ((1 << page_shift) - 1);
             const uint32_t dst = smem + stage * kBytes + lane * 16;
-            constexpr int kHalf = 16 * D / 2;                                     // bytes of 16 rows of codes
-            constexpr int kPieces = D / 16;                                       // of 16 bytes, in 16 rows of scales
-            const int page0 = page_of(kb);
             if (page_shift >= 5 && page0 >= 0 && kb + 16 < end) {                 // the whole tile lies in one page
-                const int at = kb & ((1 << page_shift) - 1);
-                const uint8_t* k = base + (size_t)page0 * page_bytes;
-                const uint8_t* c = k + at * (D / 2) + lane * 16;
+                const uint64_t off = (uint64_t)(uint32_t)page0 * page_bytes;
+                const uint8_t *k = keys + off + at * (D / 2), *v = values + off + at * (D / 2), *f = scales + off + at * (D / 16);
 #pragma unroll
-                for (int i = 0; i < 2 * kHalf / 512; ++i) cp_async16(dst + i * 512, c + i * 512);
+                for (int i = 0; i < kCodes / 512; ++i) cp_async16(dst + i * 512, k + i * 512);
                 if constexpr (kPlanes == 2) {
 #pragma unroll
-                    for (int i = 0; i < 2 * kHalf / 512; ++i) cp_async16(dst + kCodes + i * 512, c + value_at + i * 512);
+                    for (int i = 0; i < kCodes / 512; ++i) cp_async16(dst + kCodes + i * 512, v + i * 512);
                 }
-                const uint8_t* f = k + ((size_t)(D / 2) << page_shift) + at * (D / 16);
-#pragma unroll
-                for (int i = lane; i < 2 * kPlanes * kPieces; i += 32)
-                    cp_async16(dst - lane * 16 + kPlanes * kCodes + i * 16, f + (i >= 2 * kPieces ? value_at - 2 * kPieces * 16 : 0) + i * 16);
-                there = 3u;
+                if constexpr (kScaleLanes == 32) {                                // D = 256: a plane's scales are 512 bytes
+                    cp_async16(dst + kPlanes * kCodes, f);
+                    if constexpr (kPlanes == 2) cp_async16(dst + 2 * kCodes + kScales, f + (values - keys));
+                } else if (kPlanes * kScaleLanes == 32 || lane < kPlanes * kScaleLanes) {
+                    cp_async16(dst + kPlanes * kCodes, f);                        // the planes' scales follow one another in the stage
+                }
             } else {
-#pragma unroll
+#pragma unroll 1
                 for (int h = 0; h < 2; ++h) {
-                    const int key = kb + 16 * h, page = page_of(key), at = key & ((1 << page_shift) - 1);
-                    const uint8_t* k = base + (size_t)max(page, 0) * page_bytes;
-                    const uint32_t n = page >= 0 ? 16u : 0u;
-                    if (page >= 0) there |= 1u << h;
+                    const int key = kb + 16 * h, page = page_of(key), in = key & ((1 << page_shift) - 1);
+                    if (page < 0) {
+                        missing |= 1u << h;
+                        continue;
+                    }
+                    const uint64_t off = (uint64_t)(uint32_t)page * page_bytes;
 #pragma unroll
                     for (int v = 0; v < kPlanes; ++v) {
+                        const uint8_t* c = (v ? values : keys) + off + in * (D / 2);
+                        const uint8_t* f = (v ? values : keys) + off + ((size_t)(D / 2) << page_shift) + in * (D / 16);
 #pragma unroll
-                        for (int i = 0; i < kHalf / 512; ++i)
-                            cp_async16(dst + v * kCodes + h * kHalf + i * 512, k + v * value_at + (size_t)at * (D / 2) + i * 512 + lane * 16, n);
-                        if (lane < kPieces)
-                            cp_async16(dst + kPlanes * kCodes + v * kScales + h * (kScales / 2), k + v * value_at + ((size_t)(D / 2) << page_shift) + (size_t)at * (D / 16) + lane * 16, n);
+                        for (int i = 0; i < kCodes / 1024; ++i) cp_async16(dst + v * kCodes + h * (kCodes / 2) + i * 512, c + i * 512);
+                        if (lane < kScales / 32) cp_async16(dst + kPlanes * kCodes + v * kScales + h * (kScales / 2), f);
                     }
                 }
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        return there;
+        return missing;
     }
 };
 
@@ -410,26 +407,8 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
         ref[n][0] = ref[n][1] = kRefStart;
         sum[n][0] = sum[n][1] = 0.f;
     }
-    int stage = 0;
-    for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
-        const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
-        __syncwarp();                                                        // the stage to be filled has been read by all lanes
-        const uint32_t more = ring.load(ahead, next, next < tile1);
-        flags = (flags & ~(3u << (2 * ahead))) | (more << (2 * ahead));
-        next += kFp4Warps;
-        asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
-        __syncwarp();
-        const uint8_t* st = ring_ptr + stage * Ring::kBytes;
-        const uint32_t there = (flags >> (2 * stage)) & 3u;
-        const int kb = tile * kFp4Tile;
-        float s[2][NT][4];
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-            KeyTile<D> kt;
-            kt.load(st + m * (16 * D / 2), st + 2 * Ring::kCodes + m * D, g, t);
-            kt.template scores<NT>(qb, s[m]);
-        }
-        const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there == 3u;
+    // Scores of a tile to probabilities, and those times its values.
+    auto take = [&](auto open, const uint8_t* st, int kb, uint32_t missing, const float (&s)[2][NT][4]) {
         float x[2][NT][4];
         auto shifted = [&]() {
 #pragma unroll
@@ -438,7 +417,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) x[m][n][i] = fmaf(s[m][n][i], factor[n][i & 1], -ref[n][i & 1]);
-            if (!open) {
+            if constexpr (!decltype(open)::value) {
 #pragma unroll
                 for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -446,7 +425,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1);
-                            if (!((there >> m) & 1u) || key < low[n][i & 1] || key >= high[n][i & 1]) x[m][n][i] = -INFINITY;
+                            if (((missing >> m) & 1u) || key < low[n][i & 1] || key >= high[n][i & 1]) x[m][n][i] = -INFINITY;
                         }
             }
         };
@@ -499,9 +478,31 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
             }
             ValueTile<D> vt;
             vt.load(st + Ring::kCodes + m * (16 * D / 2), st + 2 * Ring::kCodes + Ring::kScales + m * D, g, t);
-            if (!open) vt.clear(t, end - kb - 16 * m);
+            if constexpr (!decltype(open)::value) vt.clear(t, (missing >> m) & 1u ? 0 : end - kb - 16 * m);
             vt.template add<NT>(pb, o);
         }
+    };
+    int stage = 0;
+    for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
+        const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
+        __syncwarp();                                                        // the stage to be filled has been read by all lanes
+        flags = (flags & ~(3u << (2 * ahead))) | (ring.load(ahead, next, next < tile1) << (2 * ahead));
+        next += kFp4Warps;
+        asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
+        __syncwarp();
+        const uint8_t* st = ring_ptr + stage * Ring::kBytes;
+        const uint32_t missing = (flags >> (2 * stage)) & 3u;
+        const int kb = tile * kFp4Tile;
+        float s[2][NT][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            KeyTile<D> kt;
+            kt.load(st + m * (16 * D / 2), st + 2 * Ring::kCodes + m * D, g, t);
+            kt.template scores<NT>(qb, s[m]);
+        }
+        // A tile that every column sees whole takes no masks; the code for the others stands apart
+        if (kb >= all_low && kb + kFp4Tile <= all_high && missing == 0u) take(std::true_type(), st, kb, missing, s);
+        else take(std::false_type(), st, kb, missing, s);
         stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -820,10 +821,9 @@ __global__ void __launch_bounds__(kFp4Warps * 32, D == 256 ? 2 : 3) attention_fp
         for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
             const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
             __syncwarp();
-            const uint32_t more = ring.load(ahead, next, next < tile1);
-            flags = (flags & ~(3u << (2 * ahead))) | (more << (2 * ahead));
+            flags = (flags & ~(3u << (2 * ahead))) | (ring.load(ahead, next, next < tile1) << (2 * ahead));
             next += kFp4Warps;
-            const uint32_t there = (flags >> (2 * stage)) & 3u;
+            const uint32_t there = ~(flags >> (2 * stage)) & 3u;
             const int kb = tile * kFp4Tile;
             // a lane's own key: half t / 2, row g or g + 8 of it
             const int mine = kb + 16 * (t >> 1) + key_place(g) + 8 * (t & 1);
@@ -972,6 +972,7 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     const int columns = p.max_q_len * (p.hq / p.hkv), cols = fp4_columns(columns, d);
     if (p.max_items != p.hkv * ((columns + cols - 1) / cols)) return fail("telb_paged_attention_fp4: items of another size");
     if (p.max_items > 65535) return fail("telb_paged_attention_fp4: too many rows x heads");
+    if (2LL * p.hkv * p.page_size * (d / 2 + d / 16) >= 1LL << 31) return fail("telb_paged_attention_fp4: pages of less than 2 GB");
     if (p.num_seqs > 65535) return fail("telb_paged_attention_fp4: more than 65535 sequences");
     if (p.weights && (!p.stat || weight_ctas < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
     if (is_bf16) {
