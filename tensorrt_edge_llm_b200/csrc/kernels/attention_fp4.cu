@@ -899,6 +899,7 @@ int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t st
     if (dev < 0 || dev >= 64 || !configured[dev]) {
         cudaError_t e = cudaFuncSetAttribute(attention_fp4_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4)", e);
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
@@ -967,7 +968,7 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (d != 64 && d != 128 && d != 256) return fail("telb_paged_attention_fp4: head_dim must be 64, 128 or 256");
     if (p.page_size < 16 || p.page_size != 1 << p.page_shift) return fail("telb_paged_attention_fp4: the page size must be a power of two, at least 16");
     if (p.hkv <= 0 || p.hq % p.hkv) return fail("telb_paged_attention_fp4: query heads must be a multiple of the KV heads");
-    if (p.ranks < 0 || p.ranks > 8) return fail("telb_paged_attention_fp4: clusters of at most 8 CTAs");
+    if (p.ranks < 0 || p.ranks > 16) return fail("telb_paged_attention_fp4: clusters of at most 16 CTAs");
     if (p.ranks == 0 && (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans)) return fail("telb_paged_attention_fp4: no room for the parts");
     const int columns = p.max_q_len * (p.hq / p.hkv), cols = fp4_columns(columns, d);
     if (p.max_items != p.hkv * ((columns + cols - 1) / cols)) return fail("telb_paged_attention_fp4: items of another size");
