@@ -23,12 +23,12 @@ struct Fp4AttnParams {
     const float *scales, *sinks;
     float* weights;
     int2* spans;
-    int num_seqs, tokens, max_q_len, num_pages, max_pages, page_size, page_shift, hq, hkv, window, ctas, ranks, max_items;
+    float4* scores;
+    int num_seqs, tokens, max_q_len, num_pages, max_pages, page_size, page_shift, hq, hkv, window, ctas, ranks, max_items, tiles, pairs;
     float scale, decay;
 };
 
 constexpr int kFp4Warps = 4, kFp4Tile = 32;               // warps of a CTA; keys that a warp takes at a time
-constexpr int kFp4WeightSmem = 200 << 10;
 constexpr float kRefStart = -1e30f;
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -274,11 +274,10 @@ __device__ __forceinline__ int fp4_locate(const Fp4AttnParams& p, int cols, int 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// The tiles of a warp on their way into its own ring in shared memory.  A stage: key codes [32][D/2], value codes, key scales [32][D/16], value scales; with one
-// plane the keys' alone.
-template <int D, int kPlanes = 2>
+// The tiles of a warp on their way into its own ring in shared memory.  A stage: key codes [32][D/2], value codes, key scales [32][D/16], value scales.
+template <int D>
 struct Fp4Ring {
-    static constexpr int kStages = 3, kCodes = kFp4Tile * D / 2, kScales = kFp4Tile * D / 16, kBytes = kPlanes * (kCodes + kScales);
+    static constexpr int kStages = 3, kCodes = kFp4Tile * D / 2, kScales = kFp4Tile * D / 16, kBytes = 2 * (kCodes + kScales);
     static constexpr int kScaleLanes = kScales / 16 < 32 ? kScales / 16 : 32;    // lanes that copy one plane's scales
     // A lane copies its 16 bytes of every 512 of codes, and 16 bytes of scales (or, of wide heads, of every 512): where they lie in page 0, row 0.
     const uint8_t *keys, *values, *scales;
@@ -323,15 +322,13 @@ struct Fp4Ring {
                 const uint8_t *k = keys + off + at * (D / 2), *v = values + off + at * (D / 2), *f = scales + off + at * (D / 16);
 #pragma unroll
                 for (int i = 0; i < kCodes / 512; ++i) cp_async16(dst + i * 512, k + i * 512);
-                if constexpr (kPlanes == 2) {
 #pragma unroll
-                    for (int i = 0; i < kCodes / 512; ++i) cp_async16(dst + kCodes + i * 512, v + i * 512);
-                }
+                for (int i = 0; i < kCodes / 512; ++i) cp_async16(dst + kCodes + i * 512, v + i * 512);
                 if constexpr (kScaleLanes == 32) {                                // D = 256: a plane's scales are 512 bytes
-                    cp_async16(dst + kPlanes * kCodes, f);
-                    if constexpr (kPlanes == 2) cp_async16(dst + 2 * kCodes + kScales, f + (values - keys));
-                } else if (kPlanes * kScaleLanes == 32 || lane < kPlanes * kScaleLanes) {
-                    cp_async16(dst + kPlanes * kCodes, f);                        // the planes' scales follow one another in the stage
+                    cp_async16(dst + 2 * kCodes, f);
+                    cp_async16(dst + 2 * kCodes + kScales, f + (values - keys));
+                } else if (2 * kScaleLanes == 32 || lane < 2 * kScaleLanes) {
+                    cp_async16(dst + 2 * kCodes, f);                              // the planes' scales follow one another in the stage
                 }
             } else {
 #pragma unroll 1
@@ -343,12 +340,12 @@ struct Fp4Ring {
                     }
                     const uint64_t off = (uint64_t)(uint32_t)page * page_bytes;
 #pragma unroll
-                    for (int v = 0; v < kPlanes; ++v) {
+                    for (int v = 0; v < 2; ++v) {
                         const uint8_t* c = (v ? values : keys) + off + in * (D / 2);
                         const uint8_t* f = (v ? values : keys) + off + ((size_t)(D / 2) << page_shift) + in * (D / 16);
 #pragma unroll
                         for (int i = 0; i < kCodes / 1024; ++i) cp_async16(dst + v * kCodes + h * (kCodes / 2) + i * 512, c + i * 512);
-                        if (lane < kScales / 32) cp_async16(dst + kPlanes * kCodes + v * kScales + h * (kScales / 2), f);
+                        if (lane < kScales / 32) cp_async16(dst + 2 * kCodes + v * kScales + h * (kScales / 2), f);
                     }
                 }
             }
@@ -407,6 +404,10 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
         ref[n][0] = ref[n][1] = kRefStart;
         sum[n][0] = sum[n][1] = 0.f;
     }
+    const int all_chunks = (p.max_q_len * group + 7) / 8;
+    const int first_tile = fp4_first_tile(past, p.window);
+    float4* keep = nullptr;                                                      // of the sequence's first tile
+    if (p.scores && t < p.pairs) keep = p.scores + (((size_t)seq * p.hkv + kvh) * all_chunks + chunk * NT) * p.tiles * 16 * p.pairs + g * p.pairs + t;
     // Scores of a tile to probabilities, and those times its values.
     auto take = [&](auto open, const uint8_t* st, int kb, uint32_t missing, const float (&s)[2][NT][4]) {
         float x[2][NT][4];
@@ -430,6 +431,23 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
             }
         };
         shifted();
+        const int nth = kb / kFp4Tile - first_tile;
+        if (keep != nullptr && nth < p.tiles) {                                  // for the accumulated weights
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float v[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        v[i] = s[m][n][i] * factor[n][i & 1];
+                        if constexpr (!decltype(open)::value)
+                            if (x[m][n][i] == -INFINITY) v[i] = -INFINITY;
+                    }
+                    if (NT == 1 || chunk * NT + n < all_chunks)
+                        keep[((size_t)n * p.tiles + nth) * 16 * p.pairs + m * 8 * p.pairs] = make_float4(v[0], v[1], v[2], v[3]);
+                }
+        }
         float most = -INFINITY;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -761,131 +779,56 @@ __global__ void __launch_bounds__(512) attention_fp4_merge_kernel(const Fp4AttnP
 }
 
 // Accumulated attention weights: weights[page, head, slot] = decay * weights + the sum over the step's rows and the group's heads of
-// exp2(score - top) / sum, for keys that some row sees; the step's own keys start from zero.  The scores are made again: that reads the keys, half of what
-// the step has read, where keeping them would write and read 4 bytes for each (key, column).  A CTA takes a part of the line of all (sequence, KV
-// head, tile); the queries of its item stand in shared memory as the operands that the products take.  A warp owns its keys, so that every sum has one order.
-template <typename T, int D>
-__global__ void __launch_bounds__(kFp4Warps * 32, D == 256 ? 2 : 3) attention_fp4_weights_kernel(const Fp4AttnParams p) {
+// exp2(score - top) / sum, for keys that some row sees; the step's own keys start from zero.  The attention kernel has left its scores (4 bytes for each
+// key and column, mostly still in the L2 cache); making them again took the keys, their expansion and the products a second time (16 sequences of 8192:
+// 36 us against 8).  A warp owns 32 keys, so that every sum has one order.  grid (groups of 4 tiles, KV heads, sequences)
+__global__ void __launch_bounds__(128) attention_fp4_weights_kernel(const Fp4AttnParams p) {
     pdl_prologue();
-    using Ring = Fp4Ring<D, 1>;
-    constexpr int kAll = 1 << 24, kOperand = D * 16;                             // columns of an item: all; bytes of 8 columns' operands
-    extern __shared__ __align__(16) uint8_t smem[];                              // rings, operands [chunks][D/32][32 lanes] uint4, columns [chunks][8] float4
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = p.hq / p.hkv, most_chunks = (p.max_q_len * group + 7) / 8;
-    uint8_t* operands = smem + kFp4Warps * Ring::kStages * Ring::kBytes;
-    float4* params = reinterpret_cast<float4*>(operands + (size_t)most_chunks * kOperand);       // factor, top, 1 / sum, limit (as an int)
-    const Fp4Line line = fp4_line(p, kAll, lane);
-    int at = blockIdx.x * line.per;
-    const int stop = min(line.total, at + line.per);
-    if (at >= stop) return;
-    int seq_start = 0, seq = fp4_locate(p, kAll, lane, at, seq_start);
-    const float base = p.scale * 1.4426950408889634f * p.scales[0];
-    const uint32_t ring_at = smem_u32(smem) + warp * Ring::kStages * Ring::kBytes;
-    const uint8_t* ring_ptr = smem + warp * Ring::kStages * Ring::kBytes;
-    while (at < stop) {
-        const int ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
-        const int tiles = fp4_tiles(past, ql, p.window);
-        if (at >= seq_start + tiles * p.hkv) {
-            seq_start += tiles * p.hkv;
-            ++seq;
-            continue;
-        }
-        const int kvh = (at - seq_start) / tiles, off = (at - seq_start) - kvh * tiles;
-        const int count = min(tiles - off, stop - at);
-        const int tile0 = fp4_first_tile(past, p.window) + off, tile1 = tile0 + count;
-        const int q0 = p.q_start[seq], chunks = min((columns + 7) / 8, most_chunks);
-        const int first = p.window > 0 ? max(0, past + 1 - p.window) : 0, end = past + ql;
-        const int all_low = p.window > 0 ? max(0, end - p.window) : 0, all_high = past + 1;       // visible to every row
-
-        Ring ring;
-        ring.begin(p, seq, kvh, end, ring_at, lane);
-        uint32_t flags = 0;
-        int next = tile0 + warp;
+    const int seq = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = p.hq / p.hkv, ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
+    const int index = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (index >= min(fp4_tiles(past, ql, p.window), p.tiles)) return;
+    const int kb = (fp4_first_tile(past, p.window) + index) * kFp4Tile, first = p.window > 0 ? max(0, past + 1 - p.window) : 0;
+    // a lane's own key: half t / 2, row g or g + 8 of it
+    const int mine = kb + 16 * (t >> 1) + key_place(g) + 8 * (t & 1), lp = mine >> p.page_shift;
+    const int page = mine >= first && mine < past + ql && lp < p.max_pages ? p.page_table[(size_t)seq * p.max_pages + lp] : -1;
+    float* w = (unsigned)page < (unsigned)p.num_pages ? p.weights + ((size_t)page * p.hkv + kvh) * p.page_size + (mine & (p.page_size - 1)) : nullptr;
+    const float old = w && mine < past ? p.decay * *w : 0.f;
+    const int all_chunks = (p.max_q_len * group + 7) / 8, chunks = min((columns + 7) / 8, all_chunks), q0 = p.q_start[seq];
+    const float4* src = p.scores + (((size_t)seq * p.hkv + kvh) * all_chunks * p.tiles + index) * 16 * p.pairs + g * p.pairs + t;
+    float given[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    if (t < p.pairs) {
+#pragma unroll 4
+        for (int ch = 0; ch < chunks; ++ch) {
+            float4 s[2];
 #pragma unroll
-        for (int s = 0; s < Ring::kStages - 1; ++s, next += kFp4Warps) flags |= ring.load(s, next, next < tile1) << (2 * s);
-        for (int ch = warp; ch < chunks; ch += kFp4Warps) {
-            const int c = ch * 8 + g, r = c / group, h = kvh * group + c - r * group;
-            uint32_t qb[D / 16][2];
-            const size_t row = (size_t)(q0 + r) * p.hq + h;
-            const float up = load_query<T, D>(reinterpret_cast<const T*>(p.q) + row * D + t * (D / 4), c < columns, qb);
+            for (int m = 0; m < 2; ++m) s[m] = src[(size_t)ch * p.tiles * 16 * p.pairs + m * 8 * p.pairs];
+            float2 st[2];
 #pragma unroll
-            for (int j = 0; j < D / 32; ++j)
-                *reinterpret_cast<uint4*>(operands + (size_t)ch * kOperand + (j * 32 + lane) * 16) = make_uint4(qb[2 * j][0], qb[2 * j][1], qb[2 * j + 1][0], qb[2 * j + 1][1]);
-            if (t == 0) {
-                const float2 st = c < columns ? *reinterpret_cast<const float2*>(p.stat + row * 2) : make_float2(0.f, 0.f);
-                params[ch * 8 + g] = make_float4(base * up, st.x, st.y, __int_as_float(c < columns ? past + r + 1 : 0));
+            for (int c = 0; c < 2; ++c) {
+                const int col = ch * 8 + 2 * t + c, r = col / group;
+                st[c] = col < columns ? *reinterpret_cast<const float2*>(p.stat + ((size_t)(q0 + r) * p.hq + kvh * group + col - r * group) * 2) : make_float2(0.f, 0.f);
             }
-        }
-        __syncthreads();
-        int stage = 0;
-        for (int tile = tile0 + warp; tile < tile1; tile += kFp4Warps) {
-            const int ahead = stage == 0 ? Ring::kStages - 1 : stage - 1;
-            __syncwarp();
-            flags = (flags & ~(3u << (2 * ahead))) | (ring.load(ahead, next, next < tile1) << (2 * ahead));
-            next += kFp4Warps;
-            const uint32_t there = ~(flags >> (2 * stage)) & 3u;
-            const int kb = tile * kFp4Tile;
-            // a lane's own key: half t / 2, row g or g + 8 of it
-            const int mine = kb + 16 * (t >> 1) + key_place(g) + 8 * (t & 1);
-            const int page = ((there >> (t >> 1)) & 1u) && mine >= first && mine < end ? ring.table[mine >> p.page_shift] : -1;
-            float* w = page >= 0 ? p.weights + ((size_t)page * p.hkv + kvh) * p.page_size + (mine & (p.page_size - 1)) : nullptr;
-            const float old = w && mine < past ? p.decay * *w : 0.f;
-            asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 1) : "memory");
-            __syncwarp();
-            const uint8_t* st = ring_ptr + stage * Ring::kBytes;
-            KeyTile<D> kt[2];
-            uint32_t a[2][D / 32][8];
 #pragma unroll
             for (int m = 0; m < 2; ++m) {
-                kt[m].load(st + m * (16 * D / 2), st + Ring::kCodes + m * D, g, t);
-                kt[m].operands(a[m]);
-            }
-            const bool open = kb >= all_low && kb + kFp4Tile <= all_high && there == 3u;
-            float given[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-            for (int ch = 0; ch < chunks; ++ch) {
-                float s[2][4];
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[m][i] = 0.f;
-#pragma unroll
-                for (int j = 0; j < D / 32; ++j) {
-                    const uint4 b = *reinterpret_cast<const uint4*>(operands + (size_t)ch * kOperand + (j * 32 + lane) * 16);
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {
-                        mma_f16(s[m], *reinterpret_cast<const uint32_t(*)[4]>(&a[m][j][0]), b.x, b.y);
-                        mma_f16(s[m], *reinterpret_cast<const uint32_t(*)[4]>(&a[m][j][4]), b.z, b.w);
-                    }
+                given[m][0] += exp2_approx(s[m].x - st[0].x) * st[0].y;
+                given[m][1] += exp2_approx(s[m].z - st[0].x) * st[0].y;
+                if (ch * 8 + 2 * t + 1 < columns) {                              // the last column may have no neighbour
+                    given[m][0] += exp2_approx(s[m].y - st[1].x) * st[1].y;
+                    given[m][1] += exp2_approx(s[m].w - st[1].x) * st[1].y;
                 }
-                const float4 col[2] = {params[ch * 8 + 2 * t], params[ch * 8 + 2 * t + 1]};
-#pragma unroll
-                for (int m = 0; m < 2; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float4 c = col[i & 1];
-                        float e = exp2_approx(fmaf(s[m][i], c.x, -c.y));
-                        if (!open) {
-                            const int key = kb + 16 * m + key_place(g) + 8 * (i >> 1), high = __float_as_int(c.w);
-                            if (key >= high || (p.window > 0 && key < high - p.window)) e = 0.f;
-                        }
-                        given[m][i >> 1] = fmaf(e, c.z, given[m][i >> 1]);
-                    }
             }
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 1);
-                    given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 2);
-                }
-            const float sum = t & 2 ? (t & 1 ? given[1][1] : given[1][0]) : (t & 1 ? given[0][1] : given[0][0]);
-            if (w) *w = old + sum;
-            stage = stage + 1 == Ring::kStages ? 0 : stage + 1;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        at += count;
-        if (at < stop) __syncthreads();                                          // the operands make room for the next item's
     }
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 1);
+            given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 2);
+        }
+    const float sum = t & 2 ? (t & 1 ? given[1][1] : given[1][0]) : (t & 1 ? given[0][1] : given[0][0]);
+    if (w) *w = old + sum;
 }
 
 template <typename T, int D, int NT>
@@ -926,23 +869,12 @@ int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t st
 }
 
 template <typename T, int D>
-int launch_attention_fp4(const Fp4AttnParams& p, int weight_ctas, cudaStream_t stream) {
+int launch_attention_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
     const int columns = p.max_q_len * (p.hq / p.hkv);
     constexpr int kMost = D == 256 ? 1 : 2;
     const int rc = columns <= 8 ? launch_attention_fp4_nt<T, D, 1>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost>(p, columns, stream);
     if (rc || !p.weights) return rc;
-    using Ring = Fp4Ring<D, 1>;
-    const int chunks = (columns + 7) / 8, smem = kFp4Warps * Ring::kStages * Ring::kBytes + chunks * (D * 16 + 128);
-    if (smem > kFp4WeightSmem) return fail("telb_paged_attention_fp4: too many rows x heads of a KV head for accumulated weights");
-    static bool configured[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(attention_fp4_weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp4WeightSmem);
-        if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4_weights)", e);
-        if (dev >= 0 && dev < 64) configured[dev] = true;
-    }
-    TELB_LAUNCH("attention_fp4_weights_kernel", (attention_fp4_weights_kernel<T, D>), dim3(weight_ctas), dim3(kFp4Warps * 32), smem, stream, p);
+    TELB_LAUNCH("attention_fp4_weights_kernel", attention_fp4_weights_kernel, dim3((p.tiles + 3) / 4, p.hkv, p.num_seqs), dim3(128), 0, stream, p);
     return 0;
 }
 
@@ -960,9 +892,9 @@ extern "C" int telb_attention_fp4_ctas(int columns, int d) {
 
 // ranks > 0: clusters of so many CTAs per item (sequence, KV head, C columns); 0: the line of all items' tiles cut into `ctas` parts, with
 // part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C: 8, or 16 for more than 8 columns of at most 128 features; max_items = KV heads x chunks of the longest
-// sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2] is scratch and its keys are cut
-// into `weight_ctas` parts.
-extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int weight_ctas, int is_bf16, cudaStream_t stream) {
+// sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2]
+// and `scores` [num_seqs, hkv, columns / 8, tiles, 2, 8, pairs] float4 are scratch: `tiles` of 32 keys hold every sequence's, `pairs` columns of 8 (at most 4).
+extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int is_bf16, cudaStream_t stream) {
     const Fp4AttnParams& p = *params;
     if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
     if (d != 64 && d != 128 && d != 256) return fail("telb_paged_attention_fp4: head_dim must be 64, 128 or 256");
@@ -975,13 +907,14 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (p.max_items > 65535) return fail("telb_paged_attention_fp4: too many rows x heads");
     if (2LL * p.hkv * p.page_size * (d / 2 + d / 16) >= 1LL << 31) return fail("telb_paged_attention_fp4: pages of less than 2 GB");
     if (p.num_seqs > 65535) return fail("telb_paged_attention_fp4: more than 65535 sequences");
-    if (p.weights && (!p.stat || weight_ctas < 1 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the softmax statistics");
+    if (p.weights && (!p.stat || !p.scores || p.tiles < 1 || p.pairs < 1 || p.pairs > 4 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the scores");
+    if (!p.weights && p.scores) return fail("telb_paged_attention_fp4: scores are kept for weights");
     if (is_bf16) {
-        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, weight_ctas, stream);
-        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, weight_ctas, stream);
-        return launch_attention_fp4<__nv_bfloat16, 256>(p, weight_ctas, stream);
+        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, stream);
+        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, stream);
+        return launch_attention_fp4<__nv_bfloat16, 256>(p, stream);
     }
-    if (d == 128) return launch_attention_fp4<__half, 128>(p, weight_ctas, stream);
-    if (d == 64) return launch_attention_fp4<__half, 64>(p, weight_ctas, stream);
-    return launch_attention_fp4<__half, 256>(p, weight_ctas, stream);
+    if (d == 128) return launch_attention_fp4<__half, 128>(p, stream);
+    if (d == 64) return launch_attention_fp4<__half, 64>(p, stream);
+    return launch_attention_fp4<__half, 256>(p, stream);
 }

@@ -660,7 +660,7 @@ def _fp4_lib():
     """The kernel library with the argument types of these entry points."""
     L, i, p = lib(), c_int, c_vp
     L.telb_rope_kv_write_fp4.argtypes = [ctypes.c_char_p, i, i, p]
-    L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, i, p]
+    L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, p]
     L.telb_attention_fp4_ctas.argtypes = [i, i]
     L.telb_kv_fp4_stage.argtypes = [p] * 7 + [i] * 9 + [p]
     L.telb_kv_evict.argtypes = [ctypes.c_char_p, p]
@@ -668,7 +668,7 @@ def _fp4_lib():
 
 
 _FP4_WRITE = struct.Struct("15P11if")       # Fp4WriteParams (csrc/kernels/kv_fp4.cu)
-_FP4_ATTN = struct.Struct("14P13i2f")       # Fp4AttnParams (csrc/kernels/attention_fp4.cu)
+_FP4_ATTN = struct.Struct("15P15i2f0P")     # Fp4AttnParams (csrc/kernels/attention_fp4.cu)
 _EVICT = struct.Struct("6P12i")             # EvictParams (csrc/kernels/kv_evict.cu)
 
 
@@ -808,20 +808,21 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
         ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(columns, d), n * items * tiles // 4))
     elif ctas < 0:
         ranks, ctas = -ctas, 0
-    part_o = part_ml = spans = stat = 0
+    part_o = part_ml = spans = stat = scores = pairs = 0
     if ctas or weights is not None:
-        # parts of outputs, their references and sums, (first, last) CTA of every item; softmax statistics of the rows
-        room = (2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items if ctas else 0, 2 * t * hq if weights is not None else 0)
+        # parts of outputs, their references and sums, (first, last) CTA of every item; for the weights, scores of every key and column and the rows' statistics
+        pairs = 0 if weights is None else min(4, (columns + 1) // 2)
+        room = (n * hkv * -(-columns // 8) * tiles * 64 * pairs, 2 * ctas * cols * d, 4 * ctas * cols, 2 * n * items if ctas else 0, 2 * t * hq if pairs else 0)
         ws = torch.empty(sum(room), dtype=torch.float32, device=q.device)
-        part_o = ws.data_ptr()
-        part_ml = part_o + 4 * room[0]
-        spans = part_ml + 4 * room[1]
-        stat = spans + 4 * room[2] if weights is not None else 0
+        scores = ws.data_ptr() if pairs else 0
+        part_o = ws.data_ptr() + 4 * room[0]
+        part_ml = part_o + 4 * room[1]
+        spans = part_ml + 4 * room[2]
+        stat = spans + 4 * room[3] if pairs else 0
     ptr = _ptrs("paged_attention_fp4", dev, (q, kv_layer, out, meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights))
-    p = _FP4_ATTN.pack(*ptr[:3], part_o, part_ml, stat, *ptr[3:], spans, n, t, meta.max_q_len, pages, meta.page_table.shape[1], meta.page_size,
-                       meta.page_size.bit_length() - 1, hq, hkv, window, ctas, ranks, items, scale, decay)
-    weight_ctas = max(1, min(2 * 148 if columns > 64 else 3 * 148, n * hkv * tiles // 4))
-    _check(L.telb_paged_attention_fp4(p, d, weight_ctas, is_bf16, _raw_stream(dev)), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None))
+    p = _FP4_ATTN.pack(*ptr[:3], part_o, part_ml, stat, *ptr[3:], spans, scores, n, t, meta.max_q_len, pages, meta.page_table.shape[1], meta.page_size,
+                       meta.page_size.bit_length() - 1, hq, hkv, window, ctas, ranks, items, tiles, pairs, scale, decay)
+    _check(L.telb_paged_attention_fp4(p, d, is_bf16, _raw_stream(dev)), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None))
     return out
 
 
