@@ -106,7 +106,7 @@ def main() -> int:
     ap.add_argument("--dtype", default="nvfp4", choices=["nvfp4", "bf16", "fp16"])
     ap.add_argument("--layers", type=int, default=None, help="debug only; anything but the full depth is not the named config")
     ap.add_argument("--comm", default="fused", choices=["fused", "nccl"])
-    ap.add_argument("--kv-cache-dtype", default="model", choices=["model", "fp8"],
+    ap.add_argument("--kv-cache-dtype", default="model", choices=["model", "fp8", "nvfp4"],
                     help="KV page storage; anything but the default (the compute type) is not the named headline configuration")
     args = ap.parse_args()
     if args.impl == "reference":

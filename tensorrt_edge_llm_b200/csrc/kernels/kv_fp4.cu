@@ -312,44 +312,87 @@ __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4Wr
     }
 }
 
-// A CTA per page of the 16-bit copy (64 rows; sequence blockIdx.y, logical page blockIdx.x) and plane (K|V, head) blockIdx.z.  Rows from `count` on, up
-// to the page's end, become zero.
-template <typename T>
-__global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table, const int* __restrict__ past_len,
-                                                           const int* __restrict__ q_len, const int* __restrict__ page_table,
-                                                           const float* __restrict__ scales, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d,
-                                                           int window) {
+// A CTA per page of the 16-bit copy (64 rows; logical page blockIdx.x, plane (K|V, head) blockIdx.y, sequence blockIdx.z); a thread expands blocks of 16
+// features.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table,
+                                                           const int* __restrict__ past_len, const int* __restrict__ q_len, const int* __restrict__ page_table,
+                                                           const float* __restrict__ scales, int max_pages, int num_pages, int page_shift, int stage_pages, int hkv,
+                                                           int window, int own) {
     pdl_prologue();
-    const int seq = blockIdx.y, lp = blockIdx.x, plane = blockIdx.z;
+    const int seq = blockIdx.z, lp = blockIdx.x, plane = blockIdx.y;
     if (plane == 0 && threadIdx.x == 0) stage_table[seq * stage_pages + lp] = seq * stage_pages + lp;
-    const int past = past_len[seq];
-    const int count = past + (q_len ? q_len[seq] : 0);
+    const int past = past_len[seq], total = past + q_len[seq], count = own ? total : past;
     if (window > 0 && (lp + 1) * 64 + 2 * 128 <= past - window) return;        // before every tile that the windowed kernels touch
-    const size_t slab = fp4_slab_bytes(page_size, d);
+    const size_t slab = fp4_slab_bytes(1 << page_shift, D);
     const float scale = scales ? scales[plane >= hkv] : 1.f;
-    T* dst = stage + (((size_t)seq * stage_pages + lp) * 2 * hkv + plane) * 64 * d;
-    for (int i = threadIdx.x; i < 64 * d / 8; i += blockDim.x) {
-        const int r = i / (d / 8), e = (i - r * (d / 8)) * 8, slot = lp * 64 + r;
-        alignas(16) T out[8];
-        int page = -1;
-        if (slot < count && slot / page_size < max_pages) page = page_table[(size_t)seq * max_pages + slot / page_size];
-        if ((unsigned)page >= (unsigned)num_pages) {
+    T* dst = stage + (((size_t)seq * stage_pages + lp) * 2 * hkv + plane) * 64 * D;
+    constexpr int B = D / 16;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) out[j] = Cvt<T>::from_f(0.f);
-        } else {
+    for (int u = 0; u < 64 * B / 256; ++u) {
+        const int i = u * 256 + threadIdx.x, r = i / B, b = i % B, slot = lp * 64 + r;
+        if (slot >= count && slot < total) continue;
+        const int page = slot < count && slot >> page_shift < max_pages ? page_table[(size_t)seq * max_pages + (slot >> page_shift)] : -1;
+        uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if ((unsigned)page < (unsigned)num_pages) {
             const uint8_t* src = pool + ((size_t)page * 2 * hkv + plane) * slab;
-            const int at = slot % page_size;
-            uint32_t h[4];
-            e2m1x8_to_half(*reinterpret_cast<const uint32_t*>(src + (size_t)at * (d / 2) + e / 2), h[0], h[1], h[2], h[3]);
-            const float step = __fmul_rn(e4m3_to_float(src[(size_t)page_size * (d / 2) + (size_t)at * (d / 16) + e / 16]), scale);
+            const int at = slot & ((1 << page_shift) - 1);
+            const uint2 w = *reinterpret_cast<const uint2*>(src + (size_t)at * (D / 2) + b * 8);
+            const float step = __fmul_rn(e4m3_to_float(src[((size_t)(D / 2) << page_shift) + (size_t)at * B + b]), scale);
+            uint32_t h[8];
+            e2m1x8_to_half(w.x, h[0], h[1], h[2], h[3]);
+            e2m1x8_to_half(w.y, h[4], h[5], h[6], h[7]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
-                out[2 * j] = fp4_round<T>(__fmul_rn(f.x, step));
-                out[2 * j + 1] = fp4_round<T>(__fmul_rn(f.y, step));
+            for (int half = 0; half < 2; ++half) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[4 * half + j]));
+                    v[2 * j] = fp4_bound<T>(__fmul_rn(f.x, step));
+                    v[2 * j + 1] = fp4_bound<T>(__fmul_rn(f.y, step));
+                }
+                out[half] = pack8<T>(v);
             }
         }
-        *reinterpret_cast<uint4*>(dst + (size_t)r * d + e) = *reinterpret_cast<const uint4*>(out);
+        *reinterpret_cast<uint4*>(dst + (size_t)r * D + b * 16) = out[0];
+        *reinterpret_cast<uint4*>(dst + (size_t)r * D + b * 16 + 8) = out[1];
+    }
+}
+
+// Rows of accepted draft tokens move together: the row at slot past + path[j] to past + j, j from 1, of every layer, plane and head.  All words of a row
+// (codes, then block scales) are read before any is written.
+constexpr int kCommitWords = 12;                                // of a thread
+template <int D>
+__global__ void __launch_bounds__(256) kv_fp4_commit_path_kernel(uint8_t* __restrict__ pool, const int* __restrict__ page_table, const int* __restrict__ past_len,
+                                                                 const int* __restrict__ path, const int* __restrict__ path_len, int max_path, int max_pages,
+                                                                 int num_pages, int hkv, int page_size) {
+    pdl_prologue();
+    constexpr int kCodes = D / 8, kWords = kCodes + D / 64;     // 32-bit words of a row: codes, all
+    const int b = blockIdx.x, head = blockIdx.y % hkv, plane = blockIdx.y / hkv;       // plane: layer * 2 + (K|V)
+    const int m = min(path_len[b], max_path) - 1;               // rows to move (path[0] is the root and stays)
+    if (m <= 0) return;
+    const int past = past_len[b];
+    const size_t slab = fp4_slab_bytes(page_size, D);
+    auto word_at = [&](int slot, int w) -> uint32_t* {
+        const int lp = slot / page_size, page = lp < max_pages ? page_table[(size_t)b * max_pages + lp] : -1, at = slot - lp * page_size;
+        if ((unsigned)page >= (unsigned)num_pages) return nullptr;
+        uint8_t* s = pool + ((((size_t)(plane >> 1) * num_pages + page) * 2 + (plane & 1)) * hkv + head) * slab;
+        return reinterpret_cast<uint32_t*>(w < kCodes ? s + (size_t)at * (D / 2) + w * 4 : s + (size_t)page_size * (D / 2) + (size_t)at * (D / 16) + (w - kCodes) * 4);
+    };
+    uint32_t v[kCommitWords];
+    const int total = m * kWords;
+#pragma unroll
+    for (int i = 0; i < kCommitWords; ++i) {
+        const int x = threadIdx.x + i * 256, j = x / kWords + 1, w = x % kWords;
+        const uint32_t* src = x < total ? word_at(past + path[(size_t)b * max_path + j], w) : nullptr;
+        v[i] = src ? *src : 0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kCommitWords; ++i) {
+        const int x = threadIdx.x + i * 256, j = x / kWords + 1, w = x % kWords;
+        uint32_t* dst = x < total ? word_at(past + j, w) : nullptr;
+        if (dst) *dst = v[i];
     }
 }
 
@@ -397,20 +440,46 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
     return 0;
 }
 
-// pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [num_seqs * stage_pages, 2, Hkv, 64, d], page s * stage_pages + i for rows 64 i.. of sequence s.  `q_len` null: only the
-// rows that were cached before this step.  `scales` null: code * block scale, which both 16-bit types hold exactly.
+// pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [num_seqs * stage_pages, 2, Hkv, 64, d], page s * stage_pages + i for
+// rows 64 i.. of sequence s.  own: the step's own rows too.  `scales` null: code * block scale, which both 16-bit types hold exactly.
 extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table, const int* past_len, const int* q_len, const int* page_table, const float* scales,
-                                 int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d, int window, int is_bf16,
+                                 int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d, int window, int own, int is_bf16,
                                  cudaStream_t stream) {
     if (num_seqs <= 0 || stage_pages <= 0) return 0;
-    if (d % 16 || page_size % 16) return fail("telb_kv_fp4_stage: head_dim and page size must be multiples of 16");
+    if (d != 64 && d != 128 && d != 256) return fail("telb_kv_fp4_stage: head_dim must be 64, 128 or 256");
+    if (page_size < 16 || page_size & (page_size - 1)) return fail("telb_kv_fp4_stage: the page size must be a power of two, at least 16");
     if (num_seqs > 65535 || 2 * hkv > 65535) return fail("telb_kv_fp4_stage: more than 65535 sequences or planes");
-    const dim3 grid(stage_pages, num_seqs, 2 * hkv), blk(256);
-    if (is_bf16)
-        TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<__nv_bfloat16>), grid, blk, 0, stream, (const uint8_t*)pool, (__nv_bfloat16*)stage, stage_table, past_len,
-                    q_len, page_table, scales, max_pages, num_pages, page_size, stage_pages, hkv, d, window);
-    else
-        TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<__half>), grid, blk, 0, stream, (const uint8_t*)pool, (__half*)stage, stage_table, past_len, q_len,
-                    page_table, scales, max_pages, num_pages, page_size, stage_pages, hkv, d, window);
+    int shift = 0;
+    while (1 << shift < page_size) ++shift;
+    const dim3 grid(stage_pages, 2 * hkv, num_seqs), blk(256);
+#define STAGE_FP4(T, D) TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<T, D>), grid, blk, 0, stream, (const uint8_t*)pool, (T*)stage, stage_table, past_len, q_len, \
+                                    page_table, scales, max_pages, num_pages, shift, stage_pages, hkv, window, own)
+    if (is_bf16) {
+        if (d == 128) STAGE_FP4(__nv_bfloat16, 128);
+        else if (d == 64) STAGE_FP4(__nv_bfloat16, 64);
+        else STAGE_FP4(__nv_bfloat16, 256);
+    } else {
+        if (d == 128) STAGE_FP4(__half, 128);
+        else if (d == 64) STAGE_FP4(__half, 64);
+        else STAGE_FP4(__half, 256);
+    }
+#undef STAGE_FP4
+    return 0;
+}
+
+// pool: all layers [layers, num_pages, 2, hkv, slab].
+extern "C" int telb_kv_fp4_commit_path(void* pool, const int* page_table, const int* past_len, const int* path, const int* path_len, int batch, int max_path,
+                                       int max_pages, int layers, int num_pages, int hkv, int page_size, int d, cudaStream_t stream) {
+    if (batch <= 0 || layers <= 0) return 0;
+    if (d != 64 && d != 128 && d != 256) return fail("telb_kv_fp4_commit_path: head_dim must be 64, 128 or 256");
+    if ((max_path - 1) * (d / 8 + d / 64) > 256 * kCommitWords) return fail("telb_kv_fp4_commit_path: accepted path too long for one block");
+    if (2LL * layers * hkv > 65535) return fail("telb_kv_fp4_commit_path: more than 65535 planes");
+    const dim3 grid(batch, layers * 2 * hkv), blk(256);
+#define COMMIT_FP4(D) TELB_LAUNCH("kv_fp4_commit_path_kernel", (kv_fp4_commit_path_kernel<D>), grid, blk, 0, stream, (uint8_t*)pool, page_table, past_len, path, path_len, \
+                                  max_path, max_pages, num_pages, hkv, page_size)
+    if (d == 128) COMMIT_FP4(128);
+    else if (d == 64) COMMIT_FP4(64);
+    else COMMIT_FP4(256);
+#undef COMMIT_FP4
     return 0;
 }

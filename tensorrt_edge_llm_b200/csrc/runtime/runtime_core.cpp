@@ -325,7 +325,9 @@ long long LLMEngineConfig::kv_bytes_per_token() const {
         return n * eb;
     }
     const int kvh = std::max(1, num_kv_heads / std::max(1, world_size));
-    return 2LL * num_attention_layers() * kvh * head_dim * eb;
+    const long long elements = 2LL * num_attention_layers() * kvh * head_dim;
+    if (kv_cache_dtype == "nvfp4" || kv_cache_dtype == "NVFP4") return elements * 9 / 16;       // codes of four bits, an E4M3 scale per 16
+    return elements * eb;
 }
 
 long long LLMEngineConfig::kv_pool_bytes() const {

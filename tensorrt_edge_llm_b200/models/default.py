@@ -78,7 +78,7 @@ class Attention(nn.Module):
         else:
             self.q_norm = self.k_norm = None
         self.prefix = prefix
-        self.register_buffer("kv_scales", torch.ones(2, dtype=torch.float32))      # FP8 KV cache: K and V dequantisation scales
+        self.register_buffer("kv_scales", torch.ones(2, dtype=torch.float32))      # FP8 / four-bit KV cache: K and V dequantisation scales
         if getattr(cfg, "attention_sink_bias", False):
             # one learned logit per (local) query head with no value row: it only grows the softmax denominator
             # (reference: tensorrt_edgellm/config.py:691-692, the draft models' attention_sink_bias buffer)
@@ -100,8 +100,20 @@ class Attention(nn.Module):
                                           out_scale=gs, sinks=self.attention_sink_bias)
         return self.o_proj(o if gs is not None else o.reshape(o.shape[0], -1))
 
+    def _forward_fp4(self, qkv, meta, kv_layer, cos_sin):
+        """Four-bit pages: rows are quantised as they are written.  Steps of few rows read the pages in place; the others attend over 16-bit
+        pages of the step's sequences, which hold the cached rows expanded and the step's own as they were rounded."""
+        heads = (self.num_q_heads, self.num_kv_heads, self.head_dim, self.kv_scales, None if self.q_norm is None else self.q_norm.weight,
+                 None if self.k_norm is None else self.k_norm.weight, self.eps)
+        if ops.fp4_direct(meta, self.num_q_heads // self.num_kv_heads):
+            q = ops.rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, *heads)
+            return ops.paged_attention_fp4(q, kv_layer, meta, self.scale, self.kv_scales, sliding_window=self.sliding_window, sinks=self.attention_sink_bias)
+        stage, staged = ops.kv_fp4_stage(kv_layer, meta, self.kv_scales, qkv.dtype, self.sliding_window or 0)
+        q = ops.rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, *heads, stage=stage, stage_table=staged.page_table)
+        return ops.paged_attention(q, stage, staged, self.scale, self.sliding_window, self.attention_sink_bias)
+
     def load_checkpoint(self, fetch) -> bool:
-        """FP8 KV-cache scales of quantised checkpoints (``k_proj.k_scale`` / ``v_proj.v_scale``, one per layer)."""
+        """FP8 and four-bit KV-cache scales of quantised checkpoints (``k_proj.k_scale`` / ``v_proj.v_scale``, one per layer)."""
         for i, name in enumerate(("k_proj.k_scale", "v_proj.v_scale")):
             t = fetch(f"{self.prefix}.{name}")
             if t is not None:
@@ -121,8 +133,8 @@ class Attention(nn.Module):
 
     def _forward_shared_kv(self, x, meta, kv_layer, cos_sin):
         """KV-shared layer: queries only; ``kv_layer`` is the donor's cache, already holding this step's rows."""
-        if kv_layer.dtype == torch.float8_e4m3fn:
-            raise NotImplementedError("KV-shared layers over an FP8 cache are not built")
+        if kv_layer.dtype in (torch.float8_e4m3fn, torch.uint8):
+            raise NotImplementedError("KV-shared layers over an FP8 or four-bit cache are not built")
         q = ops.rope_q(self.qkv_proj(x), kv_layer, meta, cos_sin, self.num_q_heads, self.head_dim,
                        None if self.q_norm is None else self.q_norm.weight, self.eps)
         o = ops.paged_attention(q, kv_layer, meta, self.scale, self.sliding_window, self.attention_sink_bias)
@@ -134,6 +146,9 @@ class Attention(nn.Module):
         qkv = self.qkv_proj(x)
         if self.k_eq_v or self.value_norm:
             qkv = self._derive_values(qkv)
+        if kv_layer.dtype == torch.uint8:
+            o = self._forward_fp4(qkv, meta, kv_layer, cos_sin)
+            return self.o_proj(o.reshape(o.shape[0], -1))
         pool_layer = None
         if kv_layer.dtype == torch.float8_e4m3fn:
             pool_layer = kv_layer

@@ -227,6 +227,9 @@ def stream_norm(stream, weight, eps, *, delta=None, routed=None, mult=1.0, step=
     return ref.stream_norm(*args)
 
 
+FP4_DIRECT_COLUMNS = 64      # rows x heads of a KV head up to which a step reads four-bit pages in place
+
+
 @dataclass
 class Bigram:
     """Second embedding of a token: row ``(previous * mul_prev + token * mul_cur) mod buckets`` of ``table``, row ``buckets`` where a
@@ -393,10 +396,16 @@ def rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, num_q_heads, num_kv_heads, h
     return f(qkv, kv_layer, meta, cos_sin, num_q_heads, num_kv_heads, head_dim, scales, q_norm_w, k_norm_w, eps, stage, stage_table)
 
 
+def fp4_direct(meta, group):
+    """Whether :func:`paged_attention_fp4` reads the pages of this step (``group`` query heads a KV head) in place."""
+    return meta.tree_mask is None and meta.max_q_len * group <= FP4_DIRECT_COLUMNS
+
+
 def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
     """16-bit copies of the rows that the step's sequences have in a four-bit layer, for the prompt kernels: ``(stage, meta)`` with the pages
-    ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  Rows cached before the step, with ``new_rows`` the step's own too; what
-    lies behind them in a page is zero.  ``window`` > 0: pages that no row of the step can see may be left out."""
+    ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  The rows cached before the step, and its own with ``new_rows`` (else their
+    places are left for :func:`rope_kv_write_fp4` to fill); what lies behind in a page is zero.  ``window`` > 0: pages that no row of the
+    step can see may be left out."""
     f = cuda_ops().kv_fp4_stage if kv_layer.is_cuda else ref.kv_fp4_stage
     return f(kv_layer, meta, scales, dtype, window, new_rows)
 

@@ -16,7 +16,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from . import reference as ref_ops
+from . import fp4_direct, reference as ref_ops
 from .meta import StepMeta
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_lib", "libtelb_kernels.so")
@@ -662,8 +662,9 @@ def _fp4_lib():
     L.telb_rope_kv_write_fp4.argtypes = [ctypes.c_char_p, i, i, p]
     L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, p]
     L.telb_attention_fp4_ctas.argtypes = [i, i]
-    L.telb_kv_fp4_stage.argtypes = [p] * 7 + [i] * 9 + [p]
+    L.telb_kv_fp4_stage.argtypes = [p] * 7 + [i] * 10 + [p]
     L.telb_kv_evict.argtypes = [ctypes.c_char_p, p]
+    L.telb_kv_fp4_commit_path.argtypes = [p] * 5 + [i] * 8 + [p]
     return L
 
 
@@ -737,13 +738,22 @@ def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int
     stage = torch.empty(n * per, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
     table = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device)
     _check(_fp4_lib().telb_kv_fp4_stage(
-        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, meta.past_len, meta.q_len if new_rows else None, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
-        meta.page_size, per, hkv, d, window or 0, int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
+        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, meta.past_len, meta.q_len, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
+        meta.page_size, per, hkv, d, window or 0, int(new_rows), int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
     return stage, dataclasses.replace(meta, page_table=table, page_size=64)
 
 
-FP4_DIRECT_COLUMNS = 64      # rows x heads of a KV head up to which a step reads four-bit pages in place
-FP4_WEIGHT_COLUMNS = 256     # and up to which it keeps account of the attention weights
+FP4_WEIGHT_COLUMNS = 256     # rows x heads of a KV head up to which a step keeps account of the attention weights
+
+
+def _fp4_commit_path(pool, page_table, past_len, path, path_len) -> None:
+    """:func:`kv_commit_path` of four-bit pages, whose rows lie in two parts of a page."""
+    layers, pages, _, hkv, psz, row = pool.shape
+    ref_ops.fp4_head_dim(pool[0])
+    pt, pl, pth, pln = (v.to(torch.int32).contiguous() for v in (page_table, past_len, path, path_len))
+    dev = pool.get_device()
+    _check(_fp4_lib().telb_kv_fp4_commit_path(*_ptrs("kv_commit_path", dev, (pool, pt, pl, pth, pln)), pth.shape[0], pth.shape[1], pt.shape[1], layers, pages, hkv, psz,
+                                              row * 16 // 9, _raw_stream(dev)), "kv_commit_path")
 
 
 def _fp4_ranks(items: int, tiles: int) -> int:
@@ -789,7 +799,7 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
         if sinks.dtype != torch.float32 or not sinks.is_contiguous() or not sinks.is_cuda:
             sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
     if direct is None:
-        direct = weights is not None or (meta.tree_mask is None and columns <= FP4_DIRECT_COLUMNS)
+        direct = weights is not None or fp4_direct(meta, hq // hkv)
     if not direct or meta.tree_mask is not None:
         if direct:
             raise ValueError("paged_attention_fp4: tree masks are read by the prompt kernels only")
@@ -920,6 +930,8 @@ def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sin
         sliding_window, kernel = -1, "tile"
     if sinks is not None:
         sinks = sinks.to(device=q.device, dtype=torch.float32).contiguous()
+    if kv_layer.dtype == torch.uint8:
+        raise TypeError("paged_attention: four-bit pages are read by paged_attention_fp4")
     q = q.contiguous()
     t, hq, d = q.shape
     hkv = kv_layer.shape[2]
@@ -2112,6 +2124,8 @@ def candidate_rescore(hidden, lm_head, cand):
 
 def kv_commit_path(pool, page_table, past_len, path, path_len) -> None:
     assert pool.is_contiguous() and pool.element_size() in (1, 2)
+    if pool.dtype == torch.uint8:
+        return _fp4_commit_path(pool, page_table, past_len, path, path_len)
     if pool.element_size() == 1:            # FP8 pages: a row of D bytes moves as D / 2 16-bit elements
         pool = pool.view(torch.int16)
     layers, pages, _, hkv, psz, d = pool.shape

@@ -1036,6 +1036,11 @@ def kv_commit_path(pool: torch.Tensor, page_table: torch.Tensor, past_len: torch
                    path_len: torch.Tensor) -> None:
     """Compact the accepted path in the paged cache ``pool [L, pages, 2, Hkv, P, D]``: the entry at
     slot ``past + path[j]`` moves to slot ``past + j`` (``j ≥ 1``), in place."""
+    if pool.dtype == torch.uint8:               # four-bit pages: a row's codes and its block scales lie apart
+        for layer in pool:
+            for part in fp4_page_parts(layer):
+                kv_commit_path(part[None].view(torch.int8), page_table, past_len, path, path_len)
+        return
     p = pool.shape[4]
     for i in range(path.shape[0]):
         past, m = int(past_len[i]), int(path_len[i])

@@ -21,11 +21,11 @@ def build_quant_config(quantization: str, exclude: Sequence[str] = ("lm_head",),
     """The ``hf_quant_config.json`` body for one of the supported weight formats."""
     if quantization not in _ALGOS or _ALGOS[quantization] is None:
         raise ValueError(f"unsupported quantization {quantization!r}; choose one of {sorted(k for k, v in _ALGOS.items() if v)}")
-    if kv_cache_quantization not in (None, "fp8"):
-        raise ValueError("kv_cache_quantization must be fp8 or unset")
+    if kv_cache_quantization not in (None, "fp8", "nvfp4"):
+        raise ValueError("kv_cache_quantization must be fp8, nvfp4 or unset")
     return {"producer": {"name": "tensorrt_edge_llm_b200"},
             "quantization": {"quant_algo": _ALGOS[quantization], "group_size": group_size or (16 if quantization == "nvfp4" else 128),
-                             "kv_cache_quant_algo": "FP8" if kv_cache_quantization == "fp8" else None,
+                             "kv_cache_quant_algo": kv_cache_quantization.upper() if kv_cache_quantization else None,
                              "exclude_modules": list(exclude)}}
 
 

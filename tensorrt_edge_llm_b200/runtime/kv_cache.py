@@ -61,7 +61,8 @@ class KVCacheManager:
                  max_pages_per_seq: int = 64, device="cpu", dtype: Optional[torch.dtype] = None,
                  num_layers: Optional[int] = None, bounded_swa: Optional[bool] = None, kv_dtype: Optional[str] = None):
         """``kv_dtype``: ``"fp8"`` stores keys and values as E4M3 bytes (half the bytes per cached token; the attention layers
-        work on a 16-bit staging copy of the pages a step touches, see ``csrc/kernels/kv_fp8.cu``); ``None`` / ``"auto"`` follows
+        work on a 16-bit staging copy of the pages a step touches, see ``csrc/kernels/kv_fp8.cu``); ``"nvfp4"`` stores E2M1 codes
+        with an E4M3 scale per 16 features (9/32 of the 16-bit bytes, layout: :func:`ops.rope_kv_write_fp4`); ``None`` / ``"auto"`` follows
         the checkpoint's ``kv_cache_quant`` setting; ``"fp16"`` / ``"bf16"`` / ``"model"`` keep the compute type."""
         self.cfg = cfg
         # Bounded sliding-window storage (``cpp/runtime/state/boundedSwaKVPageManager.cpp`` in the reference): every
@@ -85,13 +86,22 @@ class KVCacheManager:
         self.num_layers = num_layers if num_layers is not None else sum(t in KV_LAYERS for t in cfg.layer_types)
         hkv = max(cfg.num_key_value_heads // cfg.tp_size, 1)
         self.dtype = dtype or cfg.compute_dtype
-        if kv_dtype in (None, "auto"):
+        asked = kv_dtype not in (None, "auto")
+        if not asked:
             kv_dtype = getattr(cfg.quant, "kv_cache_quant", None)
         self.kv_fp8 = str(kv_dtype).lower() in ("fp8", "fp8_e4m3", "e4m3") and dtype is None
         if self.kv_fp8:
             if cfg.head_dim % 16:
                 raise ValueError("an FP8 KV cache needs a head_dim that is a multiple of 16")
             self.dtype = torch.float8_e4m3fn
+        self.kv_fp4 = str(kv_dtype).lower() in ("nvfp4", "fp4") and dtype is None
+        if self.kv_fp4:
+            why = self._fp4_unsupported(cfg, page_size, device, num_layers)
+            if why and asked:
+                raise ValueError(f"a four-bit KV cache {why}")
+            self.kv_fp4 = not why            # a checkpoint's own setting gives way to the compute type
+        if self.kv_fp4:
+            self.dtype = torch.uint8
         # Stacks whose attention layers have sizes of their own, or cache one latent row per token instead of keys and values: one
         # tensor per layer, all indexed by the same page table (the pool tensor is empty then and only names the device, the type and
         # the page count).
@@ -106,7 +116,8 @@ class KVCacheManager:
                                      for n, (h, d) in zip(planes, geometry)]
             elif geometry:
                 hkv, head_dim = geometry[0]
-        self.pool = torch.zeros(0 if self._layer_pools else self.num_layers, num_pages, 2, hkv, page_size, head_dim, dtype=self.dtype, device=device)
+        row = head_dim * 9 // 16 if self.kv_fp4 else head_dim        # four-bit rows: codes and block scales
+        self.pool = torch.zeros(0 if self._layer_pools else self.num_layers, num_pages, 2, hkv, page_size, row, dtype=self.dtype, device=device)
         # hybrid models: model layer index → attention pool index, plus the recurrent state pools
         self._attn_index = {}
         for i, t in enumerate(cfg.layer_types):
@@ -115,7 +126,7 @@ class KVCacheManager:
         self.recurrent = None
         if cfg.is_hybrid:
             from ..models.nemotron_h import RecurrentState
-            self.recurrent = RecurrentState(cfg, max_seats, device, cfg.compute_dtype if self.kv_fp8 else self.dtype)
+            self.recurrent = RecurrentState(cfg, max_seats, device, cfg.compute_dtype if self.kv_fp8 or self.kv_fp4 else self.dtype)
         self.alloc = PageAllocator(num_pages)
         self.table = torch.full((max_seats, max_pages_per_seq), -1, dtype=torch.int32)   # host truth
         self.lengths = [0] * max_seats
@@ -128,6 +139,23 @@ class KVCacheManager:
             self.native = _rt.KVPageTable(num_pages, page_size, max_seats, max_pages_per_seq)
         except ImportError:
             self.native = None
+
+    @staticmethod
+    def _fp4_unsupported(cfg: ModelConfig, page_size: int, device, num_layers: Optional[int]) -> Optional[str]:
+        """Why four-bit pages cannot hold this model's cache, or None."""
+        if cfg.head_dim not in (64, 128, 256):
+            return "needs a head_dim of 64, 128 or 256"
+        if page_size < 16 or page_size & (page_size - 1):
+            return "needs pages of a power of two of rows, at least 16"
+        if torch.device(device).type == "cuda" and cfg.compute_dtype == torch.float32:
+            return "on the GPU takes 16-bit activations"
+        if num_layers is not None:
+            return "is not built for draft heads"
+        if cfg.kv_geometry() is not None:
+            return "is not built for stacks with per-layer attention sizes"
+        if any(cfg.kv_donor(i) >= 0 for i in range(cfg.num_hidden_layers)):
+            return "is not built for KV-shared layers"
+        return None
 
     def kv_layer(self, model_layer: int) -> torch.Tensor:
         """KV pool of attention layer ``model_layer`` (index into the model's layer list)."""

@@ -62,7 +62,7 @@ class ModelConfig:
     max_input_len: int = 4096
     max_batch_size: int = 1
     max_kv_cache_capacity: int = 8192
-    kv_cache_dtype: str = "auto"                   # auto (follow the checkpoint's kv_cache_quant) | fp8 | model
+    kv_cache_dtype: str = "auto"                   # auto (follow the checkpoint's kv_cache_quant) | fp8 | nvfp4 | model
     speculative_config: Optional[SpeculativeConfig] = None
     context_cache_config: ContextCacheConfig = field(default_factory=ContextCacheConfig)
     multimodal_config: MultimodalConfig = field(default_factory=MultimodalConfig)
@@ -147,8 +147,8 @@ def create_argument_parser(prog: str = "trtedge serve") -> argparse.ArgumentPars
     m.add_argument("--max-input-len", type=int, default=4096)
     m.add_argument("--max-batch-size", type=int, default=1)
     m.add_argument("--max-kv-cache-capacity", type=int, default=8192)
-    m.add_argument("--kv-cache-dtype", "--kv-cache-quantization", dest="kv_cache_dtype", default="auto", choices=["auto", "fp8", "model"],
-                   help="KV page storage: fp8 = E4M3 bytes (half the memory per cached token); auto follows the checkpoint")
+    m.add_argument("--kv-cache-dtype", "--kv-cache-quantization", dest="kv_cache_dtype", default="auto", choices=["auto", "fp8", "nvfp4", "model"],
+                   help="KV page storage: fp8 = E4M3 bytes (half the memory per cached token), nvfp4 = E2M1 codes with block scales (9/32); auto follows the checkpoint")
     m.add_argument("--enable-in-flight-batching", action="store_true")
     m.add_argument("--ifb-scheduling-mode", default="auto", choices=["auto", "mixed", "prefill_first", "single_cohort"])
     m.add_argument("--max-num-tokens", type=int, default=0)

@@ -48,7 +48,12 @@ def test_stage_is_the_host_formulation(dtype, d, page):
     for new in (False, True):
         want, meta_w = ref.kv_fp4_stage(layer, meta, scales, dtype, 0, new)
         got, meta_g = ops.kv_fp4_stage(layer.cuda(), meta.to("cuda"), scales.cuda(), dtype, 0, new)
-        assert torch.equal(meta_g.page_table.cpu(), meta_w.page_table) and torch.equal(got.cpu(), want)
+        got = got.cpu()
+        if not new:                                   # the step's own rows are left for the write
+            for q, past, row in ((2, 70, 0), (1, 0, 1), (5, 128, 2)):
+                for slot in range(past, past + q):
+                    got[meta_w.page_table[row, slot // 64], :, :, slot % 64] = 0.0
+        assert torch.equal(meta_g.page_table.cpu(), meta_w.page_table) and torch.equal(got, want)
 
 
 # q_lens, past, query heads, KV heads, head size, page, window
@@ -266,3 +271,59 @@ def test_refusals_on_the_gpu():
                  lambda: ops.kv_evict(lg.transpose(2, 3), w, m.page_table, m.past_len, m.page_table, 4)):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_commit_path_moves_codes_and_scales(d):
+    g = torch.Generator().manual_seed(d)
+    pool = torch.randint(0, 256, (3, 9, 2, 2, 32, d * 9 // 16), generator=g, dtype=torch.uint8)
+    table = torch.tensor([[4, 1, 0], [2, 5, -1], [7, 8, 3]], dtype=torch.int32)
+    past, path = torch.tensor([30, 3, 0]), torch.tensor([[0, 2, 5, 6], [0, 1, 4, 0], [0, 0, 0, 0]])
+    plen = torch.tensor([4, 3, 1])
+    got = pool.cuda()
+    ops.kv_commit_path(got, table.cuda(), past.cuda(), path.int().cuda(), plen.int().cuda())
+    ops.kv_commit_path(pool, table, past, path, plen)
+    assert torch.equal(got.cpu(), pool)
+
+
+@pytest.mark.parametrize("family", ["dense", "window"])
+def test_model_with_four_bit_kv_eager_and_graph(family):
+    """Chunked prompts, steps and captured steps on the GPU against the same model on the host, and tree steps against plain ones."""
+    from tensorrt_edge_llm_b200 import AutoModel
+    from tensorrt_edge_llm_b200.config import tiny_llama_config
+    from tensorrt_edge_llm_b200.runtime.kv_cache import KVCacheManager
+    from tensorrt_edge_llm_b200.runtime.runner import ModelRunner
+    dev = torch.device("cuda", 0)
+    cfg = tiny_llama_config(num_hidden_layers=3, vocab_size=512, dtype="bfloat16", head_dim=128, num_attention_heads=4, num_key_value_heads=2, hidden_size=512)
+    if family == "window":
+        cfg.sliding_window = 100
+    model, host = AutoModel.from_config(cfg, device=dev, random_init=0), AutoModel.from_config(cfg, device="cpu", random_init=0)
+    host.load_state_dict(model.state_dict())
+    g = torch.Generator().manual_seed(5)
+    prompts = torch.randint(0, cfg.vocab_size, (2, 300), generator=g).tolist()
+    feed = torch.randint(0, cfg.vocab_size, (5, 2), generator=g).tolist()
+
+    def run(m, device, kv_dtype, graphs=True):
+        kv = KVCacheManager(cfg, num_pages=24, page_size=64, max_seats=2, max_pages_per_seq=10, device=device, kv_dtype=kv_dtype)
+        r = ModelRunner(m, kv, max_num_tokens=256)
+        r.use_cuda_graphs = graphs and device != "cpu"
+        out = [r.prefill([0, 1], prompts).float()]
+        for toks in feed:
+            out.append(r.step([0, 1], [[t] for t in toks]).float())
+        many = r.step([0, 1], [[3, 5, 7], [11, 13, 17]], logits_all=True).float()
+        mask = torch.tensor([[1], [3], [7]] * 2, dtype=torch.int32, device=device)      # a chain as a tree: the same rows through the prompt kernels
+        for s in (0, 1):
+            kv.rewind(s, kv.lengths[s] - 3)
+        tree = r.step([0, 1], [[3, 5, 7], [11, 13, 17]], logits_all=True, tree_mask=mask).float()
+        toks = r.decode_greedy([0, 1], out[-1].argmax(-1).to(torch.int32), 12)
+        return torch.stack(out).cpu(), many.cpu(), tree.cpu(), toks.cpu(), kv
+
+    full = run(model, dev, "model")
+    four, many, tree, toks, kv = run(model, dev, "nvfp4")
+    assert kv.pool.dtype == torch.uint8
+    want, many_h, _, _, _ = run(host, "cpu", "nvfp4")
+    cos = lambda a, b: float(torch.nn.functional.cosine_similarity(a.flatten(1), b.flatten(1), dim=1).min())
+    # bf16 layers: a code on a border may fall to either side of it, as in any two orders of the same sums
+    assert cos(four, want) > 0.995 and cos(many, many_h) > 0.995 and cos(tree, many) > 0.995
+    assert cos(full[0], four) > 0.95
+    assert torch.equal(run(model, dev, "nvfp4", graphs=False)[3], toks)

@@ -5,9 +5,12 @@ import pytest
 import torch
 
 from fp4_kv_cases import make_step, oracle_attention, oracle_evict, page_values
-from tensorrt_edge_llm_b200 import ops
+from tensorrt_edge_llm_b200 import AutoModel, ops
+from tensorrt_edge_llm_b200.config import QuantConfig, tiny_llama_config
 from tensorrt_edge_llm_b200.ops import build_step_meta
 from tensorrt_edge_llm_b200.ops import reference as ref
+from tensorrt_edge_llm_b200.runtime.kv_cache import KVCacheManager
+from tensorrt_edge_llm_b200.runtime.runner import ModelRunner
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
@@ -77,11 +80,102 @@ def test_stage_holds_the_rows_and_zeros_behind_them():
     for new in (False, True):
         stage, staged = ops.kv_fp4_stage(layer, meta, scales, torch.bfloat16, new_rows=new)
         for s, (ql, past) in enumerate(((2, 70), (1, 3))):
-            rows = past + (ql if new else 0)
             for slot in range(staged.page_table.shape[1] * 64):
+                if past <= slot < past + ql and not new:          # left for the write
+                    continue
                 got = stage[staged.page_table[s, slot // 64], :, :, slot % 64]
-                want = vals[meta.page_table[s, slot // 32], :, :, slot % 32].bfloat16() if slot < rows else torch.zeros(())
+                want = vals[meta.page_table[s, slot // 32], :, :, slot % 32].bfloat16() if slot < past + ql else torch.zeros(())
                 assert (got == want).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_commit_path_moves_codes_and_scales(d):
+    g = torch.Generator().manual_seed(d)
+    pool = torch.randint(0, 256, (2, 6, 2, 3, 16, d * 9 // 16), generator=g, dtype=torch.uint8)
+    table = torch.tensor([[4, 1, 0], [2, 5, -1]], dtype=torch.int32)
+    past, path, plen = torch.tensor([14, 3]), torch.tensor([[0, 2, 5, 6], [0, 1, 4, 0]]), torch.tensor([4, 3])
+    want = pool.clone()
+    for layer in range(2):
+        src, dst = ref.fp4_page_parts(pool[layer]), ref.fp4_page_parts(want[layer])
+        for b in range(2):
+            for j in range(1, int(plen[b])):
+                a, z = int(past[b] + path[b, j]), int(past[b]) + j
+                for x, y in zip(src, dst):
+                    y[table[b, z // 16], :, :, z % 16] = x[table[b, a // 16], :, :, a % 16]
+    ops.kv_commit_path(pool, table, past, path, plen)
+    assert torch.equal(pool, want)
+
+
+def _run(model, cfg, prompts, feed, kv_dtype, page=64, max_tokens=8192):
+    kv = KVCacheManager(cfg, num_pages=40, page_size=page, max_seats=2, max_pages_per_seq=16, kv_dtype=kv_dtype)
+    r = ModelRunner(model, kv, max_num_tokens=max_tokens)
+    out = [r.prefill([0, 1], prompts)]
+    for toks in feed:
+        out.append(r.step([0, 1], [[t] for t in toks]))
+    return torch.stack(out), kv
+
+
+@pytest.mark.parametrize("head,page,chunk", [(64, 64, 8192), (128, 16, 64), (64, 32, 32)])
+def test_model_over_four_bit_pages_is_the_model_whose_rows_are_rounded(head, page, chunk, monkeypatch):
+    """The same logits as a 16-bit cache whose rows are rounded to what four bits hold as they are written, in whole and chunked prompts and steps."""
+    cfg = tiny_llama_config(num_hidden_layers=2, vocab_size=256, dtype="float32", head_dim=head, num_attention_heads=4, num_key_value_heads=2, hidden_size=128)
+    model = AutoModel.from_config(cfg, random_init=0)
+    g = torch.Generator().manual_seed(7)
+    prompts = [torch.randint(0, 256, (n,), generator=g).tolist() for n in (90, 67)]
+    feed = torch.randint(0, 256, (4, 2), generator=g).tolist()
+    for layer in model.model.layers:
+        layer.self_attn.kv_scales.copy_(torch.tensor([0.003, 0.002]))
+    got, kv4 = _run(model, cfg, prompts, feed, "nvfp4", page, chunk)
+    assert kv4.pool.dtype == torch.uint8 and kv4.bytes_per_token == 2 * 2 * 2 * head * 9 // 16
+    plain = ref.rope_kv_write
+
+    def rounded(qkv, kv_layer, meta, *a, **kw):
+        q = plain(qkv, kv_layer, meta, *a, **kw)
+        sid = meta.seq_ids.long()
+        slot = meta.past_len.long()[sid] + torch.arange(qkv.shape[0]) - meta.q_start.long()[sid]
+        pg, at = meta.page_table.long()[sid, slot // page], slot % page
+        kv_layer[pg, :, :, at] = ref.fp4_encode_rows(kv_layer[pg, :, :, at].float(), torch.tensor([0.003, 0.002]).view(1, 2, 1, 1))[2]
+        return q
+
+    full, _ = _run(model, cfg, prompts, feed, "model", page, chunk)
+    monkeypatch.setattr(ops, "rope_kv_write", rounded)
+    want, kv16 = _run(model, cfg, prompts, feed, "model", page, chunk)
+    assert kv16.bytes_per_token * 9 == kv4.bytes_per_token * 64       # fp32 pool here
+    # 32-bit sums of another order; a code on a border may fall to the other side of it in a later layer
+    assert (got - want).norm() < 1e-3 * want.norm()
+    cos = torch.nn.functional.cosine_similarity(full.flatten(1), got.flatten(1), dim=1)
+    assert float(cos.min()) > 0.97
+
+
+def test_cache_manager_chooses_and_refuses_four_bits():
+    cfg = tiny_llama_config(num_hidden_layers=2, vocab_size=256, dtype="bfloat16", head_dim=64, num_attention_heads=4, num_key_value_heads=2, hidden_size=128)
+    make = lambda c=cfg, **kw: KVCacheManager(c, num_pages=4, max_seats=1, max_pages_per_seq=2, **{"page_size": 64, **kw})
+    assert make(kv_dtype="nvfp4").kv_fp4 and not make().kv_fp4 and not make(kv_dtype="model").kv_fp4
+    cfg.quant = QuantConfig(kv_cache_quant="nvfp4")
+    assert make().kv_fp4 and make().pool.shape == (2, 4, 2, 2, 64, 36) and not make(kv_dtype="model").kv_fp4
+    odd = tiny_llama_config(num_hidden_layers=2, vocab_size=256, dtype="bfloat16", head_dim=32, num_attention_heads=4, num_key_value_heads=2, hidden_size=128)
+    for c, kw in ((odd, {}), (cfg, dict(page_size=48)), (cfg, dict(page_size=8))):
+        with pytest.raises(ValueError):
+            make(c, kv_dtype="nvfp4", **kw)
+    odd.quant = QuantConfig(kv_cache_quant="nvfp4")
+    assert not make(odd).kv_fp4 and make(odd).pool.dtype == torch.bfloat16        # a checkpoint's own setting gives way
+    with pytest.raises(TypeError):
+        ops.cuda_ops().paged_attention(torch.zeros(1, 4, 64), make().pool[0], None, 0.1)
+
+
+def test_native_configuration_counts_four_bit_rows(tmp_path):
+    import json
+    from tensorrt_edge_llm_b200.checkpoint.artifacts import runtime_config_dict
+    from tensorrt_edge_llm_b200.config import parse_quant_config, qwen3_8b_config
+    from tensorrt_edge_llm_b200.quantization.quantize import build_quant_config
+    from tensorrt_edge_llm_b200.runtime import native as rt
+    body = build_quant_config("nvfp4", kv_cache_quantization="nvfp4")
+    (tmp_path / "hf_quant_config.json").write_text(json.dumps(body))
+    assert body["quantization"]["kv_cache_quant_algo"] == "NVFP4" and parse_quant_config(str(tmp_path), {}).kv_cache_quant == "nvfp4"
+    dense = qwen3_8b_config(dtype="float16", quant=QuantConfig(quant_type="nvfp4", group_size=16, kv_cache_quant="nvfp4"))
+    c = rt.LLMEngineConfig.from_runtime_config(json.dumps(runtime_config_dict(dense, 64, 1024, 1216, 1), default=str))
+    small = qwen3_8b_config(dtype="float16", num_hidden_layers=2, quant=dense.quant)
+    assert KVCacheManager(small, num_pages=2, page_size=64, max_seats=1, max_pages_per_seq=2).bytes_per_token * 18 == c.kv_bytes_per_token() == 36 * 2 * 8 * 72
 
 
 @pytest.mark.parametrize("kind", ["fp4", "fp8", "bf16"])
