@@ -105,9 +105,12 @@ class Attention(nn.Module):
         pages of the step's sequences, which hold the cached rows expanded and the step's own as they were rounded."""
         heads = (self.num_q_heads, self.num_kv_heads, self.head_dim, self.kv_scales, None if self.q_norm is None else self.q_norm.weight,
                  None if self.k_norm is None else self.k_norm.weight, self.eps)
-        if ops.fp4_direct(meta, self.num_q_heads // self.num_kv_heads):
+        group = self.num_q_heads // self.num_kv_heads
+        weights = meta.kv_weights[self.layer_idx] if meta.kv_weights is not None and ops.fp4_weighed(meta, group) else None
+        if weights is not None or ops.fp4_direct(meta, group):
             q = ops.rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, *heads)
-            return ops.paged_attention_fp4(q, kv_layer, meta, self.scale, self.kv_scales, sliding_window=self.sliding_window, sinks=self.attention_sink_bias)
+            return ops.paged_attention_fp4(q, kv_layer, meta, self.scale, self.kv_scales, sliding_window=self.sliding_window, sinks=self.attention_sink_bias,
+                                           weights=weights)
         stage, staged = ops.kv_fp4_stage(kv_layer, meta, self.kv_scales, qkv.dtype, self.sliding_window or 0)
         q = ops.rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, *heads, stage=stage, stage_table=staged.page_table)
         return ops.paged_attention(q, stage, staged, self.scale, self.sliding_window, self.attention_sink_bias)

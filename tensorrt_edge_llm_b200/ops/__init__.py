@@ -228,6 +228,7 @@ def stream_norm(stream, weight, eps, *, delta=None, routed=None, mult=1.0, step=
 
 
 FP4_DIRECT_COLUMNS = 64      # rows x heads of a KV head up to which a step reads four-bit pages in place
+FP4_WEIGHT_COLUMNS = 256     # and up to which it can keep account of the attention weights
 
 
 @dataclass
@@ -399,6 +400,11 @@ def rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, num_q_heads, num_kv_heads, h
 def fp4_direct(meta, group):
     """Whether :func:`paged_attention_fp4` reads the pages of this step (``group`` query heads a KV head) in place."""
     return meta.tree_mask is None and meta.max_q_len * group <= FP4_DIRECT_COLUMNS
+
+
+def fp4_weighed(meta, group):
+    """Whether :func:`paged_attention_fp4` can keep account of the attention weights of this step."""
+    return meta.tree_mask is None and meta.max_q_len * group <= FP4_WEIGHT_COLUMNS
 
 
 def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):

@@ -16,7 +16,7 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-from . import fp4_direct, reference as ref_ops
+from . import FP4_WEIGHT_COLUMNS, fp4_direct, fp4_weighed, reference as ref_ops
 from .meta import StepMeta
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "_lib", "libtelb_kernels.so")
@@ -743,9 +743,6 @@ def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int
     return stage, dataclasses.replace(meta, page_table=table, page_size=64)
 
 
-FP4_WEIGHT_COLUMNS = 256     # rows x heads of a KV head up to which a step keeps account of the attention weights
-
-
 def _fp4_commit_path(pool, page_table, past_len, path, path_len) -> None:
     """:func:`kv_commit_path` of four-bit pages, whose rows lie in two parts of a page."""
     layers, pages, _, hkv, psz, row = pool.shape
@@ -789,7 +786,7 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     if weights is not None:
         if weights.dtype != torch.float32 or not weights.is_contiguous() or weights.shape != (pages, hkv, meta.page_size):
             raise ValueError(f"paged_attention_fp4: weights are contiguous fp32 {(pages, hkv, meta.page_size)}")
-        if meta.tree_mask is not None or columns > FP4_WEIGHT_COLUMNS:
+        if not fp4_weighed(meta, hq // hkv):
             raise ValueError(f"paged_attention_fp4: weights are kept for causal steps of at most {FP4_WEIGHT_COLUMNS} rows x heads of a KV head, not {columns}")
         if direct is False:
             raise ValueError("paged_attention_fp4: weights come from the kernel that reads the pages in place")

@@ -50,6 +50,8 @@ class StepMeta:
     # Skip-softmax: fp32 [N] log2(lambda) per sequence (lambda = S / sequence length from the deployed scale table; -inf where
     # the sequence is shorter than the first calibrated length), or None when the deployment runs dense.
     skip_thr: Optional[torch.Tensor] = None
+    # Accumulated attention weights of four-bit pages, fp32 [layers, pages, Hkv, P]: steps of few rows add theirs (None: nobody keeps account).
+    kv_weights: Optional[torch.Tensor] = None
     # What the host knows of the step: (q_len, past_len) per sequence (None: only the device tensors are valid, as in a captured
     # decode step), and plans that ops derive from it once per step and share between layers.
     host_lens: Optional[tuple] = None

@@ -59,11 +59,13 @@ class KVCacheManager:
 
     def __init__(self, cfg: ModelConfig, num_pages: int, page_size: int = 64, max_seats: int = 64,
                  max_pages_per_seq: int = 64, device="cpu", dtype: Optional[torch.dtype] = None,
-                 num_layers: Optional[int] = None, bounded_swa: Optional[bool] = None, kv_dtype: Optional[str] = None):
+                 num_layers: Optional[int] = None, bounded_swa: Optional[bool] = None, kv_dtype: Optional[str] = None, keep_weights: bool = False):
         """``kv_dtype``: ``"fp8"`` stores keys and values as E4M3 bytes (half the bytes per cached token; the attention layers
         work on a 16-bit staging copy of the pages a step touches, see ``csrc/kernels/kv_fp8.cu``); ``"nvfp4"`` stores E2M1 codes
         with an E4M3 scale per 16 features (9/32 of the 16-bit bytes, layout: :func:`ops.rope_kv_write_fp4`); ``None`` / ``"auto"`` follows
-        the checkpoint's ``kv_cache_quant`` setting; ``"fp16"`` / ``"bf16"`` / ``"model"`` keep the compute type."""
+        the checkpoint's ``kv_cache_quant`` setting; ``"fp16"`` / ``"bf16"`` / ``"model"`` keep the compute type.
+        ``keep_weights``: attention weights of cached rows are added up (``weights`` [layers, pages, Hkv, P], four-bit pages) and :meth:`shorten`
+        can drop the rows that got the least."""
         self.cfg = cfg
         # Bounded sliding-window storage (``cpp/runtime/state/boundedSwaKVPageManager.cpp`` in the reference): every
         # attention layer of the model looks back at most `sliding_window` tokens, so pages that lie wholly before the
@@ -127,6 +129,13 @@ class KVCacheManager:
         if cfg.is_hybrid:
             from ..models.nemotron_h import RecurrentState
             self.recurrent = RecurrentState(cfg, max_seats, device, cfg.compute_dtype if self.kv_fp8 or self.kv_fp4 else self.dtype)
+        self.weights: Optional[torch.Tensor] = None
+        self._spare = max_seats                  # the seat that holds a shortened sequence's new pages until it changes over
+        if keep_weights:
+            if not self.kv_fp4 or self.recurrent is not None or self.window or cfg.layer_windows:
+                raise ValueError("attention weights are kept for four-bit pages of stacks whose layers all attend without a window")
+            self.weights = torch.zeros(self.num_layers, num_pages, hkv, page_size, dtype=torch.float32, device=device)
+            max_seats = max_seats + 1
         self.alloc = PageAllocator(num_pages)
         self.table = torch.full((max_seats, max_pages_per_seq), -1, dtype=torch.int32)   # host truth
         self.lengths = [0] * max_seats
@@ -187,6 +196,8 @@ class KVCacheManager:
             else:
                 new = self.alloc.alloc(need - len(have))
             self.table[seat, len(have):need] = torch.tensor(new, dtype=torch.int32)
+            if self.weights is not None:
+                self.weights[:, list(new)] = 0.0            # what the pages' last sequence left
             have.extend(new)
             self.table_version += 1
 
@@ -235,6 +246,30 @@ class KVCacheManager:
             have[i] = -1
         self.table[seat, :upto] = -1
         self.table_version += 1
+
+    @torch.no_grad()
+    def shorten(self, seat: int, keep: int, first: int, recent: int) -> int:
+        """Keep ``keep`` rows of ``seat`` in every layer and KV head (:func:`ops.kv_evict`), in new pages; returns how many tokens went.  The pages
+        that they were in go back to the pool (or to the other sequences that share them)."""
+        from .. import ops
+        length = self.lengths[seat]
+        if self.weights is None:
+            raise ValueError("rows are dropped by attention weight: keep_weights")
+        if length <= keep:
+            return 0
+        spare, dev = self._spare, self.pool.device
+        self.reserve(spare, keep)
+        try:
+            old, to = self.table_rows([seat]).to(dev), self.table_rows([spare])[:, :(keep + self.page_size - 1) // self.page_size].contiguous().to(dev)
+            n = torch.tensor([length], dtype=torch.int32).to(dev)
+            for layer in range(self.num_layers):
+                ops.kv_evict(self.pool[layer], self.weights[layer], old, n, to, keep, first, recent)
+            pages = self.pages_of(spare)
+            self.free(seat)
+            self.adopt_prefix(seat, pages, keep)
+        finally:
+            self.free(spare)
+        return length - keep
 
     def live_pages(self, seat: int) -> int:
         return sum(pg >= 0 for pg in self._pages.get(seat, []))

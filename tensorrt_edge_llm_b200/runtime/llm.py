@@ -54,9 +54,10 @@ class LLM:
                  enable_prefix_cache: bool = False, scheduling: Optional[dict] = None, draft_model=None, speculative=None,
                  context_cache_max_records: int = 4096, context_cache_max_snapshots: int = 64,
                  embedding_quantization: Optional[str] = None, tp_mirror=None, mapping: Optional[Mapping] = None,
-                 kv_cache_dtype: Optional[str] = None, dtype: Optional[str] = None):
+                 kv_cache_dtype: Optional[str] = None, dtype: Optional[str] = None, kv_budget: int = 0):
         """``dtype``: compute type to load the checkpoint in instead of the one it names ("bfloat16" | "float16" | "float32"; 32-bit
-        models run on the CPU, and on the GPU where every layer of the family has fp32 kernels)."""
+        models run on the CPU, and on the GPU where every layer of the family has fp32 kernels).  ``kv_budget`` > 0 (static batches over
+        four-bit pages): a sequence that outgrows so many cached rows is cut back to the first, the latest and the most attended ones."""
         if device is None:
             device = "cuda" if torch.cuda.is_available() else "cpu"
         self.device = torch.device(device)
@@ -81,10 +82,19 @@ class LLM:
         canvas_headroom = self.cfg.diffusion.canvas_length if self.cfg.diffusion is not None else 0
         pages_per_seq = (max_kv_cache_capacity + canvas_headroom + page_size - 1) // page_size
         total_pages = kv_pages or (pages_per_seq * max_batch_size + 1)
+        if kv_budget:
+            if enable_in_flight_batching or draft_model is not None or self.cfg.diffusion is not None or self.cfg.tp_size > 1:
+                raise ValueError("kv_budget is built for static batches on one GPU without a draft model")
+            if kv_budget < 4 * ModelRunner.BUDGET_FIRST:
+                raise ValueError(f"kv_budget of at least {4 * ModelRunner.BUDGET_FIRST} rows")
+            if kv_budget + ModelRunner.BUDGET_SLACK >= max_kv_cache_capacity:
+                raise ValueError(f"kv_budget {kv_budget} and {ModelRunner.BUDGET_SLACK + 1} more rows must be within max_kv_cache_capacity {max_kv_cache_capacity}")
+            total_pages = kv_pages or total_pages + kv_budget // page_size + 1          # a sequence holds its new pages beside the old while it is cut back
         # "fp8": E4M3 KV pages (`--kv-cache-quantization fp8` checkpoints select it through their quantisation config)
         self.kv = KVCacheManager(self.cfg, total_pages, page_size, max_seats=max_batch_size,
-                                 max_pages_per_seq=pages_per_seq, device=self.device, kv_dtype=kv_cache_dtype)
+                                 max_pages_per_seq=pages_per_seq, device=self.device, kv_dtype=kv_cache_dtype, keep_weights=kv_budget > 0)
         self.runner = ModelRunner(self.model, self.kv, self.device, max_num_tokens=max_num_tokens)
+        self.runner.kv_budget = int(kv_budget)
         self.runner.vocab_map = self._vocab_map
         self.lora = None
         self.runner.lora = None
@@ -464,7 +474,7 @@ class LLM:
         for s in seats:
             self.kv.free(s)
         for s, p in zip(seats, ids):
-            self.kv.reserve(s, len(p) + sp.max_tokens)
+            self.kv.reserve(s, len(p) + (0 if self.runner.kv_budget else sp.max_tokens))
         states = [lp.make_row_state(self.guided_vocab, guided=sp.guided, logit_bias=sp.logit_bias, num_logprobs=sp.logprobs,
                                     vocab_size=self.cfg.vocab_size) for _ in range(n)]
         eos = self.cfg.eos_token_id
@@ -541,7 +551,7 @@ class LLM:
         for s, p in zip(seats, ids):
             if len(p) > self.max_input_len:
                 raise ValueError(f"prompt of {len(p)} tokens exceeds max_input_len {self.max_input_len}")
-            self.kv.reserve(s, len(p) + sp.max_tokens)
+            self.kv.reserve(s, len(p) + (0 if self.runner.kv_budget else sp.max_tokens))
         t0 = time.perf_counter()
         if isinstance(ids, torch.Tensor):
             logits = self.runner.prefill_tensor(seats, ids)      # pinned host tensor → one H2D copy per chunk

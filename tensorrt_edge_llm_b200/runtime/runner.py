@@ -67,6 +67,10 @@ class ModelRunner:
         # reduced-vocabulary LM head: logits cover `vocab_map.numel()` columns, column c is token vocab_map[c]
         self.vocab_map: Optional[torch.Tensor] = None
         self.rope_delta: dict = {}          # seat → multimodal RoPE position offset of its decode rows
+        # Rows a sequence may keep (0: all).  One that has grown more than BUDGET_SLACK beyond it is cut back to the first, the latest and the rows
+        # with the largest attention weights; what it has dropped moves the positions of its later rows.
+        self.kv_budget = 0
+        self.dropped: Dict[int, int] = {}
 
     # ---- eager ragged step -----------------------------------------------------------------
     def _meta(self, seats: Sequence[int], q_lens: Sequence[int], logits_all=False, tree_mask=None,
@@ -75,6 +79,9 @@ class ModelRunner:
         for s, q, p in zip(seats, q_lens, past):
             if p == 0:
                 self.rope_delta.pop(s, None)          # a fresh sequence on this seat
+                self.dropped.pop(s, None)
+            if self.dropped.get(s) and p + q + self._offset(s) > self.model.cfg.max_position_embeddings:
+                raise ValueError(f"position {p + q + self._offset(s) - 1} exceeds the model's {self.model.cfg.max_position_embeddings}")
             self.kv.reserve(s, p + q)
         meta = build_step_meta(q_lens, past, self.kv.table_rows(seats), self.kv.page_size, slot_ids=seats,
                                logits_all=logits_all, device=self.device, tree_mask=tree_mask, positions=positions, logits_rows=logits_rows)
@@ -85,23 +92,44 @@ class ModelRunner:
             meta.skip_thr = thresholds_log2(table, [p + q for p, q in zip(past, q_lens)], device=self.device)
         return meta
 
+    BUDGET_SLACK, BUDGET_FIRST, BUDGET_VOTERS = 64, 4, 32
+
+    def _offset(self, seat: int) -> int:
+        """How far a sequence's next position lies ahead of its cached rows."""
+        return self.rope_delta.get(seat, 0) + self.dropped.get(seat, 0)
+
+    def _whole_cache(self, what: str) -> None:
+        if self.kv_budget:
+            raise ValueError(f"kv_budget is not built for {what}")
+
+    def trim(self, seats: Sequence[int], slack: int = BUDGET_SLACK) -> None:
+        """Cut sequences that have outgrown the budget back to it."""
+        if not self.kv_budget:
+            return
+        for s in seats:
+            if self.kv.lengths[s] > self.kv_budget + slack:
+                self.dropped[s] = self.dropped.get(s, 0) + self.kv.shorten(s, self.kv_budget, self.BUDGET_FIRST, self.kv_budget // 4)
+
     def rope_delta_empty(self) -> bool:
         """No resident sequence carries a multimodal position offset (captured passes take positions as given)."""
         return not any(self.rope_delta.values())
 
     @torch.no_grad()
     def step(self, seats: Sequence[int], token_lists: Sequence[Sequence[int]], logits_all=False,
-             commit=True, tree_mask=None, positions=None, logits_rows=None) -> torch.Tensor:
+             commit=True, tree_mask=None, positions=None, logits_rows=None, votes=True) -> torch.Tensor:
         """Run one ragged step; returns logits ``[L, V]`` (last row of each sequence unless
-        ``logits_all`` or an explicit list of packed rows, ``logits_rows``).  KV lengths advance by the rows fed when ``commit``."""
+        ``logits_all`` or an explicit list of packed rows, ``logits_rows``).  KV lengths advance by the rows fed when ``commit``.
+        Under a KV budget the rows' attention weights count toward what stays, unless not ``votes``."""
         q_lens = [len(t) for t in token_lists]
         for s in seats:
             if self.kv.lengths[s] == 0:
                 self.rope_delta.pop(s, None)          # a fresh sequence on this seat
-        if positions is None and self.rope_delta and any(self.rope_delta.get(s) for s in seats):
-            # sequences whose prompt held images: text positions run ahead of / behind the cache length by a fixed offset
-            positions = [self.kv.lengths[s] + self.rope_delta.get(s, 0) + j for s, q in zip(seats, q_lens) for j in range(q)]
+                self.dropped.pop(s, None)
+        if positions is None and any(self._offset(s) for s in seats):
+            # sequences whose prompt held images, or that have dropped rows: positions run ahead of / behind the cache length
+            positions = [self.kv.lengths[s] + self._offset(s) + j for s, q in zip(seats, q_lens) for j in range(q)]
         meta = self._meta(seats, q_lens, logits_all, tree_mask, positions, logits_rows)
+        meta.kv_weights = self.kv.weights if votes else None
         flat = [t for ts in token_lists for t in ts]
         if self.device.type == "cuda":
             host = torch.tensor(flat, dtype=torch.int32).pin_memory()
@@ -112,6 +140,8 @@ class ModelRunner:
         if commit:
             for s, q in zip(seats, q_lens):
                 self.kv.commit(s, q)
+            if self.kv_budget and votes and max(q_lens, default=0) == 1:
+                self.trim(seats)
         return logits
 
     @torch.no_grad()
@@ -122,7 +152,17 @@ class ModelRunner:
         the budget is split on page boundaries (``cpp/scheduler/stepPlanner.cpp`` rule)."""
         n = len(seats)
         with prof.time_stage(prof.PREFILL, batch=n, tokens=sum(len(x) for x in prompts)):
-            return self._prefill(seats, prompts)
+            if not self.kv_budget:
+                return self._prefill(seats, prompts)
+            # the prompts' last rows are a step of their own, whose attention weights say what of the prompts stays
+            group = self.model.cfg.num_attention_heads // self.model.cfg.num_key_value_heads
+            last = max(1, min(self.BUDGET_VOTERS, ops.FP4_WEIGHT_COLUMNS // group))
+            front = [(s, p[:-last]) for s, p in zip(seats, prompts) if len(p) > last]
+            if front:
+                self._prefill([s for s, _ in front], [p for _, p in front])
+            logits = self.step(seats, [p[-last:] for p in prompts])
+            self.trim(seats)
+            return logits
 
     def _prefill(self, seats, prompts) -> torch.Tensor:
         n = len(seats)
@@ -146,7 +186,7 @@ class ModelRunner:
                 finishing.append((i, done[i] + take == len(prompts[i])))
                 done[i] += take
                 budget -= take
-            logits = self.step(step_seats, step_tokens)
+            logits = self.step(step_seats, step_tokens, votes=not self.kv_budget)
             for row, (i, fin) in enumerate(finishing):
                 if fin:
                     out[i] = logits[row]
@@ -160,6 +200,7 @@ class ModelRunner:
 
         ``positions3`` (one ``[3, T_i]`` tensor per sequence, see ``ops.reference.mrope_positions``) switches the step to
         multimodal RoPE; ``rope_deltas`` are remembered per seat and added to the position of every later decode row."""
+        self._whole_cache("embedding rows")
         q_lens = [int(e.shape[0]) for e in embeds]
         meta = self._meta(seats, q_lens)
         if deepstack:
@@ -182,6 +223,7 @@ class ModelRunner:
         and decode rows (already embedded by the caller).  ``positions3[i]`` is the ``[3, T_i]`` position block of sequence
         ``i`` or ``None`` for text-like rows, which take ``cache length + decode offset + j`` on all three components.
         ``deepstack`` indexes rows of the packed step.  Commits every row; returns last-row logits ``[N, V]``."""
+        self._whole_cache("embedding rows")
         q_lens = [int(e.shape[0]) for e in embeds]
         for s in seats:
             if self.kv.lengths[s] == 0:
@@ -212,6 +254,8 @@ class ModelRunner:
     def prefill_tensor(self, seats: Sequence[int], ids: torch.Tensor) -> torch.Tensor:
         """Prefill equal-length prompts given as one tensor ``[N, S]`` (pinned host or device
         memory); chunks hold whole sequences.  Returns last-token logits ``[N, V]``."""
+        if self.kv_budget:
+            return self.prefill(seats, ids.tolist())
         n, s_len = ids.shape
         per = max(1, self.max_num_tokens // s_len)
         outs = []
@@ -286,6 +330,7 @@ class ModelRunner:
     def step_candidates(self, seats: Sequence[int], token_lists: Sequence[Sequence[int]], k: int):
         """One ragged decode step that ends in per-shard candidates instead of logits (tensor-parallel sampling without the
         full-vocabulary gather): ``(values [B, world · k], token ids [B, world · k])``."""
+        self._whole_cache("a vocabulary-sharded head")
         q_lens = [len(t) for t in token_lists]
         positions = None
         if self.rope_delta and any(self.rope_delta.get(s) for s in seats):
@@ -318,7 +363,7 @@ class ModelRunner:
     # ---- decode ----------------------------------------------------------------------------
     def can_graph_step(self, seats: Sequence[int]) -> bool:
         """Whether one all-resident greedy decode step of these seats may run from the captured graph."""
-        return (self.use_cuda_graphs and not self.kv.bounded_swa and len(seats) > 0
+        return (self.use_cuda_graphs and not self.kv_budget and not self.kv.bounded_swa and len(seats) > 0
                 and not any(self.rope_delta.get(s) for s in seats))
 
     @torch.no_grad()
@@ -365,8 +410,21 @@ class ModelRunner:
             return self._decode_greedy(seats, first_tokens, steps)
 
     def _decode_greedy(self, seats, first_tokens, steps) -> torch.Tensor:
+        if not self.kv_budget:
+            return self._decode_greedy_run(seats, first_tokens, steps)
+        toks, out = first_tokens, []
+        while steps > 0:            # until the longest sequence has to be cut back
+            self.trim(seats)
+            run = min(steps, self.kv_budget + self.BUDGET_SLACK + 1 - max(self.kv.lengths[s] for s in seats))
+            out.append(self._decode_greedy_run(seats, toks, run))
+            toks, steps = out[-1][:, -1], steps - run
+        return torch.cat(out, dim=1)
+
+    def _decode_greedy_run(self, seats, first_tokens, steps) -> torch.Tensor:
         n = len(seats)
         for s in seats:
+            if self.dropped.get(s) and self.kv.lengths[s] + steps + self._offset(s) > self.model.cfg.max_position_embeddings:
+                raise ValueError(f"position {self.kv.lengths[s] + steps + self._offset(s) - 1} exceeds the model's {self.model.cfg.max_position_embeddings}")
             self.kv.reserve(s, self.kv.lengths[s] + steps)
         if self.use_cuda_graphs and not any(self.rope_delta.get(s) for s in seats):
             g = self._graphs.get(n)
@@ -421,7 +479,7 @@ class _DecodeGraph:
             positions=torch.zeros(n, **i32), seq_ids=torch.arange(n, **i32),
             page_table=torch.full((n, kv.max_pages_per_seq), -1, **i32), slot_ids=torch.zeros(n, **i32),
             logits_idx=torch.arange(n, **i32), page_size=kv.page_size, num_seqs=n, num_tokens=n,
-            max_q_len=1, max_seq_len=kv.max_pages_per_seq * kv.page_size)
+            max_q_len=1, max_seq_len=kv.max_pages_per_seq * kv.page_size, kv_weights=kv.weights)
         self.out = torch.zeros(self.MAX_STEPS, n, **i32)
         self.step_idx = torch.zeros(1, dtype=torch.int64, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
@@ -456,6 +514,8 @@ class _DecodeGraph:
         devbuf = host.to(self.r.device, non_blocking=True)
         self.meta.past_len.copy_(devbuf[:n])
         self.meta.positions.copy_(devbuf[:n])
+        if any(self.r.dropped.get(s) for s in seats):
+            self.meta.positions.add_(torch.tensor([self.r.dropped.get(s, 0) for s in seats], dtype=torch.int32).to(self.r.device))
         self.meta.slot_ids.copy_(devbuf[n:2 * n])
         self.ids.copy_(devbuf[2 * n:3 * n])
         self.meta.page_table.copy_(devbuf[3 * n:].view(n, mp))
@@ -502,6 +562,7 @@ class _DecodeGraph:
             # warm up once eagerly (allocator, lazy kernels), restore state, then capture
             recurrent = self.r.kv.recurrent
             saved = recurrent.snapshot(seats) if recurrent is not None else None      # the warm-up step advances the state rows
+            votes = None if self.r.kv.weights is None else self.r.kv.weights.clone()
             s = torch.cuda.Stream(device=self.r.device)
             s.wait_stream(torch.cuda.current_stream(self.r.device))
             with torch.cuda.stream(s):
@@ -509,6 +570,8 @@ class _DecodeGraph:
             torch.cuda.current_stream(self.r.device).wait_stream(s)
             if saved is not None:
                 recurrent.restore(seats, saved)
+            if votes is not None:
+                self.r.kv.weights.copy_(votes)
             self._load_state(seats, first_tokens)
             from ..ops import cuda as _cu
             before = _cu.LAUNCHES
