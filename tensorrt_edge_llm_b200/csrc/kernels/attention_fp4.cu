@@ -362,7 +362,8 @@ struct Fp4Occupancy {
 };
 
 // One item's tiles [tile0, tile1), every fourth of them this warp's: outputs of the warp over its keys, the references of their probabilities and their sums.
-template <typename T, int D, int NT>
+// kVotes: the scores are kept for the accumulated weights.
+template <typename T, int D, int NT, bool kVotes>
 __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kvh, int chunk, int q0, int past, int columns, int tile0, int tile1, uint32_t ring_at,
                                          const uint8_t* ring_ptr, float base, float (&o)[NT][D / 16][4], float (&ref)[NT][2], float (&sum)[NT][2]) {
     constexpr int C = 8 * NT;
@@ -407,7 +408,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
     const int all_chunks = (p.max_q_len * group + 7) / 8;
     const int first_tile = fp4_first_tile(past, p.window);
     float4* keep = nullptr;                                                      // of the sequence's first tile
-    if (p.scores && t < p.pairs) keep = p.scores + (((size_t)seq * p.hkv + kvh) * all_chunks + chunk * NT) * p.tiles * 16 * p.pairs + g * p.pairs + t;
+    if (kVotes && t < p.pairs) keep = p.scores + (((size_t)seq * p.hkv + kvh) * all_chunks + chunk * NT) * p.tiles * 16 * p.pairs + g * p.pairs + t;
     // Scores of a tile to probabilities, and those times its values.
     auto take = [&](auto open, const uint8_t* st, int kb, uint32_t missing, const float (&s)[2][NT][4]) {
         float x[2][NT][4];
@@ -432,7 +433,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
         };
         shifted();
         const int nth = kb / kFp4Tile - first_tile;
-        if (keep != nullptr && nth < p.tiles) {                                  // for the accumulated weights
+        if (kVotes && keep != nullptr && nth < p.tiles) {
 #pragma unroll
             for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -568,16 +569,23 @@ __device__ __forceinline__ void fp4_join(float* smem_f, int live, float (&o)[NT]
     }
 }
 
-// Four outputs of a column whose keys have all been joined: the sink, the sum and the values' scale, then the one rounding.
-template <typename T, int D>
-__device__ __forceinline__ void fp4_finish(const Fp4AttnParams& p, size_t row, int h, int d, float4 acc, float top, float l) {
+// A column's sink joins its sum: the factor of what came before; `l` becomes 1 / sum.
+__device__ __forceinline__ float fp4_sink(const Fp4AttnParams& p, int h, float& top, float& l) {
+    float f = 1.f;
     if (p.sinks) {
-        const float z = p.sinks[h] * 1.4426950408889634f, m = fmaxf(top, z), f = exp2_approx(top - m);
-        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+        const float z = p.sinks[h] * 1.4426950408889634f, m = fmaxf(top, z);
+        f = exp2_approx(top - m);
         l = l * f + exp2_approx(z - m);
         top = m;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l, f = inv * p.scales[1];           // a row that sees nothing gives zeros
+    l = l == 0.f ? 0.f : 1.f / l;                                                // a row that sees nothing gives zeros
+    return f;
+}
+
+// Four outputs of a column whose keys have all been joined: the sink, the sum and the values' scale, then the one rounding.
+template <typename T, int D>
+__device__ __forceinline__ void fp4_finish(const Fp4AttnParams& p, size_t row, int h, int d, float4 acc, float top, float l) {
+    const float keep = fp4_sink(p, h, top, l), inv = l, f = inv * keep * p.scales[1];
     *reinterpret_cast<uint2*>(reinterpret_cast<T*>(p.out) + row * D + d) = make_uint2(Cvt<T>::pack2(acc.x * f, acc.y * f), Cvt<T>::pack2(acc.z * f, acc.w * f));
     if (p.stat && d == 0) *reinterpret_cast<float2*>(p.stat + row * 2) = make_float2(top, inv);
 }
@@ -593,9 +601,73 @@ __device__ __forceinline__ void fp4_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// Accumulated attention weights: weights[page, head, slot] = decay * weights + the sum over the step's rows and the group's heads of
+// exp2(score - top) / sum, for keys that some row sees; the step's own keys start from zero.  fp4_keys has left its scores (4 bytes for each
+// key and column, mostly still in the L2 cache); making them again took the keys, their expansion and the products a second time (16 sequences of 8192:
+// 36 us against 8).  A warp owns 32 keys, so that every sum has one order.  Where a CTA's columns are all that the step has, it adds them itself
+// once the sums are known, and every lane reads what it wrote (16 sequences of 8192: 55 us for the step, with a kernel for the weights 59).
+// U tiles at a time: first, first + stride ... of those below `tiles`; `stat(column)` gives (top, 1 / sum).
+template <int U, typename Stat>
+__device__ __forceinline__ void fp4_weigh(const Fp4AttnParams& p, int seq, int kvh, int ql, int past, int index, int stride, int tiles, Stat stat) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, columns = ql * (p.hq / p.hkv);
+    if (index >= tiles) return;
+    const int first_tile = fp4_first_tile(past, p.window), first = p.window > 0 ? max(0, past + 1 - p.window) : 0;
+    float* w[U];
+    float old[U], given[U][2][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        // a lane's own key: half t / 2, row g or g + 8 of it
+        const int at = index + u * stride, mine = (first_tile + at) * kFp4Tile + 16 * (t >> 1) + key_place(g) + 8 * (t & 1), lp = mine >> p.page_shift;
+        const int page = at < tiles && mine >= first && mine < past + ql && lp < p.max_pages ? p.page_table[(size_t)seq * p.max_pages + lp] : -1;
+        w[u] = (unsigned)page < (unsigned)p.num_pages ? p.weights + ((size_t)page * p.hkv + kvh) * p.page_size + (mine & (p.page_size - 1)) : nullptr;
+        old[u] = w[u] && mine < past ? p.decay * *w[u] : 0.f;
+        given[u][0][0] = given[u][0][1] = given[u][1][0] = given[u][1][1] = 0.f;
+    }
+    const int all_chunks = (p.max_q_len * (p.hq / p.hkv) + 7) / 8, chunks = min((columns + 7) / 8, all_chunks);
+    const float4* src = p.scores + (((size_t)seq * p.hkv + kvh) * all_chunks * p.tiles + index) * 16 * p.pairs + g * p.pairs + t;
+    if (t < p.pairs) {
+#pragma unroll 4 / U
+        for (int ch = 0; ch < chunks; ++ch) {
+            float4 s[U][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int m = 0; m < 2; ++m)
+                    s[u][m] = index + u * stride < tiles ? src[((size_t)ch * p.tiles + u * stride) * 16 * p.pairs + m * 8 * p.pairs]
+                                                         : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            float2 st[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) st[c] = ch * 8 + 2 * t + c < columns ? stat(ch * 8 + 2 * t + c) : make_float2(0.f, 0.f);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    given[u][m][0] += exp2_approx(s[u][m].x - st[0].x) * st[0].y;
+                    given[u][m][1] += exp2_approx(s[u][m].z - st[0].x) * st[0].y;
+                    if (ch * 8 + 2 * t + 1 < columns) {                          // the last column may have no neighbour
+                        given[u][m][0] += exp2_approx(s[u][m].y - st[1].x) * st[1].y;
+                        given[u][m][1] += exp2_approx(s[u][m].w - st[1].x) * st[1].y;
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                given[u][m][r] += __shfl_xor_sync(0xffffffffu, given[u][m][r], 1);
+                given[u][m][r] += __shfl_xor_sync(0xffffffffu, given[u][m][r], 2);
+            }
+        const float sum = t & 2 ? (t & 1 ? given[u][1][1] : given[u][1][0]) : (t & 1 ? given[u][0][1] : given[u][0][0]);
+        if (w[u]) *w[u] = old[u] + sum;
+    }
+}
+
 // Many items: a cluster per item, its CTAs take equal parts of the item's tiles and join their results through shared memory.
 // grid (CTAs of a cluster, items of a sequence, sequences)
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kVotes>
 __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas)) attention_fp4_cluster_kernel(const Fp4AttnParams p) {
     pdl_prologue();
     constexpr int C = 8 * NT;
@@ -608,20 +680,41 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
     const int first = fp4_first_tile(past, p.window), tiles = fp4_tiles(past, ql, p.window);
     const int tile0 = first + tiles * rank / ranks, tile1 = first + tiles * (rank + 1) / ranks;
     float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
-    fp4_keys<T, D, NT>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, smem_u32(smem) + warp * Ring::kStages * Ring::kBytes,
+    fp4_keys<T, D, NT, kVotes>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, smem_u32(smem) + warp * Ring::kStages * Ring::kBytes,
                        smem + warp * Ring::kStages * Ring::kBytes, p.scale * 1.4426950408889634f * p.scales[0], o, ref, sum);
     float* smem_f = reinterpret_cast<float*>(smem);
     const int live = min(C, columns - chunk * C);
+    // the CTA's own references and sums lie behind all warps' results, (top, 1 / sum) of the item's columns behind those
+    float4* own_ml = reinterpret_cast<float4*>(smem_f + kFp4Warps * C * (D + 2));
+    float2* s_stat = reinterpret_cast<float2*>(own_ml + C);
+    const bool weigh = kVotes && p.max_items == p.hkv;
+    auto weights = [&]() {
+        const int limit = min(tiles, p.tiles);
+        constexpr int U = NT == 1 ? 4 : 2;
+        for (int i = tile0 + warp - first; i < tile1 - first; i += U * kFp4Warps)
+            fp4_weigh<U>(p, seq, kvh, ql, past, i, kFp4Warps, min(limit, tile1 - first), [&](int col) { return s_stat[col]; });
+    };
     auto finish = [&](int col, int d, float4 acc, float top, float l) {
         const int c = chunk * C + col, r = c / group, h = kvh * group + c - r * group;
         fp4_finish<T, D>(p, (size_t)(q0 + r) * p.hq + h, h, d, acc, top, l);
     };
+    auto stat_of = [&](int col, float top, float l) {
+        const int c = chunk * C + col, r = c / group;
+        fp4_sink(p, kvh * group + c - r * group, top, l);
+        s_stat[col] = make_float2(top, l);
+    };
     if (ranks == 1) {
-        fp4_join<D, NT>(smem_f, live, o, ref, sum, finish);
+        fp4_join<D, NT>(smem_f, live, o, ref, sum, [&](int col, int d, float4 acc, float top, float l) {
+            finish(col, d, acc, top, l);
+            if (weigh && d == 0) stat_of(col, top, l);
+        });
+        if (weigh) {
+            __syncthreads();
+            weights();
+        }
         return;
     }
-    // the CTA's own results take the first warp's place (a thread reads what it replaces), references and sums lie behind all of them
-    float4* own_ml = reinterpret_cast<float4*>(smem_f + kFp4Warps * C * (D + 2));
+    // the CTA's own results take the first warp's place (a thread reads what it replaces)
     fp4_join<D, NT>(smem_f, live, o, ref, sum, [&](int col, int d, float4 acc, float top, float l) {
         *reinterpret_cast<float4*>(smem_f + col * D + d) = acc;
         if (d == 0) own_ml[col] = make_float4(top, l, 0.f, 0.f);
@@ -651,11 +744,23 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
         }
         finish(col, d, acc, top, l);
     }
+    if (weigh && threadIdx.x < live) {
+        float top = kRefStart, l = 0.f;
+        float4 ml[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) ml[r] = r < ranks ? cluster_load_f4(own_ml + threadIdx.x, r) : make_float4(kRefStart, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, ml[r].x);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) l += exp2_approx(ml[r].x - top) * ml[r].y;
+        stat_of(threadIdx.x, top, l);
+    }
     fp4_cluster_sync();                                                          // nobody leaves while its results may be read
+    if (weigh) weights();
 }
 
 // Few items and many keys: the line.
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kVotes>
 __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas)) attention_fp4_kernel(const Fp4AttnParams p) {
     pdl_prologue();
     constexpr int C = 8 * NT;
@@ -687,7 +792,7 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
         const int tile0 = fp4_first_tile(past, p.window) + off, tile1 = tile0 + count;
         const int q0 = p.q_start[seq];
         float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
-        fp4_keys<T, D, NT>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, ring_at, ring_ptr, base, o, ref, sum);
+        fp4_keys<T, D, NT, kVotes>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, ring_at, ring_ptr, base, o, ref, sum);
         const bool whole = count == tiles;
         const size_t slot = (size_t)blockIdx.x * 2 + (off == 0);                 // parts: [0] what began in an earlier CTA, [1] what goes on in a later one
         if (threadIdx.x == 0 && off == 0 && item < p.max_items)
@@ -778,71 +883,28 @@ __global__ void __launch_bounds__(512) attention_fp4_merge_kernel(const Fp4AttnP
     fp4_finish<T, D>(p, (size_t)(p.q_start[seq] + r) * p.hq + h, h, d, out, top, l);
 }
 
-// Accumulated attention weights: weights[page, head, slot] = decay * weights + the sum over the step's rows and the group's heads of
-// exp2(score - top) / sum, for keys that some row sees; the step's own keys start from zero.  The attention kernel has left its scores (4 bytes for each
-// key and column, mostly still in the L2 cache); making them again took the keys, their expansion and the products a second time (16 sequences of 8192:
-// 36 us against 8).  A warp owns 32 keys, so that every sum has one order.  grid (groups of 4 tiles, KV heads, sequences)
+// The weights where the attention kernel could not add them itself.  grid (groups of 4 tiles, KV heads, sequences)
 __global__ void __launch_bounds__(128) attention_fp4_weights_kernel(const Fp4AttnParams p) {
     pdl_prologue();
-    const int seq = blockIdx.z, kvh = blockIdx.y, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int group = p.hq / p.hkv, ql = p.q_len[seq], past = p.past_len[seq], columns = ql * group;
-    const int index = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (index >= min(fp4_tiles(past, ql, p.window), p.tiles)) return;
-    const int kb = (fp4_first_tile(past, p.window) + index) * kFp4Tile, first = p.window > 0 ? max(0, past + 1 - p.window) : 0;
-    // a lane's own key: half t / 2, row g or g + 8 of it
-    const int mine = kb + 16 * (t >> 1) + key_place(g) + 8 * (t & 1), lp = mine >> p.page_shift;
-    const int page = mine >= first && mine < past + ql && lp < p.max_pages ? p.page_table[(size_t)seq * p.max_pages + lp] : -1;
-    float* w = (unsigned)page < (unsigned)p.num_pages ? p.weights + ((size_t)page * p.hkv + kvh) * p.page_size + (mine & (p.page_size - 1)) : nullptr;
-    const float old = w && mine < past ? p.decay * *w : 0.f;
-    const int all_chunks = (p.max_q_len * group + 7) / 8, chunks = min((columns + 7) / 8, all_chunks), q0 = p.q_start[seq];
-    const float4* src = p.scores + (((size_t)seq * p.hkv + kvh) * all_chunks * p.tiles + index) * 16 * p.pairs + g * p.pairs + t;
-    float given[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    if (t < p.pairs) {
-#pragma unroll 4
-        for (int ch = 0; ch < chunks; ++ch) {
-            float4 s[2];
-#pragma unroll
-            for (int m = 0; m < 2; ++m) s[m] = src[(size_t)ch * p.tiles * 16 * p.pairs + m * 8 * p.pairs];
-            float2 st[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int col = ch * 8 + 2 * t + c, r = col / group;
-                st[c] = col < columns ? *reinterpret_cast<const float2*>(p.stat + ((size_t)(q0 + r) * p.hq + kvh * group + col - r * group) * 2) : make_float2(0.f, 0.f);
-            }
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {
-                given[m][0] += exp2_approx(s[m].x - st[0].x) * st[0].y;
-                given[m][1] += exp2_approx(s[m].z - st[0].x) * st[0].y;
-                if (ch * 8 + 2 * t + 1 < columns) {                              // the last column may have no neighbour
-                    given[m][0] += exp2_approx(s[m].y - st[1].x) * st[1].y;
-                    given[m][1] += exp2_approx(s[m].w - st[1].x) * st[1].y;
-                }
-            }
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 1);
-            given[m][r] += __shfl_xor_sync(0xffffffffu, given[m][r], 2);
-        }
-    const float sum = t & 2 ? (t & 1 ? given[1][1] : given[1][0]) : (t & 1 ? given[0][1] : given[0][0]);
-    if (w) *w = old + sum;
+    const int seq = blockIdx.z, kvh = blockIdx.y, ql = p.q_len[seq], past = p.past_len[seq], group = p.hq / p.hkv, q0 = p.q_start[seq];
+    fp4_weigh<1>(p, seq, kvh, ql, past, blockIdx.x * 4 + (threadIdx.x >> 5), 1, min(fp4_tiles(past, ql, p.window), p.tiles), [&](int col) {
+        const int r = col / group;
+        return *reinterpret_cast<const float2*>(p.stat + ((size_t)(q0 + r) * p.hq + kvh * group + col - r * group) * 2);
+    });
 }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool kVotes>
 int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t stream) {
     constexpr int C = 8 * NT;
     constexpr int kSmem = kFp4Warps * Fp4Ring<D>::kStages * Fp4Ring<D>::kBytes;
-    static_assert(kSmem >= kFp4Warps * C * (D + 2) * 4 + C * 16, "the warps' results fit where their rings were");
+    static_assert(kSmem >= kFp4Warps * C * (D + 2) * 4 + C * 24, "the warps' results fit where their rings were");
     static bool configured[64] = {};
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !configured[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(attention_fp4_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaError_t e = cudaFuncSetAttribute(attention_fp4_kernel<T, D, NT, kVotes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT, kVotes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT, kVotes>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4)", e);
         if (dev >= 0 && dev < 64) configured[dev] = true;
     }
@@ -860,10 +922,10 @@ int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t st
         attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = pdl_enabled() ? 2 : 1;
-        cudaError_t e = cudaLaunchKernelEx(&cfg, attention_fp4_cluster_kernel<T, D, NT>, p);
+        cudaError_t e = cudaLaunchKernelEx(&cfg, attention_fp4_cluster_kernel<T, D, NT, kVotes>, p);
         return e == cudaSuccess ? 0 : fail("attention_fp4_cluster_kernel", e);
     }
-    TELB_LAUNCH("attention_fp4_kernel", (attention_fp4_kernel<T, D, NT>), dim3(p.ctas), dim3(kFp4Warps * 32), kSmem, stream, p);
+    TELB_LAUNCH("attention_fp4_kernel", (attention_fp4_kernel<T, D, NT, kVotes>), dim3(p.ctas), dim3(kFp4Warps * 32), kSmem, stream, p);
     TELB_LAUNCH("attention_fp4_merge_kernel", (attention_fp4_merge_kernel<T, D, NT>), dim3(p.max_items, p.num_seqs, min(columns, C)), dim3(512), 0, stream, p);
     return 0;
 }
@@ -872,8 +934,10 @@ template <typename T, int D>
 int launch_attention_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
     const int columns = p.max_q_len * (p.hq / p.hkv);
     constexpr int kMost = D == 256 ? 1 : 2;
-    const int rc = columns <= 8 ? launch_attention_fp4_nt<T, D, 1>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost>(p, columns, stream);
-    if (rc || !p.weights) return rc;
+    if (!p.weights)
+        return columns <= 8 ? launch_attention_fp4_nt<T, D, 1, false>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost, false>(p, columns, stream);
+    const int rc = columns <= 8 ? launch_attention_fp4_nt<T, D, 1, true>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost, true>(p, columns, stream);
+    if (rc || (p.ranks > 0 && p.max_items == p.hkv)) return rc;     // a cluster has all columns of its keys: it adds the weights itself
     TELB_LAUNCH("attention_fp4_weights_kernel", attention_fp4_weights_kernel, dim3((p.tiles + 3) / 4, p.hkv, p.num_seqs), dim3(128), 0, stream, p);
     return 0;
 }
