@@ -123,9 +123,19 @@ def bench_attention(args):
         kv, kv_alt = kv.to(torch.float8_e4m3fn), kv_alt.to(torch.float8_e4m3fn)
         q8 = qt.to(torch.float8_e4m3fn)
         kv_scales = torch.ones(2, device="cuda")
+    fp4 = getattr(args, "kv_dtype", "model") == "nvfp4"
+    if fp4:                 # four-bit pages, read in place or expanded by the rule of the op
+        fp4_scales, identity = torch.full((2,), 1e-3, device="cuda"), torch.cat([torch.ones(past + q, d // 2), torch.zeros(past + q, d // 2)], dim=1).cuda()
+        rows = build_step_meta([past + q] * b, [0] * b, table, page, device="cuda")
+        packed = [torch.zeros(b * pages_per, 2, hkv, page, d * 9 // 16, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        for pool in packed:
+            cu.rope_kv_write_fp4(torch.randn(rows.num_tokens, (hq + 2 * hkv) * d, device="cuda").bfloat16(), pool, rows, identity, hq, hkv, d, fp4_scales)
+        kv, kv_alt = packed
 
     def fn():
         flip[0] ^= 1
+        if fp4:
+            return cu.paged_attention_fp4(qt, kv if flip[0] else kv_alt, meta, d ** -0.5, fp4_scales)
         if fp8:
             return cu.paged_attention_decode_fp8(q8, kv if flip[0] else kv_alt, meta, d ** -0.5, None, kv_scales, torch.bfloat16,
                                                  splits=args.splits or None)
@@ -134,13 +144,13 @@ def bench_attention(args):
     out = fn()
     if args.check:      # numerics against the fp32 statement of the op
         from ..ops import reference as ref
-        want = ref.paged_attention(qt, kv, meta, d ** -0.5)
+        want = ref.paged_attention_fp4(qt, kv, meta, d ** -0.5, fp4_scales) if fp4 else ref.paged_attention(qt, kv, meta, d ** -0.5)
         err = ((out.float() - want.float()).norm() / want.float().norm()).item()
         assert err < 8e-3, err
     # a single launch timed with events also counts the host time to encode descriptors and launch: decode-size
     # calls are therefore timed as a captured chain of launches
     med, best = time_fn(fn, args.warmup, args.iters, flush, (args.graph or 8) if q <= 4 else 0)
-    if args.trace:      # per-tile timeline of the first CTA (ns since it started)
+    if args.trace and not fp4:      # per-tile timeline of the first CTA (ns since it started)
         tr = torch.zeros(3, 64, 4, dtype=torch.int64, device="cuda")
         cu.paged_attention(qt, kv, meta, d ** -0.5, splits=args.splits or None, trace=tr)
         torch.cuda.synchronize()
@@ -149,7 +159,7 @@ def bench_attention(args):
         for role, evs in names.items():
             for e, nm in enumerate(evs):
                 print(f"trace {nm:>14}: " + " ".join(f"{int(tr[role, j, e]):6d}" for j in range(tiles)))
-    kv_bytes = b * (past + q) * hkv * d * 2 * (1 if fp8 else 2)
+    kv_bytes = b * (past + q) * hkv * d * 2 * (9 / 16 if fp4 else 1 if fp8 else 2)
     flops = 4.0 * b * hq * d * (q * past + q * (q + 1) / 2)
     roof = max(flops / fl, kv_bytes / bw)
     print(json.dumps({"kernel": "paged_attention", "batch": b, "past": past, "q": q, "median_us": round(med * 1e6, 2),
@@ -304,7 +314,8 @@ def main():
     a.add_argument("--variant", type=int, default=-1, help="ring / residency variant of the decode kernel (up to 4 rows) or of the one-tile kernel, which then takes the step (telb_set_decode_variant, telb_set_attn_variant)")
     a.add_argument("--splits", type=int, default=0, help="KV splits (0 = heuristic)")
     a.add_argument("--check", action="store_true", help="compare with the fp32 reference first")
-    a.add_argument("--kv-dtype", default="model", choices=["model", "fp8"], help="fp8: E4M3 cache pages read in place (decode shapes)")
+    a.add_argument("--kv-dtype", default="model", choices=["model", "fp8", "nvfp4"],
+                   help="fp8: E4M3 cache pages read in place (decode shapes); nvfp4: four-bit pages")
     a.add_argument("--trace", action="store_true", help="print the per-tile timeline of the first CTA of the decode kernel")
     a.add_argument("--trace-tiles", type=int, default=0, help="tiles of the first CTA to print (it walks several items)")
     o = sub.add_parser("ops")

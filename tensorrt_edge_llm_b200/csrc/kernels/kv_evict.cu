@@ -1,7 +1,7 @@
 // Shortening a paged cache by accumulated attention weight.  For every sequence and KV head
 //
 //   kv_evict_select  the rows that stay: the first ones, the latest ones, and of those between them the heaviest (equal weights: the earlier row),
-//                    in ascending order.  A radix selection over the weights' bit patterns, eight bits a pass, then an ordered compaction.
+//                    in ascending order.  A radix selection over the bit patterns of the weights, then an ordered compaction.
 //   kv_evict_move    copies of those rows (keys, values, block scales, weights) into the rows 0, 1, 2 .. of other pages.
 #include "host_utils.h"
 #include "tc5_common.cuh"
@@ -45,7 +45,7 @@ __device__ __forceinline__ void cluster_sync_all() {
 // from the histograms of all of them, 11, 11 and 10 bits at a time (mostly the first two passes do); then every CTA writes its part of the
 // rows that stay, in order.
 __global__ void __launch_bounds__(kEvictThreads) kv_evict_select_kernel(const EvictParams p) {
-    extern __shared__ uint32_t held[];
+    extern __shared__ __align__(16) uint32_t held[];
     __shared__ __align__(16) int hist[2][kEvictBins];           // of two passes in turn: one is read by the cluster while the next is cleared
     __shared__ int coarse[2][256];                              // sums of eight neighbours
     __shared__ int s_warp[8], s_found[3], s_counts[2];

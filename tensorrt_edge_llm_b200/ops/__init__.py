@@ -422,7 +422,8 @@ def paged_attention_fp4(q, kv_layer, meta, scale, scales, sliding_window=None, s
 
     ``weights`` (fp32 ``[pages, Hkv, P]``, causal steps of at most 256 rows x heads of a KV head): every key that some row of the step sees
     gets ``decay * weights + `` the sum of its softmax weights over those rows and the query heads of the KV head; the step's own keys
-    start from zero, other entries stay as they are."""
+    start from zero, other entries stay as they are.  A page that keeps account must belong to one sequence of the step: two that add to it
+    at once may lose one's part."""
     f = cuda_ops().paged_attention_fp4 if q.is_cuda else ref.paged_attention_fp4
     return f(q, kv_layer, meta, scale, scales, sliding_window, sinks, weights, decay)
 

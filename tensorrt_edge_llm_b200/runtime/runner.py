@@ -140,7 +140,7 @@ class ModelRunner:
         if commit:
             for s, q in zip(seats, q_lens):
                 self.kv.commit(s, q)
-            if self.kv_budget and votes and max(q_lens, default=0) == 1:
+            if self.kv_budget and votes:
                 self.trim(seats)
         return logits
 

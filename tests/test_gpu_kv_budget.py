@@ -78,3 +78,19 @@ def test_generate_under_a_budget_ends_clean():
     for s in range(3):
         llm.kv.free(s)
     assert (llm.kv.native.free_pages if llm.kv.native is not None else llm.kv.alloc.free_pages) == free
+
+
+def test_requests_in_flight_over_four_bit_pages():
+    """Eleven requests share the captured steps of 16 rows, whose last row stands there several times."""
+    cfg = tiny_llama_config(num_hidden_layers=2, vocab_size=256, dtype="bfloat16", head_dim=64, num_attention_heads=4, num_key_value_heads=2, hidden_size=256)
+    kw = dict(device="cuda", max_input_len=128, max_kv_cache_capacity=192, page_size=16, kv_cache_dtype="nvfp4", random_init_seed=0)
+    flight = LLM(cfg, max_batch_size=16, enable_in_flight_batching=True, enable_prefix_cache=True, **kw)
+    prompts = _prompts(60, 3, 100, 33, 17, 48, 5, 90, 77, 64, 21)
+    outs = [o.token_ids for o in flight.generate(prompts, SamplingParams(max_tokens=24, ignore_eos=True))]
+    alone = LLM(cfg, max_batch_size=1, **kw)
+    for p, out in zip(prompts, outs):
+        assert len(out) == 24
+        alone.kv.free(0)
+        logits = alone.runner.step([0], [p + out[:-1]], logits_all=True)[len(p) - 1:].float()
+        # steps of one row and whole prompts round by other orders of sums and by 16-bit copies: the token taken is the largest within some steps of bf16
+        assert bool((logits[torch.arange(24), torch.tensor(out)] >= logits.max(-1).values - 2 ** -5 * logits.abs().amax(-1)).all())

@@ -237,3 +237,19 @@ def test_refusals():
         ops.kv_evict(layer, w.double(), table, n, to, 4)
     with pytest.raises(ValueError):
         ops.kv_evict(layer, w, table, torch.tensor([1, 2]), to, 4)
+
+
+def test_requests_in_flight_over_four_bit_pages_are_the_static_ones():
+    from tensorrt_edge_llm_b200.runtime.llm import LLM
+    from tensorrt_edge_llm_b200.runtime.runner import SamplingParams
+    cfg = tiny_llama_config(num_hidden_layers=2, vocab_size=256, dtype="float32", head_dim=64, num_attention_heads=4, num_key_value_heads=2, hidden_size=128)
+    g = torch.Generator().manual_seed(9)
+    head = torch.randint(0, 256, (40,), generator=g).tolist()
+    prompts = [head + torch.randint(0, 256, (n,), generator=g).tolist() for n in (50, 3, 21)]          # a shared prefix of whole pages
+    sp = SamplingParams(max_tokens=12, ignore_eos=True)
+    kw = dict(device="cpu", max_batch_size=3, max_input_len=128, max_kv_cache_capacity=128, page_size=16, kv_cache_dtype="nvfp4", random_init_seed=0)
+    want = [LLM(cfg, **kw).generate([p], sp)[0].token_ids for p in prompts]
+    assert [o.token_ids for o in LLM(cfg, **kw).generate(prompts, sp)] == want
+    flight = LLM(cfg, enable_in_flight_batching=True, enable_prefix_cache=True, **kw)
+    assert [o.token_ids for o in flight.generate(prompts, sp)] == want
+    assert [o.token_ids for o in flight.generate(prompts, sp)] == want
