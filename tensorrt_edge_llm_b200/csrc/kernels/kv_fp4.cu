@@ -103,7 +103,8 @@ __device__ __forceinline__ void scale_rows(float (&v)[8], float inv, const uint4
 }
 
 // Whole heads turn: D/16 lanes a head, a lane holds features 8 l .. and D/2 + 8 l .., which turn together; a warp takes every `parts`-th group of 512 / D heads
-// of a token, whose cos / sin row, norm weights and page look-up it fetches once.
+// of a token, whose cos / sin row, norm weights and page look-up it fetches once.  A long prompt is bound by the arithmetic of the exact codes beside the
+// traffic: 8129 rows of 32 / 8 heads of 128, 16-bit copies too, 52 us (0.63 of the copy rate); 64 rows take 5.5 us, the latency of one row.
 template <typename T, int D>
 __global__ void __launch_bounds__(128, 6) rope_kv_write_fp4_kernel(const Fp4WriteParams p, int parts) {
     pdl_prologue();
