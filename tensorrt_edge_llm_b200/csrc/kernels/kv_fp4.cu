@@ -133,12 +133,12 @@ __global__ void __launch_bounds__(128, 6) rope_kv_write_fp4_kernel(const Fp4Writ
     const int s = p.seq_ids[t];
     const int slot = p.past_len[s] + (p.kv_offsets ? p.kv_offsets[t] : t - p.q_start[s]);
     const int lp = slot / p.page_size, at = slot - lp * p.page_size;
-    const int page = lp < p.max_pages ? p.page_table[(size_t)s * p.max_pages + lp] : -1;
+    const int page = slot >= 0 && lp < p.max_pages ? p.page_table[(size_t)s * p.max_pages + lp] : -1;
     int sp = -1, stage_at = 0;
     if (p.stage) {
         const int sl = slot / p.stage_page;
         stage_at = slot - sl * p.stage_page;
-        sp = sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
+        sp = slot >= 0 && sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
     }
     const float scale_k = p.scales[0], scale_v = p.scales[1], inv_k = __frcp_rn(scale_k), inv_v = __frcp_rn(scale_v);
     for (int grp = part; grp < groups; grp += parts) {
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4Wr
     const int s = p.seq_ids[t];
     const int slot = p.past_len[s] + (p.kv_offsets ? p.kv_offsets[t] : t - p.q_start[s]);
     const int lp = slot / p.page_size, at = slot - lp * p.page_size;
-    const int page = lp < p.max_pages ? p.page_table[(size_t)s * p.max_pages + lp] : -1;
+    const int page = slot >= 0 && lp < p.max_pages ? p.page_table[(size_t)s * p.max_pages + lp] : -1;
     const int head = is_v ? h - p.hq - p.hkv : h - p.hq;
     const float scale = p.scales[is_v];
     // the largest magnitude of the block, compared as bit patterns so that a NaN stays one
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4Wr
     }
     if (p.stage) {
         const int sl = slot / p.stage_page;
-        const int sp = sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
+        const int sp = slot >= 0 && sl < p.stage_max ? p.stage_table[(size_t)s * p.stage_max + sl] : -1;
         if ((unsigned)sp >= (unsigned)p.stage_pages) return;
 #pragma unroll
         for (int i = 0; i < E; ++i) x[i] = fp4_round<T>(back[i]);
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(256) kv_fp4_commit_path_kernel(uint8_t* __rest
     const int past = past_len[b];
     const size_t slab = fp4_slab_bytes(page_size, D);
     auto word_at = [&](int slot, int w) -> uint32_t* {
-        const int lp = slot / page_size, page = lp < max_pages ? page_table[(size_t)b * max_pages + lp] : -1, at = slot - lp * page_size;
+        const int lp = slot / page_size, page = slot >= 0 && lp < max_pages ? page_table[(size_t)b * max_pages + lp] : -1, at = slot - lp * page_size;
         if ((unsigned)page >= (unsigned)num_pages) return nullptr;
         uint8_t* s = pool + ((((size_t)(plane >> 1) * num_pages + page) * 2 + (plane & 1)) * hkv + head) * slab;
         return reinterpret_cast<uint32_t*>(w < kCodes ? s + (size_t)at * (D / 2) + w * 4 : s + (size_t)page_size * (D / 2) + (size_t)at * (D / 16) + (w - kCodes) * 4);

@@ -327,3 +327,35 @@ def test_model_with_four_bit_kv_eager_and_graph(family):
     assert cos(four, want) > 0.995 and cos(many, many_h) > 0.995 and cos(tree, many) > 0.995
     assert cos(full[0], four) > 0.95
     assert torch.equal(run(model, dev, "nvfp4", graphs=False)[3], toks)
+
+
+@pytest.mark.parametrize("family", ["gemma", "hybrid"])
+def test_other_stacks_over_four_bit_pages(family):
+    """256-wide heads in sliding and full layers, and attention beside recurrent layers: near the 16-bit cache over prompts and steps."""
+    from tensorrt_edge_llm_b200 import AutoModel
+    from tensorrt_edge_llm_b200.config import GdnConfig, MambaConfig, ModelConfig, hybrid_nemotron_config
+    from tensorrt_edge_llm_b200.runtime.kv_cache import KVCacheManager
+    from tensorrt_edge_llm_b200.runtime.runner import ModelRunner
+    if family == "gemma":
+        cfg = ModelConfig.from_hf_dict(dict(model_type="gemma3_text", vocab_size=512, hidden_size=512, intermediate_size=1024, num_hidden_layers=3, num_attention_heads=4,
+                                            num_key_value_heads=2, head_dim=256, sliding_window=96, query_pre_attn_scalar=256, max_position_embeddings=1024,
+                                            layer_types=["sliding_attention", "full_attention", "sliding_attention"], dtype="bfloat16"))
+    else:
+        cfg = hybrid_nemotron_config(num_hidden_layers=8, vocab_size=512, hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                                     dtype="bfloat16", max_position_embeddings=512, mamba=MambaConfig(num_heads=8, head_dim=64, d_state=128, n_groups=2, conv_kernel=4),
+                                     gdn=GdnConfig(num_k_heads=2, num_v_heads=4, head_k_dim=128, head_v_dim=128, conv_kernel=4))
+    model = AutoModel.from_config(cfg, device=torch.device("cuda", 0), random_init=0)
+    g = torch.Generator().manual_seed(3)
+    prompts, feed = [torch.randint(0, 512, (n,), generator=g).tolist() for n in (200, 37)], torch.randint(0, 512, (4, 2), generator=g).tolist()
+
+    def run(kv_dtype):
+        kv = KVCacheManager(cfg, num_pages=16, page_size=64, max_seats=2, max_pages_per_seq=6, device="cuda", kv_dtype=kv_dtype)
+        r = ModelRunner(model, kv)
+        out = [r.prefill([0, 1], prompts)] + [r.step([0, 1], [[t] for t in row]) for row in feed]
+        return torch.stack(out).float(), kv
+
+    want, _ = run("model")
+    got, kv = run("nvfp4")
+    assert kv.kv_fp4
+    # E2M1 with block scales is off by a tenth of a row's norm at most; a missing or misplaced row would leave no likeness
+    assert float(torch.nn.functional.cosine_similarity(got.flatten(0, 1), want.flatten(0, 1), dim=1).min()) > 0.95
