@@ -11,8 +11,8 @@
 // What bounds it is the issue of instructions: 16 keys of 128 features are some 290 of them for 8 columns, 224 alone for codes to half2 (4 ALU
 // instructions a word of eight codes), block scales and products; the pages' bytes would take a third to a half of the time.  So tiles that every
 // column sees whole have code without masks, and a ring of asynchronous copies per warp keeps three tiles on their way.  Measured with heads of 128:
-// 64 sequences of 1088 keys, 32 / 8 heads, 26.6 us (2.9 TB/s, 0.45 of the copy rate; 16-bit pages 55, E4M3 pages 35); 30 of up to 4000 38.9 us; one of 131000,
-// 32 / 4 heads, 34 us; one of 700 8 us, which is latency: launch, page table, first tile, join.  Taken back: bulk copies with mbarriers in place of the
+// 64 sequences of 1088 keys, 32 / 8 heads, 26.0 us (3.0 TB/s, 0.46 of the copy rate; 16-bit pages 55, E4M3 pages 35); 30 of up to 4000 38.9 us; one of 131000,
+// 32 / 4 heads, 34 us; one of 700 7.5 us, which is latency: launch, page table, first tile, join.  Taken back: bulk copies with mbarriers in place of the
 // lanes' copies; 32 columns a warp (half the occupancy); operands expanded once for all warps of a CTA, in shared memory (half the instructions, but two
 // barriers for every 128 keys: 2 sequences of 4000 keys, 128 columns, 49 us against 50, one of 8000, 64 columns, 28 against 24).
 #include <type_traits>
@@ -293,7 +293,8 @@ struct Fp4Ring {
     uint32_t page_bytes, smem;
     int page_shift, max_pages, num_pages, ids_at, ids, end, lane;
 
-    __device__ __forceinline__ void begin(const Fp4AttnParams& p, int seq, int kvh, int end_, uint32_t smem_, int lane_) {
+    // `first_ids`: the lane's entry of the first 32 of the table.
+    __device__ __forceinline__ void begin(const Fp4AttnParams& p, int seq, int kvh, int end_, uint32_t smem_, int lane_, int first_ids) {
         const size_t slab = fp4_slab_bytes(p.page_size, D);
         lane = lane_;
         keys = p.pool + kvh * slab + lane * 16;
@@ -304,7 +305,8 @@ struct Fp4Ring {
         page_shift = p.page_shift;
         max_pages = p.max_pages;
         num_pages = p.num_pages;
-        ids_at = -64;
+        ids_at = 0;
+        ids = first_ids;
         end = end_;
         smem = smem_;
     }
@@ -363,6 +365,11 @@ struct Fp4Ring {
     }
 };
 
+__device__ __forceinline__ int fp4_first_ids(const Fp4AttnParams& p, int seq) {
+    const int lane = threadIdx.x & 31;
+    return lane < p.max_pages ? p.page_table[(size_t)seq * p.max_pages + lane] : -1;
+}
+
 template <typename T, int D, int NT>
 struct Fp4Occupancy {
     // CTAs an SM: registers for the accumulators (4 NT D/16) and the queries (2 NT D/16) besides some 60; three stages of a ring a warp
@@ -372,8 +379,8 @@ struct Fp4Occupancy {
 // One item's tiles [tile0, tile1), every fourth of them this warp's: outputs of the warp over its keys, the references of their probabilities and their sums.
 // kVotes: the scores are kept for the accumulated weights.
 template <typename T, int D, int NT, bool kVotes>
-__device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kvh, int chunk, int q0, int past, int columns, int tile0, int tile1, uint32_t ring_at,
-                                         const uint8_t* ring_ptr, float base, float (&o)[NT][D / 16][4], float (&ref)[NT][2], float (&sum)[NT][2]) {
+__device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kvh, int chunk, int q0, int past, int columns, int tile0, int tile1, int first_ids,
+                                         uint32_t ring_at, const uint8_t* ring_ptr, float base, float (&o)[NT][D / 16][4], float (&ref)[NT][2], float (&sum)[NT][2]) {
     constexpr int C = 8 * NT;
     using Ring = Fp4Ring<D>;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -382,7 +389,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
     const int end = past + r_last + 1;
     const int all_low = p.window > 0 ? max(0, past + r_last + 1 - p.window) : 0, all_high = past + r_first + 1;      // visible to every column
     Ring ring;
-    ring.begin(p, seq, kvh, end, ring_at, lane);
+    ring.begin(p, seq, kvh, end, ring_at, lane, first_ids);
     uint32_t flags = 0;                                                      // two bits a stage
     int next = tile0 + warp;
 #pragma unroll
@@ -683,12 +690,13 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
     extern __shared__ __align__(16) uint8_t smem[];
     const int warp = threadIdx.x >> 5, ranks = gridDim.x, rank = blockIdx.x, seq = blockIdx.z;
     const int chunk = blockIdx.y / p.hkv, kvh = blockIdx.y - chunk * p.hkv;
+    const int first_ids = fp4_first_ids(p, seq);                                 // on its way with the lengths, not behind them
     const int group = p.hq / p.hkv, ql = p.q_len[seq], past = p.past_len[seq], q0 = p.q_start[seq], columns = ql * group;
     if (chunk * C >= columns) return;                                            // the whole cluster
     const int first = fp4_first_tile(past, p.window), tiles = fp4_tiles(past, ql, p.window);
     const int tile0 = first + tiles * rank / ranks, tile1 = first + tiles * (rank + 1) / ranks;
     float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
-    fp4_keys<T, D, NT, kVotes>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, smem_u32(smem) + warp * Ring::kStages * Ring::kBytes,
+    fp4_keys<T, D, NT, kVotes>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, first_ids, smem_u32(smem) + warp * Ring::kStages * Ring::kBytes,
                        smem + warp * Ring::kStages * Ring::kBytes, p.scale * 1.4426950408889634f * p.scales[0], o, ref, sum);
     float* smem_f = reinterpret_cast<float*>(smem);
     const int live = min(C, columns - chunk * C);
@@ -800,7 +808,7 @@ __global__ void __launch_bounds__(kFp4Warps * 32, (Fp4Occupancy<T, D, NT>::kCtas
         const int tile0 = fp4_first_tile(past, p.window) + off, tile1 = tile0 + count;
         const int q0 = p.q_start[seq];
         float o[NT][D / 16][4], ref[NT][2], sum[NT][2];
-        fp4_keys<T, D, NT, kVotes>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, ring_at, ring_ptr, base, o, ref, sum);
+        fp4_keys<T, D, NT, kVotes>(p, seq, kvh, chunk, q0, past, columns, tile0, tile1, fp4_first_ids(p, seq), ring_at, ring_ptr, base, o, ref, sum);
         const bool whole = count == tiles;
         const size_t slot = (size_t)blockIdx.x * 2 + (off == 0);                 // parts: [0] what began in an earlier CTA, [1] what goes on in a later one
         if (threadIdx.x == 0 && off == 0 && item < p.max_items)

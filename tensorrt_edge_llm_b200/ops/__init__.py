@@ -21,10 +21,16 @@ from .meta import StepMeta, build_step_meta
 __all__ = ["StepMeta", "build_step_meta", "ref", "cuda_ops"]
 
 
+_CUDA = None
+
+
 def cuda_ops():
     """The ctypes binding module (imported lazily so CPU-only use never touches it)."""
-    from . import cuda as _cuda
-    return _cuda
+    global _CUDA
+    if _CUDA is None:
+        from . import cuda
+        _CUDA = cuda
+    return _CUDA
 
 
 def rmsnorm(x, weight, eps):

@@ -629,10 +629,10 @@ def _on_device(fn):
     @functools.wraps(fn)
     def run(t, *args, **kw):
         dev = t.get_device()
-        if dev == torch.cuda.current_device():
-            return fn(t, *args, **kw)
         if dev < 0:
             raise ValueError(f"{fn.__name__}: a tensor on {t.device}, not on the GPU")
+        if dev == torch._C._cuda_getDevice():           # torch.cuda.current_device() costs 0.2 us
+            return fn(t, *args, **kw)
         with torch.cuda.device(dev):
             return fn(t, *args, **kw)
     return run
