@@ -441,7 +441,7 @@ def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep, first=0, re
     ``weights`` ``[pages, Hkv, P]`` (equal weights: the earlier row; NaN counts as the largest).
 
     The rows of ``kv_layer`` ``[pages, 2, Hkv, P, *]`` (any cache type) and their weights are copied, in order, to the rows 0, 1, 2 .. of the
-    pages in ``to_table`` ``[sequences, ceil(keep / P)]``, which must be none of the pages in ``page_table`` ``[sequences, pages]``.
+    pages in ``to_table`` ``[sequences, ceil(keep / P)]``: each of them once, and none that ``page_table`` ``[sequences, pages]`` names.
     Returns which rows they were, int32 ``[sequences, Hkv, keep]``, -1 behind the last row of a sequence that had fewer than ``keep`` of its
     ``lengths`` ``[sequences]``."""
     f = cuda_ops().kv_evict if kv_layer.is_cuda else ref.kv_evict
