@@ -668,7 +668,7 @@ def _fp4_lib():
     return L
 
 
-_FP4_WRITE = struct.Struct("15P11if")       # Fp4WriteParams (csrc/kernels/kv_fp4.cu)
+_FP4_WRITE = struct.Struct("15P11id")       # Fp4WriteParams (csrc/kernels/kv_fp4.cu)
 _FP4_ATTN = struct.Struct("15P15i2f0P")     # Fp4AttnParams (csrc/kernels/attention_fp4.cu)
 _EVICT = struct.Struct("6P12i")             # EvictParams (csrc/kernels/kv_evict.cu)
 

@@ -42,6 +42,22 @@ def test_write_is_the_host_formulation_bit_by_bit(q_lens, past, hq, hkv, d, page
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rot", [1.0, 0.5])
+def test_rows_as_small_as_eps_are_normalised_bit_by_bit(dtype, rot):
+    """Mean squares near eps, whose own last bits count then; and far below and above it."""
+    hq, hkv, d, t = 6, 3, 128, 400
+    meta, layer, scales, g = make_step([t], [0], 64, hkv, d, seed=4)
+    qkv = (torch.randn(t, (hq + 2 * hkv) * d, generator=g) * torch.tensor([1e-3, 2e-3, 1e-5, 30.0]).repeat(t // 4)[:, None]).to(dtype)
+    cs = ref.rope_cos_sin(t, int(d * rot), 1e4)
+    w = (1 + 0.1 * torch.randn(2, d, generator=g)).to(dtype)
+    host = layer.clone()
+    want = ref.rope_kv_write_fp4(qkv, host, meta, cs, hq, hkv, d, scales, w[0], w[1], 1e-6)
+    gpu = layer.cuda()
+    got = ops.rope_kv_write_fp4(qkv.cuda(), gpu, meta.to("cuda"), cs.cuda(), hq, hkv, d, scales.cuda(), w[0].cuda(), w[1].cuda(), 1e-6)
+    assert torch.equal(got.cpu(), want) and torch.equal(gpu.cpu(), host)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("d,page", [(64, 16), (128, 64), (256, 32)])
 def test_stage_is_the_host_formulation(dtype, d, page):
     meta, layer, scales, _ = make_step([2, 1, 5], [70, 0, 128], page, 2, d)
