@@ -37,10 +37,11 @@ __device__ __forceinline__ float inverse_root(double x) {
 }
 
 // Eight values of a block of 16, whose other eight lie in the neighbouring lane: their codes, the block's scale byte and what the codes stand for.
-// Quotients by a reciprocal and one correction (Markstein 1990) are rounded as a division rounds them, away from the ends of the range.
+// Quotients by a reciprocal and one correction (Markstein 1990) are rounded as a division rounds them, away from the ends of the range; the
+// remainder is taken with the sign that leaves a zero its own.
 __device__ __forceinline__ float quotient(float a, float b, float inv_b) {
     const float q = __fmul_rn(a, inv_b);
-    return __fmaf_rn(__fmaf_rn(-q, b, a), inv_b, q);
+    return __fmaf_rn(-__fmaf_rn(q, b, -a), inv_b, q);
 }
 __device__ __forceinline__ bool middling(float x) { return x > 1e-18f && x < 1e18f; }
 
