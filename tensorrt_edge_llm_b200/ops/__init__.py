@@ -438,7 +438,8 @@ def paged_attention_fp4(q, kv_layer, meta, scale, scales, sliding_window=None, s
 
 def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep, first=0, recent=0):
     """Shorten cached sequences to ``keep`` rows a KV head: the ``first`` ones, the ``recent`` ones and, of those between, the heaviest by
-    ``weights`` ``[pages, Hkv, P]`` (equal weights: the earlier row; NaN counts as the largest).
+    ``weights`` ``[pages, Hkv, P]`` (equal weights: the earlier row; NaN counts as the largest, a row that has no page
+    as less than any).
 
     The rows of ``kv_layer`` ``[pages, 2, Hkv, P, *]`` (any cache type) and their weights are copied, in order, to the rows 0, 1, 2 .. of the
     pages in ``to_table`` ``[sequences, ceil(keep / P)]``: each of them once, and none that ``page_table`` ``[sequences, pages]`` names.

@@ -1534,8 +1534,8 @@ def kv_evict(kv_layer, weights, page_table, lengths, to_table, keep, first=0, re
             if total > keep:
                 mid = slot[first:total - recent]
                 w = weights[page.clamp(0, pages - 1), h, slot % p][first:total - recent]
-                w = torch.where(w.isnan(), torch.full_like(w, float("inf")), w)
-                rank = torch.where(there[mid], 0, 2) - weights[page.clamp(0, pages - 1), h, slot % p][mid].isnan().int()     # NaN, numbers, no page
+                rank = torch.where(there[mid], -w.isnan().int(), 1)                                                          # NaN, numbers, no page
+                w = torch.where(w.isnan(), torch.full_like(w, float("inf")), w).masked_fill(~there[mid], 0.0)
                 order = torch.sort(-w, stable=True).indices
                 order = order[torch.sort(rank[order], stable=True).indices][:keep - first - recent]
                 pick = torch.cat([slot[:first], mid[order].sort().values, slot[total - recent:]])

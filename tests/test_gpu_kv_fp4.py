@@ -193,6 +193,22 @@ def test_evict(lengths, page, hkv, keep, first, recent, d, kind, ties):
             assert kept[s, h].tolist() == want[s][h] + [-1] * (keep - len(want[s][h]))
 
 
+def test_evict_takes_rows_without_a_page_last():
+    g = torch.Generator().manual_seed(8)
+    table = torch.randperm(300, generator=g).int().view(2, 150)
+    table[:, 3:40:3] = -1
+    table[1, 90:] = -1
+    to = torch.arange(300, 600, dtype=torch.int32).view(2, 150)
+    w = (torch.rand(600, 2, 16, generator=g) - 0.5) * torch.tensor([1.0, math.inf])[torch.randint(0, 2, (600, 2, 16), generator=g)]
+    w[0] = w[299] = math.nan
+    layer, lens = torch.randint(0, 256, (600, 2, 2, 16, 36), generator=g, dtype=torch.uint8), torch.tensor([2400, 2000], dtype=torch.int32)
+    for keep in (100, 1300, 2200):
+        lg, wg, lh, wh = layer.cuda(), w.cuda(), layer.clone(), w.clone()
+        got = ops.kv_evict(lg, wg, table.cuda(), lens.cuda(), to.cuda(), keep, 4, 32)
+        assert torch.equal(got.cpu(), ops.kv_evict(lh, wh, table, lens, to, keep, 4, 32))
+        assert torch.equal(lg.cpu(), lh) and torch.equal(wg.cpu().nan_to_num(7), wh.nan_to_num(7))
+
+
 def test_write_attend_evict_attend_in_a_captured_graph_and_on_another_stream():
     """A conversation: the prompt is written and attended to, steps keep account of the weights, rows are dropped, steps go on over what is left."""
     hq, hkv, d, page, past, keep = 8, 2, 128, 64, 300, 128

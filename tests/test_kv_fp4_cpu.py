@@ -239,6 +239,20 @@ def test_refusals():
         ops.kv_evict(layer, w, table, torch.tensor([1, 2]), to, 4)
 
 
+def test_evict_takes_rows_without_a_page_last_and_the_earlier_first():
+    g = torch.Generator().manual_seed(8)
+    table = torch.tensor([[5, -1, 2, -1, 7]], dtype=torch.int32)
+    w = -torch.rand(10, 1, 16, generator=g)
+    w[2, 0, 4] = -math.inf
+    w[0, 0, ::3] = math.nan                 # of a page that the table does not name
+    layer = torch.randint(0, 256, (10, 2, 1, 16, 36), generator=g, dtype=torch.uint8)
+    for keep in (30, 45, 60):
+        got = ops.kv_evict(layer.clone(), w.clone(), table, torch.tensor([80], dtype=torch.int32), torch.tensor([[0, 1, 3, 4]], dtype=torch.int32), keep, 0, 0)[0, 0].tolist()
+        there = sorted((i for i in range(80) if i // 16 in (0, 2, 4)), key=lambda i: (-float(w[table[0, i // 16], 0, i % 16]), i))
+        gone = [i for i in range(80) if i // 16 in (1, 3)]
+        assert got == sorted((there + gone)[:keep])
+
+
 def test_requests_in_flight_over_four_bit_pages_are_the_static_ones():
     from tensorrt_edge_llm_b200.runtime.llm import LLM
     from tensorrt_edge_llm_b200.runtime.runner import SamplingParams
