@@ -864,7 +864,7 @@ def parse_quant_config(model_dir: str, hf: Optional[Dict[str, Any]] = None) -> Q
     elif quant_type in (QUANT_INT4_AWQ, QUANT_INT4_GPTQ):
         group = int(qc.get("group_size", qc.get("q_group_size", AWQ_GROUP)))
     kv = qc.get("kv_cache_quant_algo") or (qc.get("kv_cache_scheme") and "fp8")
-    kv = "fp8" if kv and "FP8" in str(kv).upper() else "nvfp4" if kv and "FP4" in str(kv).upper() else None
+    kv = "fp8" if kv and "FP8" in str(kv).upper() else "nvfp4" if kv and "NVFP4" in str(kv).upper() else None
     excluded = list(qc.get("exclude_modules") or qc.get("ignore") or qc.get("modules_to_not_convert") or [])
     return QuantConfig(quant_type=quant_type, group_size=group, kv_cache_quant=kv, excluded=excluded,
                        awq_layout="autoawq" if method == "awq" else "modelopt",

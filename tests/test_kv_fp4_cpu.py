@@ -267,3 +267,21 @@ def test_requests_in_flight_over_four_bit_pages_are_the_static_ones():
     flight = LLM(cfg, enable_in_flight_batching=True, enable_prefix_cache=True, **kw)
     assert [o.token_ids for o in flight.generate(prompts, sp)] == want
     assert [o.token_ids for o in flight.generate(prompts, sp)] == want
+
+
+@pytest.mark.parametrize("flight", [False, True])
+def test_draft_trees_over_four_bit_pages_are_lossless(flight):
+    """Verification goes through 16-bit copies, steps read the pages in place, accepted rows move: the tokens are those of plain decoding."""
+    from tensorrt_edge_llm_b200.runtime.llm import LLM
+    from tensorrt_edge_llm_b200.runtime.runner import SamplingParams
+    from tensorrt_edge_llm_b200.runtime.speculative import SpecConfig
+    sizes = dict(vocab_size=256, dtype="float32", head_dim=64, num_attention_heads=4, num_key_value_heads=2, hidden_size=128)
+    cfg, dcfg = tiny_llama_config(num_hidden_layers=4, **sizes), tiny_llama_config(num_hidden_layers=1, **sizes)
+    dcfg.draft_type, dcfg.eagle3_target_hidden_size, dcfg.draft_vocab_size = "eagle3", 128, 0
+    g = torch.Generator().manual_seed(12)
+    prompts = [torch.randint(0, 256, (n,), generator=g).tolist() for n in (19, 34)]
+    sp = SamplingParams(max_tokens=10, ignore_eos=True)
+    kw = dict(device="cpu", max_batch_size=2, max_input_len=64, max_kv_cache_capacity=128, page_size=16, kv_cache_dtype="nvfp4", random_init_seed=0)
+    want = [o.token_ids for o in LLM(cfg, **kw).generate(prompts, sp)]
+    spec = LLM(cfg, draft_model=dcfg, speculative=SpecConfig(draft_steps=3, top_k=2, verify_tokens=8), enable_in_flight_batching=flight, **kw)
+    assert spec.kv.kv_fp4 and [o.token_ids for o in spec.generate(prompts, sp)] == want
