@@ -408,7 +408,8 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
     if (d != 64 && d != 128 && d != 256) return fail("telb_rope_kv_write_fp4: head_dim must be 64, 128 or 256");
     if (p.rot < 0 || p.rot > d || p.rot % (d / 16)) return fail("telb_rope_kv_write_fp4: the rotated part must be a multiple of head_dim / 16");
     if (p.rot == d) {
-        // A warp for all heads of a token where that fills the device, else one for every group of heads
+        // A warp for all heads of a token where that fills the device, else several, up to one for every group of heads.  32 / 8 heads of 128, 1, 2, 4, 12
+        // warps a token (us): 64 tokens 11.6, 7.7, 5.9, 4.8; 500: 12.1, 8.7, 8.2, 8.1; 2000: 21, 19, 19, 24; 8129: 51, 52, 59, 85.
         const int groups = (p.hq + 2 * p.hkv + 512 / d - 1) / (512 / d);
         const int parts = (int)min((long long)groups, max(1LL, (16LL * 4 * sm_count() + p.tokens - 1) / p.tokens));
         const long long warps = (long long)p.tokens * parts;
