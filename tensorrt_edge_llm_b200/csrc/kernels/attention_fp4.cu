@@ -947,12 +947,12 @@ int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t st
 }
 
 template <typename T, int D>
-int launch_attention_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
+int launch_attention_fp4(const Fp4AttnParams& p, int cols, cudaStream_t stream) {
     const int columns = p.max_q_len * (p.hq / p.hkv);
     constexpr int kMost = D == 256 ? 1 : 2;
     if (!p.weights)
-        return columns <= 8 ? launch_attention_fp4_nt<T, D, 1, false>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost, false>(p, columns, stream);
-    const int rc = columns <= 8 ? launch_attention_fp4_nt<T, D, 1, true>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost, true>(p, columns, stream);
+        return cols == 8 ? launch_attention_fp4_nt<T, D, 1, false>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost, false>(p, columns, stream);
+    const int rc = cols == 8 ? launch_attention_fp4_nt<T, D, 1, true>(p, columns, stream) : launch_attention_fp4_nt<T, D, kMost, true>(p, columns, stream);
     if (rc || (p.ranks > 0 && p.max_items == p.hkv)) return rc;     // a cluster has all columns of its keys: it adds the weights itself
     TELB_LAUNCH("attention_fp4_weights_kernel", attention_fp4_weights_kernel, dim3((p.tiles + 3) / 4, p.hkv, p.num_seqs), dim3(128), 0, stream, p);
     return 0;
@@ -962,21 +962,17 @@ int launch_attention_fp4(const Fp4AttnParams& p, cudaStream_t stream) {
 
 using namespace telb;
 
-// Columns (rows x heads of a KV head) that an item takes, of a step with `columns` of them.
-// 16 expand the keys half as often as 8 where there are more (8 heads of 128, 8 against 16 at a time, us: 16 sequences of 2000 keys, 64 columns: 65 against 57, 16 columns:
-// 25 against 26; 64 of 1000, 16 columns: 40 against 38; one of 8000, 16: 16 against 15; 4 of 2000, 16: 11 against 13.5); of 256 features their outputs would not fit the registers.
-static int fp4_columns(int columns, int d) { return columns <= 8 || d == 256 ? 8 : 16; }
-// CTAs that run at once.
-extern "C" int telb_attention_fp4_ctas(int columns, int d) {
-    const int nt = fp4_columns(columns, d) / 8;
+// CTAs that run at once, with items of `cols` columns.
+extern "C" int telb_attention_fp4_ctas(int cols, int d) {
+    const int nt = cols / 8;
     return sm_count() * (d * nt <= 128 ? 4 : d * nt <= 256 && d < 256 ? 3 : 2);
 }
 
 // ranks > 0: clusters of so many CTAs per item (sequence, KV head, C columns); 0: the line of all items' tiles cut into `ctas` parts, with
-// part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C: 8, or 16 for more than 8 columns of at most 128 features; max_items = KV heads x chunks of the longest
+// part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C = cols: 8, or 16 of at most 128 features; max_items = KV heads x chunks of the longest
 // sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2]
 // and `scores` [num_seqs, hkv, columns / 8, tiles, 2, 8, pairs] float4 are scratch: `tiles` of 32 keys hold every sequence's, `pairs` columns of 8 (at most 4).
-extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int is_bf16, cudaStream_t stream) {
+extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int cols, int d, int is_bf16, cudaStream_t stream) {
     const Fp4AttnParams& p = *params;
     if (p.tokens <= 0 || p.num_seqs <= 0) return 0;
     if (d != 64 && d != 128 && d != 256) return fail("telb_paged_attention_fp4: head_dim must be 64, 128 or 256");
@@ -984,7 +980,8 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (p.hkv <= 0 || p.hq % p.hkv) return fail("telb_paged_attention_fp4: query heads must be a multiple of the KV heads");
     if (p.ranks < 0 || p.ranks > 16) return fail("telb_paged_attention_fp4: clusters of at most 16 CTAs");
     if (p.ranks == 0 && (p.ctas < 1 || !p.part_o || !p.part_ml || !p.spans)) return fail("telb_paged_attention_fp4: no room for the parts");
-    const int columns = p.max_q_len * (p.hq / p.hkv), cols = fp4_columns(columns, d);
+    const int columns = p.max_q_len * (p.hq / p.hkv);
+    if (cols != 8 && (cols != 16 || d == 256)) return fail("telb_paged_attention_fp4: items of 8 columns, or 16 of at most 128 features");
     if (p.max_items != p.hkv * ((columns + cols - 1) / cols)) return fail("telb_paged_attention_fp4: items of another size");
     if (p.max_items > 65535) return fail("telb_paged_attention_fp4: too many rows x heads");
     if (2LL * p.hkv * p.page_size * (d / 2 + d / 16) >= 1LL << 31) return fail("telb_paged_attention_fp4: pages of less than 2 GB");
@@ -992,11 +989,11 @@ extern "C" int telb_paged_attention_fp4(const Fp4AttnParams* params, int d, int 
     if (p.weights && (!p.stat || !p.scores || p.tiles < 1 || p.pairs < 1 || p.pairs > 4 || p.hkv > 65535)) return fail("telb_paged_attention_fp4: weights without room for the scores");
     if (!p.weights && p.scores) return fail("telb_paged_attention_fp4: scores are kept for weights");
     if (is_bf16) {
-        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, stream);
-        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, stream);
-        return launch_attention_fp4<__nv_bfloat16, 256>(p, stream);
+        if (d == 128) return launch_attention_fp4<__nv_bfloat16, 128>(p, cols, stream);
+        if (d == 64) return launch_attention_fp4<__nv_bfloat16, 64>(p, cols, stream);
+        return launch_attention_fp4<__nv_bfloat16, 256>(p, cols, stream);
     }
-    if (d == 128) return launch_attention_fp4<__half, 128>(p, stream);
-    if (d == 64) return launch_attention_fp4<__half, 64>(p, stream);
-    return launch_attention_fp4<__half, 256>(p, stream);
+    if (d == 128) return launch_attention_fp4<__half, 128>(p, cols, stream);
+    if (d == 64) return launch_attention_fp4<__half, 64>(p, cols, stream);
+    return launch_attention_fp4<__half, 256>(p, cols, stream);
 }

@@ -660,7 +660,7 @@ def _fp4_lib():
     """The kernel library with the argument types of these entry points."""
     L, i, p = lib(), c_int, c_vp
     L.telb_rope_kv_write_fp4.argtypes = [ctypes.c_char_p, i, i, p]
-    L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, p]
+    L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, i, p]
     L.telb_attention_fp4_ctas.argtypes = [i, i]
     L.telb_kv_fp4_stage.argtypes = [p] * 7 + [i] * 10 + [p]
     L.telb_kv_evict.argtypes = [ctypes.c_char_p, p]
@@ -806,14 +806,17 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     q = _aligned(q)
     out = torch.empty_like(q)
     dev, n, L = q.get_device(), meta.num_seqs, _fp4_lib()
-    cols = 8 if columns <= 8 or d == 256 else 16          # columns of an item, as the launcher has it
-    items = hkv * -(-columns // cols)
     tiles = -(-min(meta.max_seq_len, window + meta.max_q_len if window else meta.max_seq_len) // 32) + 1
+    # Columns of an item.  16 expand the keys half as often, 8 are quicker to begin and to join and leave more CTAs an SM.  8 heads of 128, 8 : 16 (us): one
+    # sequence of 1000 keys, 16 columns 6.5 : 7.8, 4 of 2000 9.7 : 12.4, 16 of 1000 13.2 : 16.5, 8 of 4000 24.0 : 24.5, 64 of 1000 39.7 : 38.3; 64 columns: 4 of 2000
+    # 23.9 : 24.2, one of 8000 24.7 : 23.7, 16 of 2000 65 : 57.  The outputs of 16 columns of 256 features would not fit the registers.
+    cols = 8 if columns <= 8 or d == 256 or n * hkv * -(-columns // 8) * tiles <= 16384 else 16
+    items = hkv * -(-columns // cols)
     ranks = 0
     if ctas is None:
         # keeping account of the weights, a CTA of 8 columns waits more: 16 sequences of 8192 keys, 8 heads: 2, 4, 8 CTAs 61, 55, 59 us
         ranks = _fp4_ranks(n * items, tiles, 512 if weights is not None and cols == 8 else 256)
-        ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(columns, d), n * items * tiles // 4))
+        ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(cols, d), n * items * tiles // 4))
     elif ctas < 0:
         ranks, ctas = -ctas, 0
     part_o = part_ml = spans = stat = scores = pairs = 0
@@ -830,7 +833,7 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     ptr = _ptrs("paged_attention_fp4", dev, (q, kv_layer, out, meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights))
     p = _FP4_ATTN.pack(*ptr[:3], part_o, part_ml, stat, *ptr[3:], spans, scores, n, t, meta.max_q_len, pages, meta.page_table.shape[1], meta.page_size,
                        meta.page_size.bit_length() - 1, hq, hkv, window, ctas, ranks, items, tiles, pairs, scale, decay)
-    _check(L.telb_paged_attention_fp4(p, d, is_bf16, _raw_stream(dev)), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None and not (ranks and items == hkv)))
+    _check(L.telb_paged_attention_fp4(p, cols, d, is_bf16, _raw_stream(dev)), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None and not (ranks and items == hkv)))
     return out
 
 
