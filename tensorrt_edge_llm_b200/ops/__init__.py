@@ -234,7 +234,7 @@ def stream_norm(stream, weight, eps, *, delta=None, routed=None, mult=1.0, step=
 
 
 # Rows x heads of a KV head up to which a step reads four-bit pages in place; more are expanded to 16 bits first.  With 32, 64, 128 of them (us, in
-# place : expanded): one sequence of 8000 keys 20, 24, 38 : 29, 31, 31; 4 of 2000 17, 24, 37 : 29, 30, 33; 16 of 2000 38, 57, 92 : 70, 71, 72.
+# place : expanded): one sequence of 8000 keys 17, 25, 38 : 29, 31, 31; 4 of 2000 16, 23, 37 : 29, 29, 33; 16 of 2000 38, 57, 91 : 70, 71, 72.
 FP4_DIRECT_COLUMNS = 64
 FP4_WEIGHT_COLUMNS = 256     # and up to which it can keep account of the attention weights
 
