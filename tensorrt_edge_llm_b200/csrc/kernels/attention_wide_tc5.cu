@@ -35,6 +35,7 @@ struct AttnWideParams {
     int window;                // sliding window, 0 = none, -1 = every row sees every cached and new token
     float scale_log2;          // softmax scale * log2(e), positive
     const float* kv_scales;    // [2], of the scaled form: factors of the keys and of the values
+    const uint8_t* kv_holes;   // [N, max_pages], of the scaled form over pages of 64: a bit per 16 keys that are not there; or null
     int* status;
 };
 
@@ -260,6 +261,10 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
         float m_used = -INFINITY, l_sum = 0.f;
         bool ok = true;
         for (int j = 0; j < ntiles; ++j) {
+            // two pages of 64 keys, four bits each; a sequence's row has an even number of pages
+            uint32_t gone = 0u;
+            if constexpr (kScaled)
+                if (p.kv_holes) gone = *reinterpret_cast<const uint16_t*>(p.kv_holes + (size_t)seq * p.max_pages + 2 * (j0 + j));
             if (!mbar_wait(&s_full[t], j & 1, abort_flag, p.status, kStatusEpilogueTimeout)) { ok = false; break; }
             tc_fence_after_sync();
             uint32_t s[4][32];
@@ -268,7 +273,7 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
             tmem_ld_wait();
             const int c0 = (j0 + j) * 128;
             // tiles that every row of this query tile sees whole need no mask (most tiles of a long prompt)
-            const bool whole = !mask_row && p.window <= 0 && c0 + 127 <= (p.window < 0 ? past + qlen - 1 : past + first);
+            const bool whole = !mask_row && p.window <= 0 && gone == 0u && c0 + 127 <= (p.window < 0 ? past + qlen - 1 : past + first);
             if (!whole) {
                 if (mask_row) {
 #pragma unroll
@@ -302,6 +307,13 @@ attn_wide_kernel(const __grid_constant__ CUtensorMap tma_q, const __grid_constan
 #pragma unroll
                         for (int i = 0; i < 32; ++i)
                             if (c * 32 + i > hi || c * 32 + i < lo) s[c][i] = 0xff800000u;
+                }
+                if (kScaled && gone != 0u) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((gone >> ((c >> 1) * 8 + (c & 1) * 2 + (i >> 4))) & 1u) s[c][i] = 0xff800000u;
                 }
             }
             float mx[4];
@@ -439,7 +451,7 @@ extern "C" int telb_paged_attention_wide(const void* q, const void* kv_layer, vo
                                          const int* past_len, const int* page_table, const int* tree_mask, int mask_words, int num_seqs,
                                          int total_tokens, int num_pages, int max_pages, int page_size, int hq, int hkv, float scale,
                                          int window, int splits, float* ws, long long ws_floats, int is_bf16, int* status, const float* kv_scales,
-                                         cudaStream_t stream) {
+                                         const uint8_t* kv_holes, cudaStream_t stream) {
     AttnWideParams p{};
     p.out = out;
     p.q_start = q_start;
@@ -459,6 +471,7 @@ extern "C" int telb_paged_attention_wide(const void* q, const void* kv_layer, vo
     p.window = window;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.kv_scales = kv_scales;
+    p.kv_holes = kv_holes;
     p.status = status;
     if (splits < 1) splits = 1;
     while (splits > 1 && (long long)splits * total_tokens * hq * 129 > ws_floats) --splits;

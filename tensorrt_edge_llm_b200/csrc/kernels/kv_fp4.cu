@@ -315,9 +315,10 @@ __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4Wr
 }
 
 // A CTA per page of the 16-bit copy (64 rows; logical page blockIdx.x, plane (K|V, head) blockIdx.y, sequence blockIdx.z); a thread expands blocks of 16
-// features.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero.
+// features.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero.  holes[seq, lp] says which of a page's
+// four groups of 16 rows the cache does not have: their zeros must not be taken for keys.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table,
+__global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table, uint8_t* __restrict__ holes,
                                                            const int* __restrict__ past_len, const int* __restrict__ q_len, const int* __restrict__ page_table,
                                                            const float* __restrict__ scales, int max_pages, int num_pages, int page_shift, int stage_pages, int hkv,
                                                            int window, int own) {
@@ -325,6 +326,12 @@ __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __rest
     const int seq = blockIdx.z, lp = blockIdx.x, plane = blockIdx.y;
     if (plane == 0 && threadIdx.x == 0) stage_table[seq * stage_pages + lp] = seq * stage_pages + lp;
     const int past = past_len[seq], total = past + q_len[seq], count = own ? total : past;
+    if (plane == 0 && threadIdx.x < 32) {
+        const int slot = lp * 64 + 16 * threadIdx.x, at = slot >> page_shift;
+        const int page = threadIdx.x < 4 && slot < total && at < max_pages ? page_table[(size_t)seq * max_pages + at] : -1;
+        const unsigned gone = __ballot_sync(0xffffffffu, threadIdx.x < 4 && slot < total && (unsigned)page >= (unsigned)num_pages);
+        if (threadIdx.x == 0) holes[seq * stage_pages + lp] = (uint8_t)gone;
+    }
     if (window > 0 && (lp + 1) * 64 + 2 * 128 <= past - window) return;        // before every tile that the windowed kernels touch
     const size_t slab = fp4_slab_bytes(1 << page_shift, D);
     const float scale = scales ? scales[plane >= hkv] : 1.f;
@@ -444,8 +451,9 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
 }
 
 // pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [num_seqs * stage_pages, 2, Hkv, 64, d], page s * stage_pages + i for
-// rows 64 i.. of sequence s.  own: the step's own rows too.  `scales` null: code * block scale, which both 16-bit types hold exactly.
-extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table, const int* past_len, const int* q_len, const int* page_table, const float* scales,
+// rows 64 i.. of sequence s; holes [num_seqs, stage_pages] bytes: bit i is set where the rows 16 i .. 16 i + 15 of a page have no page of the pool.  own: the step's own
+// rows too.  `scales` null: code * block scale, which both 16-bit types hold exactly.
+extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table, uint8_t* holes, const int* past_len, const int* q_len, const int* page_table, const float* scales,
                                  int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d, int window, int own, int is_bf16,
                                  cudaStream_t stream) {
     if (num_seqs <= 0 || stage_pages <= 0) return 0;
@@ -455,7 +463,7 @@ extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table
     int shift = 0;
     while (1 << shift < page_size) ++shift;
     const dim3 grid(stage_pages, 2 * hkv, num_seqs), blk(256);
-#define STAGE_FP4(T, D) TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<T, D>), grid, blk, 0, stream, (const uint8_t*)pool, (T*)stage, stage_table, past_len, q_len, \
+#define STAGE_FP4(T, D) TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<T, D>), grid, blk, 0, stream, (const uint8_t*)pool, (T*)stage, stage_table, holes, past_len, q_len, \
                                     page_table, scales, max_pages, num_pages, shift, stage_pages, hkv, window, own)
     if (is_bf16) {
         if (d == 128) STAGE_FP4(__nv_bfloat16, 128);

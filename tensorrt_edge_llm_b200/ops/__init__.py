@@ -418,7 +418,8 @@ def fp4_weighed(meta, group):
 def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
     """16-bit copies of the rows that the step's sequences have in a four-bit layer, for the prompt kernels: ``(stage, meta)`` with the pages
     ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  The rows cached before the step, and its own with ``new_rows`` (else their
-    places are left for :func:`rope_kv_write_fp4` to fill); what lies behind in a page is zero.  ``window`` > 0: pages that no row of the
+    places are left for :func:`rope_kv_write_fp4` to fill); what lies behind in a page is zero, and so are rows without a page, which
+    :func:`paged_attention` would take for keys (:func:`paged_attention_fp4` hides them).  ``window`` > 0: pages that no row of the
     step can see may be left out."""
     f = cuda_ops().kv_fp4_stage if kv_layer.is_cuda else ref.kv_fp4_stage
     return f(kv_layer, meta, scales, dtype, window, new_rows)
@@ -426,7 +427,7 @@ def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
 
 def paged_attention_fp4(q, kv_layer, meta, scale, scales, sliding_window=None, sinks=None, weights=None, decay=1.0):
     """:func:`paged_attention` over four-bit pages (see :func:`rope_kv_write_fp4`), which hold the step's rows already.  Steps of few rows read
-    them in place; longer ones, and tree masks, go through :func:`kv_fp4_stage`.  A row that sees no key gives zeros.
+    them in place; longer ones, and tree masks, go through :func:`kv_fp4_stage`.  Keys without a page are hidden; a row that sees no key gives zeros.
 
     ``weights`` (fp32 ``[pages, Hkv, P]``, causal steps of at most 256 rows x heads of a KV head): every key that some row of the step sees
     gets ``decay * weights + `` the sum of its softmax weights over those rows and the query heads of the KV head; the step's own keys

@@ -662,7 +662,7 @@ def _fp4_lib():
     L.telb_rope_kv_write_fp4.argtypes = [ctypes.c_char_p, i, i, p]
     L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, i, p]
     L.telb_attention_fp4_ctas.argtypes = [i, i]
-    L.telb_kv_fp4_stage.argtypes = [p] * 7 + [i] * 10 + [p]
+    L.telb_kv_fp4_stage.argtypes = [p] * 8 + [i] * 10 + [p]
     L.telb_kv_evict.argtypes = [ctypes.c_char_p, p]
     L.telb_kv_fp4_commit_path.argtypes = [p] * 5 + [i] * 8 + [p]
     return L
@@ -729,18 +729,19 @@ def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: i
     pages, hkv, d = _fp4_geometry(kv_layer, meta, scales)
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"kv_fp4_stage: pages of fp16 or bf16, not {dtype}")
-    return _fp4_stage(kv_layer, meta, scales, dtype, window, new_rows, pages, hkv, d)
+    return _fp4_stage(kv_layer, meta, scales, dtype, window, new_rows, pages, hkv, d)[:2]
 
 
 def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int, new_rows: bool, pages: int, hkv: int, d: int):
-    """Without ``scales``: codes times block scales, which both 16-bit types hold exactly."""
-    n, per, dev = meta.num_seqs, max(1, (meta.max_seq_len + 63) // 64), kv_layer.get_device()
+    """Without ``scales``: codes times block scales, which both 16-bit types hold exactly.  A third result tells the prompt kernels which rows the cache
+    does not have: a byte per page, a bit per 16 rows."""
+    n, per, dev = meta.num_seqs, 2 * max(1, (meta.max_seq_len + 127) // 128), kv_layer.get_device()     # whole 128-key tiles
     stage = torch.empty(n * per, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
-    table = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device)
+    table, holes = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device), torch.empty(n, per, dtype=torch.uint8, device=kv_layer.device)
     _check(_fp4_lib().telb_kv_fp4_stage(
-        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, meta.past_len, meta.q_len, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
+        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, holes, meta.past_len, meta.q_len, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
         meta.page_size, per, hkv, d, window or 0, int(new_rows), int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
-    return stage, dataclasses.replace(meta, page_table=table, page_size=64)
+    return stage, dataclasses.replace(meta, page_table=table, page_size=64), holes
 
 
 def _fp4_commit_path(pool, page_table, past_len, path, path_len) -> None:
@@ -801,8 +802,8 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
         if direct:
             raise ValueError("paged_attention_fp4: tree masks are read by the prompt kernels only")
         # the two global scales multiply scores and outputs, in 32 bits
-        stage, staged = _fp4_stage(kv_layer, meta, None, q.dtype, window, True, pages, hkv, d)
-        return paged_attention(q, stage, staged, scale, sliding_window, sinks, kv_scales=scales)
+        stage, staged, holes = _fp4_stage(kv_layer, meta, None, q.dtype, window, True, pages, hkv, d)
+        return paged_attention(q, stage, staged, scale, sliding_window, sinks, kv_scales=scales, kv_holes=holes)
     q = _aligned(q)
     out = torch.empty_like(q)
     dev, n, L = q.get_device(), meta.num_seqs, _fp4_lib()
@@ -918,14 +919,15 @@ def _decode_splits(meta: StepMeta, hkv: int, chunk: int = 0, window: int = 0, fp
 def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sinks=None, splits: Optional[int] = None,
                     kernel: Optional[str] = None, trace: Optional[torch.Tensor] = None, causal: bool = True,
                     skip_thr: Optional[torch.Tensor] = None, skip_stats: Optional[torch.Tensor] = None, chunk: int = 0,
-                    fp32_weights: bool = False, back: Optional[tuple] = None, out: Optional[torch.Tensor] = None, kv_scales: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    fp32_weights: bool = False, back: Optional[tuple] = None, out: Optional[torch.Tensor] = None, kv_scales: Optional[torch.Tensor] = None,
+                    kv_holes: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Paged GQA attention.  Decode-shaped steps (``max_q_len * Hq/Hkv <= 16``, head_dim 128, causal)
     run the token-major XQA-style kernel; everything else the row-major tile kernel, or its two-tile form for plain steps of head size 128
     that it suits (all of them where ``splits`` is given).
     ``kernel`` forces ``"decode"`` or ``"tile"`` (one tile a CTA); ``causal=False`` lets every row see every token of its sequence; ``chunk`` > 0 limits
     a row to the keys of its own ``chunk``-token block; ``fp32_weights`` feeds the probabilities to the 16-bit P·V product as high + low
     halves.  ``kv_scales`` (two positive fp32 numbers on the device): keys and values are multiplied by them, in 32 bits, on the scores and the outputs (tile
-    kernels only).  fp32 rows and head sizes without a tensor-core form run on the CUDA cores."""
+    kernels only), and ``kv_holes`` (bytes ``[sequences, pages]`` of 64-row pages) has a bit for every 16 keys that are not there.  fp32 rows and head sizes without a tensor-core form run on the CUDA cores."""
     wide = kernel is None
     if not causal:
         sliding_window, kernel = -1, "tile"
@@ -988,7 +990,7 @@ def paged_attention(q, kv_layer, meta: StepMeta, scale, sliding_window=None, sin
         c_int(kv_layer.shape[0]), c_int(meta.page_table.shape[1]), c_int(meta.page_size), c_int(hq), c_int(hkv),
         c_int(d), c_float(scale), c_int(sliding_window or 0), c_int(splits), _p(ws.attn_ws), c_ll(ws.attn_ws.numel()),
         c_int(_is_bf16(q)), _p(ws.status), _p(sinks), _p(skip_thr), _p(skip_stats), c_int(chunk), c_int(int(fp32_weights)),
-        _p(table), c_float(mult), _p(meta.positions), c_ll(ld_out), c_int(int(wide)), _p(kv_scales), _stream()), "paged_attention", 2 if splits > 1 else 1)
+        _p(table), c_float(mult), _p(meta.positions), c_ll(ld_out), c_int(int(wide)), _p(kv_scales), _p(kv_holes), _stream()), "paged_attention", 2 if splits > 1 else 1)
     return out
 
 

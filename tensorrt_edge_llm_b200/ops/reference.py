@@ -1443,7 +1443,7 @@ def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads, num_k
 
 def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype, window=0, new_rows=False):
     d = fp4_head_dim(kv_layer)
-    n, per = meta.num_seqs, max(1, (meta.max_seq_len + 63) // 64)
+    n, per = meta.num_seqs, 2 * max(1, (meta.max_seq_len + 127) // 128)         # whole 128-key tiles
     stage = torch.zeros(n * per, 2, kv_layer.shape[2], 64, d, dtype=dtype, device=kv_layer.device)
     table = torch.arange(n * per, dtype=torch.int32, device=kv_layer.device).view(n, per)
     for s in range(n):
@@ -1464,9 +1464,6 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale, scales, sliding_wind
     g = hq // hkv
     if weights is not None and (meta.tree_mask is not None or meta.max_q_len * g > 256):
         raise ValueError("paged_attention_fp4: weights are kept for causal steps of at most 256 rows x heads of a KV head")
-    if meta.tree_mask is not None:
-        stage, staged = kv_fp4_stage(kv_layer, meta, scales, q.dtype, 0, True)
-        return paged_attention(q, stage, staged, scale, sliding_window, sinks)
     window = sliding_window if sliding_window and sliding_window > 0 else 0
     out = torch.empty_like(q)
     for s in range(meta.num_seqs):
@@ -1479,6 +1476,9 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale, scales, sliding_wind
         page = F.pad(meta.page_table[s].long(), (0, (total + p - 1) // p), value=-1)[cols // p]
         there = (page >= 0) & (page < kv_layer.shape[0])
         seen = (cols <= rows) & there
+        if meta.tree_mask is not None:
+            new = (cols - past).clamp(min=0)
+            seen = ((cols < past) | ((meta.tree_mask[r0:r0 + ql].long().gather(1, (new // 32).expand(ql, -1)) >> (new % 32)) & 1).bool()) & there
         if window:
             seen = seen & (cols > rows - window)
         sc = (q[r0:r0 + ql].float().view(ql, hkv, g, d).permute(1, 2, 0, 3) @ kv[0].transpose(-1, -2)[:, None]) * scale

@@ -1,0 +1,37 @@
+"""Steps that are too long to read four-bit pages in place, on the GPU: tables with holes, trees and windows against a 64-bit oracle."""
+import pytest
+import torch
+
+from fp4_expanded_cases import holey_step, oracle
+from tensorrt_edge_llm_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(want, top, kq, dtype):
+    """Codes times block scales have at most six significant bits: keys and values are exact in 16 bits.  Left are half a step of the result; half a step of the
+    probabilities, of the largest value; scores whose 32-bit sums over 16 steps of a matrix product are off by 16 steps of 2^-22 of |q| |k| at most, a probability
+    by as much and its sum again; and fp16 probabilities below 2^-14 of the largest, off by 2^-25 each, some thousand of them."""
+    half = torch.finfo(dtype).eps / 2
+    return half * want.abs() + (half + 2 * 2 ** -18 * kq + 2 ** -14) * top
+
+
+# q_lens, past, query heads, KV heads, head size, page, missing logical pages, window, tree
+STEPS = [([40], [100], 8, 2, 128, 64, [[0]], 0, False), ([70, 5, 300], [30, 200, 0], 8, 2, 128, 64, [[1], [0, 2], [2]], 0, False), ([600], [900], 32, 8, 128, 16, [[3, 50, 51, 70]], 0, False),
+         ([40, 100], [260, 7], 16, 4, 64, 32, [[0, 3], [2]], 0, False), ([33], [500], 8, 2, 256, 16, [[0, 1, 20]], 0, False), ([8, 20], [300, 64], 4, 2, 128, 32, [[2, 5], [0]], 0, True),
+         ([40], [130], 4, 2, 64, 16, [[3, 9]], 0, True), ([50], [700], 8, 2, 128, 64, [[9, 11]], 260, False), ([40], [700], 8, 2, 64, 64, [[9, 11]], 260, False),
+         ([90], [38], 8, 2, 128, 128, [[0]], 0, False), ([90, 30], [38, 0], 8, 2, 64, 16, [list(range(8)), [0, 1]], 0, False), ([24], [3000], 8, 2, 128, 64, [[2, 3, 30]], 0, False)]
+
+
+@pytest.mark.parametrize("q_lens,past,hq,hkv,d,page,missing,window,tree", STEPS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sunk", [False, True])
+def test_holes_are_hidden_from_expanded_steps(q_lens, past, hq, hkv, d, page, missing, window, tree, dtype, sunk):
+    meta, layer, scales, g = holey_step(q_lens, past, page, hkv, d, missing, seed=sum(past) + d, window=window, tree=tree)
+    q = (torch.randn(sum(q_lens), hq, d, generator=g) * 2).to(dtype)
+    sinks = torch.randn(hq, generator=g) if sunk else None
+    want, top, kq = oracle(q, layer, meta, d ** -0.5, scales, window, sinks)
+    got = ops.cuda_ops().paged_attention_fp4(q.cuda(), layer.cuda(), meta.to("cuda"), d ** -0.5, scales.cuda(), window or None, None if sinks is None else sinks.cuda(), direct=False)
+    assert ((got.cpu().double() - want).abs() <= bound(want, top, kq, dtype)).all()
+    assert torch.equal(got, ops.paged_attention_fp4(q.cuda(), layer.cuda(), meta.to("cuda"), d ** -0.5, scales.cuda(), sliding_window=window or None,
+                                                    sinks=None if sinks is None else sinks.cuda())) or (not tree and max(q_lens) * hq // hkv <= ops.FP4_DIRECT_COLUMNS)
