@@ -173,11 +173,11 @@ struct ValueTile {
             else s[i] = *reinterpret_cast<const uint16_t*>(f + 2 * g);
         }
     }
-    // Keys from `live` on: what lies there may be anything, NaN scales too (a zero scale takes them out).
-    __device__ __forceinline__ void clear(int t, int live) {
+    // Keys before `from` and from `live` on, which no row sees: what lies there may be anything, NaN scales too (a zero scale takes them out).
+    __device__ __forceinline__ void clear(int t, int from, int live) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (place(i, t) >= live) s[i] = 0;
+            if (place(i, t) < from || place(i, t) >= live) s[i] = 0;
     }
     template <int NT>
     __device__ __forceinline__ void add(const uint32_t (&pb)[NT][2], float (&o)[NT][D / 16][4]) const {
@@ -386,7 +386,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = p.hq / p.hkv;
     const int r_first = chunk * C / group, r_last = (min(columns, chunk * C + C) - 1) / group;
-    const int end = past + r_last + 1;
+    const int end = past + r_last + 1, begin = p.window > 0 ? max(0, past + r_first + 1 - p.window) : 0;      // the keys that some column sees
     const int all_low = p.window > 0 ? max(0, past + r_last + 1 - p.window) : 0, all_high = past + r_first + 1;      // visible to every column
     Ring ring;
     ring.begin(p, seq, kvh, end, ring_at, lane, first_ids);
@@ -512,7 +512,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
             }
             ValueTile<D> vt;
             vt.load(st + Ring::kCodes + m * (16 * D / 2), st + 2 * Ring::kCodes + Ring::kScales + m * D, g, t);
-            if constexpr (!decltype(open)::value) vt.clear(t, (missing >> m) & 1u ? 0 : end - kb - 16 * m);
+            if constexpr (!decltype(open)::value) vt.clear(t, begin - kb - 16 * m, (missing >> m) & 1u ? 0 : end - kb - 16 * m);
             vt.template add<NT>(pb, o);
         }
     };

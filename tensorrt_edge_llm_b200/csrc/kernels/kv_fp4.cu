@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4Wr
 }
 
 // A CTA per page of the 16-bit copy (64 rows; logical page blockIdx.x, plane (K|V, head) blockIdx.y, sequence blockIdx.z); a thread expands blocks of 16
-// features.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero.  holes[seq, lp] says which of a page's
+// features.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero, and so do those that a window hides from
+// every row, whose values enter the product of a tile times a probability of zero.  holes[seq, lp] says which of a page's
 // four groups of 16 rows the cache does not have: their zeros must not be taken for keys.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table, uint8_t* __restrict__ holes,
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __rest
         if (threadIdx.x == 0) holes[seq * stage_pages + lp] = (uint8_t)gone;
     }
     if (window > 0 && (lp + 1) * 64 + 2 * 128 <= past - window) return;        // before every tile that the windowed kernels touch
+    const int first = window > 0 ? past + 1 - window : 0;
     const size_t slab = fp4_slab_bytes(1 << page_shift, D);
     const float scale = scales ? scales[plane >= hkv] : 1.f;
     T* dst = stage + (((size_t)seq * stage_pages + lp) * 2 * hkv + plane) * 64 * D;
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __rest
     for (int u = 0; u < 64 * B / 256; ++u) {
         const int i = u * 256 + threadIdx.x, r = i / B, b = i % B, slot = lp * 64 + r;
         if (slot >= count && slot < total) continue;
-        const int page = slot < count && slot >> page_shift < max_pages ? page_table[(size_t)seq * max_pages + (slot >> page_shift)] : -1;
+        const int page = slot >= first && slot < count && slot >> page_shift < max_pages ? page_table[(size_t)seq * max_pages + (slot >> page_shift)] : -1;
         uint4 out[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
         if ((unsigned)page < (unsigned)num_pages) {
             const uint8_t* src = pool + ((size_t)page * 2 * hkv + plane) * slab;

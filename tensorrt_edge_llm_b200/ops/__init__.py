@@ -419,8 +419,8 @@ def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
     """16-bit copies of the rows that the step's sequences have in a four-bit layer, for the prompt kernels: ``(stage, meta)`` with the pages
     ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  The rows cached before the step, and its own with ``new_rows`` (else their
     places are left for :func:`rope_kv_write_fp4` to fill); what lies behind in a page is zero, and so are rows without a page, which
-    :func:`paged_attention` would take for keys (:func:`paged_attention_fp4` hides them).  ``window`` > 0: pages that no row of the
-    step can see may be left out."""
+    :func:`paged_attention` would take for keys (:func:`paged_attention_fp4` hides them).  ``window`` > 0: rows that no row
+    of the step can see are zero, and pages of such rows may be left out."""
     f = cuda_ops().kv_fp4_stage if kv_layer.is_cuda else ref.kv_fp4_stage
     return f(kv_layer, meta, scales, dtype, window, new_rows)
 

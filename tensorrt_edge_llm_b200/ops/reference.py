@@ -1449,6 +1449,8 @@ def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype, window=0, new_rows=Fal
     for s in range(n):
         rows = int(meta.past_len[s]) + (int(meta.q_len[s]) if new_rows else 0)
         v = _fp4_round(_fp4_rows(kv_layer, meta.page_table[s], rows, scales), dtype)
+        if window > 0:
+            v[:, :, :max(0, int(meta.past_len[s]) + 1 - window)] = 0.0
         v = F.pad(v, (0, 0, 0, per * 64 - rows)).unflatten(2, (per, 64))
         stage[s * per:(s + 1) * per] = v.permute(2, 0, 1, 3, 4)
     return stage, dataclasses.replace(meta, page_table=table, page_size=64)

@@ -72,3 +72,16 @@ def oracle(q, layer, meta, scale, scales, window=0, sinks=None):
         top = max(top, float(kv[:, 1].abs().max()))
         kq = max(kq, float(qs.norm(dim=-1).max() * kv[:, 0].norm(dim=-1).max()) * scale)
     return out, top, kq
+
+
+def poison_before_the_window(meta, layer, window):
+    """NaN block scales in all cached rows that no row of the step sees."""
+    from tensorrt_edge_llm_b200.ops import reference as ref
+    _, sf = ref.fp4_page_parts(layer)
+    p = layer.shape[3]
+    for s in range(meta.num_seqs):
+        slot = torch.arange(max(0, int(meta.past_len[s]) + 1 - window))
+        pg = meta.page_table[s].long()[slot // p]
+        there = pg >= 0
+        sf[pg[there], :, :, (slot % p)[there]] = 0x7f
+    return layer

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from fp4_expanded_cases import holey_step, oracle
+from fp4_expanded_cases import holey_step, oracle, poison_before_the_window
+from fp4_kv_cases import make_step
 from tensorrt_edge_llm_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -35,3 +36,29 @@ def test_holes_are_hidden_from_expanded_steps(q_lens, past, hq, hkv, d, page, mi
     assert ((got.cpu().double() - want).abs() <= bound(want, top, kq, dtype)).all()
     assert torch.equal(got, ops.paged_attention_fp4(q.cuda(), layer.cuda(), meta.to("cuda"), d ** -0.5, scales.cuda(), sliding_window=window or None,
                                                     sinks=None if sinks is None else sinks.cuda())) or (not tree and max(q_lens) * hq // hkv <= ops.FP4_DIRECT_COLUMNS)
+
+
+# q_lens, past, query heads, KV heads, head size, page, window; the first key that some row sees lies inside a tile of 16, 32, 64 and 128 keys
+WINDOWS = [([1], [700], 8, 2, 128, 64, 130), ([1, 3], [333, 90], 10, 2, 64, 16, 45), ([2], [350], 4, 2, 256, 32, 40), ([5], [900], 16, 2, 128, 64, 257), ([8], [500], 16, 2, 128, 128, 100)]
+
+
+@pytest.mark.parametrize("q_lens,past,hq,hkv,d,page,window", WINDOWS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("direct", [True, False])
+def test_rows_that_a_window_hides_do_not_reach_the_outputs(q_lens, past, hq, hkv, d, page, window, dtype, direct):
+    """A cached row with a NaN is seen while it is in the window and forgotten behind it, although the tile that holds it is still read."""
+    meta, layer, scales, g = make_step(q_lens, past, page, hkv, d, seed=window + d)
+    poison_before_the_window(meta, layer, window)
+    q = (torch.randn(sum(q_lens), hq, d, generator=g) * 2).to(dtype)
+    want, top, kq = oracle(q, layer, meta, d ** -0.5, scales, window)
+    args = (layer.cuda(), meta.to("cuda"), d ** -0.5, scales.cuda(), window)
+    got = ops.cuda_ops().paged_attention_fp4(q.cuda(), *args, direct=direct)
+    assert ((got.cpu().double() - want).abs() <= bound(want, top, kq, dtype)).all()
+    if direct:
+        w = torch.zeros(layer.shape[0], hkv, page, device="cuda")
+        for ctas in (None, 3, -1, -4):
+            got = ops.cuda_ops().paged_attention_fp4(q.cuda(), *args, weights=w, ctas=ctas)
+            assert ((got.cpu().double() - want).abs() <= bound(want, top, kq, dtype)).all() and w.isfinite().all()
+    stage, staged = ops.kv_fp4_stage(layer.cuda(), args[1], args[3], dtype, window, True)
+    plain = ops.paged_attention(q.cuda(), stage, staged, d ** -0.5, window)
+    assert plain.isfinite().all()

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from fp4_expanded_cases import holey_step, oracle
+from fp4_expanded_cases import holey_step, oracle, poison_before_the_window
+from fp4_kv_cases import make_step
 from tensorrt_edge_llm_b200 import ops
 
 # q_lens, past, page, missing logical pages of each sequence, window, tree
@@ -21,3 +22,15 @@ def test_holes_are_hidden_from_every_step(q_lens, past, page, missing, window, t
     got = ops.paged_attention_fp4(q, layer, meta, d ** -0.5, scales, sliding_window=window or None, sinks=sinks)
     # 32-bit: sums of 64 products (64 * 2^-24 of |q| |k|) make a probability off by that, sums of some 300 of them by 300 * 2^-24
     assert ((got.double() - want).abs() <= top * 2 ** -24 * (2 * 64 * kq + 600)).all()
+
+
+def test_rows_that_a_window_hides_do_not_reach_the_outputs():
+    for q_lens, past, window in (([1, 3], [90, 200], 37), ([40], [150], 65)):
+        meta, layer, scales, g = make_step(q_lens, past, 16, 2, 64, seed=window)
+        poison_before_the_window(meta, layer, window)
+        q = torch.randn(sum(q_lens), 6, 64, generator=g)
+        want, top, kq = oracle(q, layer, meta, 0.125, scales, window)
+        got = ops.paged_attention_fp4(q, layer, meta, 0.125, scales, sliding_window=window)
+        assert ((got.double() - want).abs() <= top * 2 ** -24 * (2 * 64 * kq + 600)).all()
+        for new in (False, True):
+            assert ops.kv_fp4_stage(layer, meta, scales, torch.bfloat16, window, new)[0].isfinite().all()
