@@ -314,18 +314,56 @@ __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4Wr
     }
 }
 
-// A CTA per page of the 16-bit copy (64 rows; logical page blockIdx.x, plane (K|V, head) blockIdx.y, sequence blockIdx.z); a thread expands blocks of 16
-// features.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero, and so do those that a window hides from
+// Pages of 64 rows that a sequence takes in a packed copy: whole 128-key tiles, one at least.
+__device__ __forceinline__ int fp4_stage_own(int total, int most) { return min(2 * max(1, (total + 127) / 128), most); }
+
+// A CTA per page of the 16-bit copy (64 rows; page blockIdx.x, plane (K|V, head) blockIdx.y); a thread expands blocks of 16 features.  Packed, the sequences'
+// pages follow one another, and the last page of the copy is zeros for what the table has behind a sequence's own pages; else every sequence has
+// `stage_pages`, and those behind its last 128-key tile, which no kernel reads, are left as they are.  Bound by the bytes, and the launch where they are few:
+// 8 sequences of 1024 rows of 8 heads of 128 10.4 us (43 MB, 0.63 of the copy rate); 63 of 1024 beside one of 32768 109 us (packed; 432 MB written, and the
+// search for a page's sequence, which costs 0.5 us of a small step), 2125 with every sequence as long as the longest.  The step's own rows are left out unless `own`; rows behind them, up to the page's end, become zero, and so do those that a window hides from
 // every row, whose values enter the product of a tile times a probability of zero.  holes[seq, lp] says which of a page's
 // four groups of 16 rows the cache does not have: their zeros must not be taken for keys.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __restrict__ pool, T* __restrict__ stage, int* __restrict__ stage_table, uint8_t* __restrict__ holes,
                                                            const int* __restrict__ past_len, const int* __restrict__ q_len, const int* __restrict__ page_table,
-                                                           const float* __restrict__ scales, int max_pages, int num_pages, int page_shift, int stage_pages, int hkv,
-                                                           int window, int own) {
+                                                           const float* __restrict__ scales, int num_seqs, int max_pages, int num_pages, int page_shift, int stage_pages,
+                                                           int packed, int hkv, int window, int own) {
     pdl_prologue();
-    const int seq = blockIdx.z, lp = blockIdx.x, plane = blockIdx.y;
-    if (plane == 0 && threadIdx.x == 0) stage_table[seq * stage_pages + lp] = seq * stage_pages + lp;
+    const int at_page = blockIdx.x, plane = blockIdx.y, lane = threadIdx.x & 31;
+    T* dst = stage + ((size_t)at_page * 2 * hkv + plane) * 64 * D;
+    constexpr int B = D / 16;
+    int seq = at_page / stage_pages, lp = at_page - seq * stage_pages;
+    if (packed) {                                               // every warp finds the page's sequence for itself
+        int base = 0;
+        seq = -1;
+        for (int s0 = 0; s0 < num_seqs && seq < 0; s0 += 32) {
+            const int n = s0 + lane < num_seqs ? fp4_stage_own(past_len[s0 + lane] + q_len[s0 + lane], stage_pages) : 0;
+            int incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += v;
+            }
+            const unsigned here = __ballot_sync(0xffffffffu, at_page < base + incl);
+            if (here) {
+                const int l = __ffs(here) - 1;
+                seq = s0 + l;
+                lp = at_page - base - __shfl_sync(0xffffffffu, incl - n, l);
+            }
+            base += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (seq < 0) {                                          // behind all sequences
+            for (int i = threadIdx.x; i < 64 * D / 8; i += 256) reinterpret_cast<uint4*>(dst)[i] = make_uint4(0, 0, 0, 0);
+            return;
+        }
+        if (lp == 0 && plane == 0)
+            for (int i = fp4_stage_own(past_len[seq] + q_len[seq], stage_pages) + threadIdx.x; i < stage_pages; i += 256) {
+                stage_table[seq * stage_pages + i] = (int)gridDim.x - 1;
+                holes[seq * stage_pages + i] = 0;
+            }
+    }
+    if (plane == 0 && threadIdx.x == 0) stage_table[seq * stage_pages + lp] = at_page;
     const int past = past_len[seq], total = past + q_len[seq], count = own ? total : past;
     if (plane == 0 && threadIdx.x < 32) {
         const int slot = lp * 64 + 16 * threadIdx.x, at = slot >> page_shift;
@@ -333,12 +371,11 @@ __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __rest
         const unsigned gone = __ballot_sync(0xffffffffu, threadIdx.x < 4 && slot < total && (unsigned)page >= (unsigned)num_pages);
         if (threadIdx.x == 0) holes[seq * stage_pages + lp] = (uint8_t)gone;
     }
+    if (lp >= fp4_stage_own(total, stage_pages)) return;
     if (window > 0 && (lp + 1) * 64 + 2 * 128 <= past - window) return;        // before every tile that the windowed kernels touch
     const int first = window > 0 ? past + 1 - window : 0;
     const size_t slab = fp4_slab_bytes(1 << page_shift, D);
     const float scale = scales ? scales[plane >= hkv] : 1.f;
-    T* dst = stage + (((size_t)seq * stage_pages + lp) * 2 * hkv + plane) * 64 * D;
-    constexpr int B = D / 16;
 #pragma unroll
     for (int u = 0; u < 64 * B / 256; ++u) {
         const int i = u * 256 + threadIdx.x, r = i / B, b = i % B, slot = lp * 64 + r;
@@ -452,21 +489,22 @@ extern "C" int telb_rope_kv_write_fp4(const Fp4WriteParams* params, int d, int i
     return 0;
 }
 
-// pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [num_seqs * stage_pages, 2, Hkv, 64, d], page s * stage_pages + i for
-// rows 64 i.. of sequence s; holes [num_seqs, stage_pages] bytes: bit i is set where the rows 16 i .. 16 i + 15 of a page have no page of the pool.  own: the step's own
+// pool: one layer; stage_table [num_seqs, stage_pages] is filled in; stage: 16-bit [stage_total, 2, Hkv, 64, d], the sequences' pages of 64 rows packed (`packed`: stage_total
+// is one more than the sum of max(1, ceil(rows / 128)) * 2 over the sequences) or num_seqs * stage_pages of them; holes [num_seqs, stage_pages] bytes: bit i is set where the rows 16 i .. 16 i + 15 of a page have no page of the pool.  own: the step's own
 // rows too.  `scales` null: code * block scale, which both 16-bit types hold exactly.
 extern "C" int telb_kv_fp4_stage(const void* pool, void* stage, int* stage_table, uint8_t* holes, const int* past_len, const int* q_len, const int* page_table, const float* scales,
-                                 int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int hkv, int d, int window, int own, int is_bf16,
-                                 cudaStream_t stream) {
-    if (num_seqs <= 0 || stage_pages <= 0) return 0;
+                                 int num_seqs, int max_pages, int num_pages, int page_size, int stage_pages, int stage_total, int packed, int hkv, int d, int window,
+                                 int own, int is_bf16, cudaStream_t stream) {
+    if (num_seqs <= 0 || stage_pages <= 0 || stage_total <= 0) return 0;
+    if (!packed && (long long)num_seqs * stage_pages != stage_total) return fail("telb_kv_fp4_stage: pages of another number");
     if (d != 64 && d != 128 && d != 256) return fail("telb_kv_fp4_stage: head_dim must be 64, 128 or 256");
     if (page_size < 16 || page_size & (page_size - 1)) return fail("telb_kv_fp4_stage: the page size must be a power of two, at least 16");
-    if (num_seqs > 65535 || 2 * hkv > 65535) return fail("telb_kv_fp4_stage: more than 65535 sequences or planes");
+    if (2 * hkv > 65535) return fail("telb_kv_fp4_stage: more than 65535 planes");
     int shift = 0;
     while (1 << shift < page_size) ++shift;
-    const dim3 grid(stage_pages, 2 * hkv, num_seqs), blk(256);
+    const dim3 grid(stage_total, 2 * hkv), blk(256);
 #define STAGE_FP4(T, D) TELB_LAUNCH("kv_fp4_stage_kernel", (kv_fp4_stage_kernel<T, D>), grid, blk, 0, stream, (const uint8_t*)pool, (T*)stage, stage_table, holes, past_len, q_len, \
-                                    page_table, scales, max_pages, num_pages, shift, stage_pages, hkv, window, own)
+                                    page_table, scales, num_seqs, max_pages, num_pages, shift, stage_pages, packed, hkv, window, own)
     if (is_bf16) {
         if (d == 128) STAGE_FP4(__nv_bfloat16, 128);
         else if (d == 64) STAGE_FP4(__nv_bfloat16, 64);

@@ -417,7 +417,8 @@ def fp4_weighed(meta, group):
 
 def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
     """16-bit copies of the rows that the step's sequences have in a four-bit layer, for the prompt kernels: ``(stage, meta)`` with the pages
-    ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  The rows cached before the step, and its own with ``new_rows`` (else their
+    ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  They take ``4 Hkv D`` bytes a row of all sequences, rounded up to 128 rows each; of steps
+    whose lengths the host does not know (captured ones), ``max_seq_len`` rows of every sequence.  The rows cached before the step, and its own with ``new_rows`` (else their
     places are left for :func:`rope_kv_write_fp4` to fill); what lies behind in a page is zero, and so are rows without a page, which
     :func:`paged_attention` would take for keys (:func:`paged_attention_fp4` hides them).  ``window`` > 0: rows that no row
     of the step can see are zero, and pages of such rows may be left out."""

@@ -662,7 +662,7 @@ def _fp4_lib():
     L.telb_rope_kv_write_fp4.argtypes = [ctypes.c_char_p, i, i, p]
     L.telb_paged_attention_fp4.argtypes = [ctypes.c_char_p, i, i, i, p]
     L.telb_attention_fp4_ctas.argtypes = [i, i]
-    L.telb_kv_fp4_stage.argtypes = [p] * 8 + [i] * 10 + [p]
+    L.telb_kv_fp4_stage.argtypes = [p] * 8 + [i] * 12 + [p]
     L.telb_kv_evict.argtypes = [ctypes.c_char_p, p]
     L.telb_kv_fp4_commit_path.argtypes = [p] * 5 + [i] * 8 + [p]
     return L
@@ -735,12 +735,13 @@ def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: i
 def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int, new_rows: bool, pages: int, hkv: int, d: int):
     """Without ``scales``: codes times block scales, which both 16-bit types hold exactly.  A third result tells the prompt kernels which rows the cache
     does not have: a byte per page, a bit per 16 rows."""
-    n, per, dev = meta.num_seqs, 2 * max(1, (meta.max_seq_len + 127) // 128), kv_layer.get_device()     # whole 128-key tiles
-    stage = torch.empty(n * per, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
+    n, dev = meta.num_seqs, kv_layer.get_device()
+    per, total, packed = ref_ops.fp4_stage_pages(meta)
+    stage = torch.empty(total, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
     table, holes = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device), torch.empty(n, per, dtype=torch.uint8, device=kv_layer.device)
     _check(_fp4_lib().telb_kv_fp4_stage(
         *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, holes, meta.past_len, meta.q_len, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
-        meta.page_size, per, hkv, d, window or 0, int(new_rows), int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
+        meta.page_size, per, total, int(packed), hkv, d, window or 0, int(new_rows), int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
     return stage, dataclasses.replace(meta, page_table=table, page_size=64), holes
 
 

@@ -1441,18 +1441,33 @@ def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads, num_k
     return q
 
 
+def fp4_stage_pages(meta: StepMeta) -> Tuple[int, int, bool]:
+    """Size of the 16-bit copy of a step's sequences in pages of 64 rows: ``(columns of its table, pages, whether they are packed)``.  A sequence takes whole
+    128-key tiles: as many as the longest, or, where the host knows that some are shorter, its own, one sequence behind the other, and a page of zeros for
+    what the table has behind them."""
+    per = 2 * max(1, (meta.max_seq_len + 127) // 128)
+    if meta.host_lens is None:
+        return per, meta.num_seqs * per, False
+    total = sum([min(2 * max(1, (q + past + 127) // 128), per) for q, past in meta.host_lens])
+    return (per, total + 1, True) if total < meta.num_seqs * per else (per, total, False)
+
+
 def kv_fp4_stage(kv_layer, meta: StepMeta, scales, dtype, window=0, new_rows=False):
     d = fp4_head_dim(kv_layer)
-    n, per = meta.num_seqs, 2 * max(1, (meta.max_seq_len + 127) // 128)         # whole 128-key tiles
-    stage = torch.zeros(n * per, 2, kv_layer.shape[2], 64, d, dtype=dtype, device=kv_layer.device)
-    table = torch.arange(n * per, dtype=torch.int32, device=kv_layer.device).view(n, per)
+    n, (per, total, packed) = meta.num_seqs, fp4_stage_pages(meta)
+    stage = torch.zeros(total, 2, kv_layer.shape[2], 64, d, dtype=dtype, device=kv_layer.device)
+    table = torch.full((n, per), total - 1, dtype=torch.int32, device=kv_layer.device)
+    at = 0
     for s in range(n):
+        own = min(2 * max(1, (int(meta.past_len[s]) + int(meta.q_len[s]) + 127) // 128), per) if packed else per
+        table[s, :own] = torch.arange(at, at + own, dtype=torch.int32, device=kv_layer.device)
         rows = int(meta.past_len[s]) + (int(meta.q_len[s]) if new_rows else 0)
         v = _fp4_round(_fp4_rows(kv_layer, meta.page_table[s], rows, scales), dtype)
         if window > 0:
             v[:, :, :max(0, int(meta.past_len[s]) + 1 - window)] = 0.0
-        v = F.pad(v, (0, 0, 0, per * 64 - rows)).unflatten(2, (per, 64))
-        stage[s * per:(s + 1) * per] = v.permute(2, 0, 1, 3, 4)
+        v = F.pad(v, (0, 0, 0, own * 64 - rows)).unflatten(2, (own, 64))
+        stage[at:at + own] = v.permute(2, 0, 1, 3, 4)
+        at += own
     return stage, dataclasses.replace(meta, page_table=table, page_size=64)
 
 

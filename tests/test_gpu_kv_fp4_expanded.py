@@ -1,4 +1,6 @@
 """Steps that are too long to read four-bit pages in place, on the GPU: tables with holes, trees and windows against a 64-bit oracle."""
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -62,3 +64,34 @@ def test_rows_that_a_window_hides_do_not_reach_the_outputs(q_lens, past, hq, hkv
     stage, staged = ops.kv_fp4_stage(layer.cuda(), args[1], args[3], dtype, window, True)
     plain = ops.paged_attention(q.cuda(), stage, staged, d ** -0.5, window)
     assert plain.isfinite().all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_copies_are_as_long_as_the_rows(d):
+    """One long sequence beside short ones, 40 of them: the packed copy is the host's, the step's outputs are those of a step whose lengths the host does not
+    know, and the memory is that of the rows, not of forty long sequences."""
+    hkv, hq, page = 2, 8, 64
+    q_lens, past = [1] * 39 + [70], [(7 * i) % 130 for i in range(38)] + [5000, 0]
+    meta, layer, scales, g = make_step(q_lens, past, page, hkv, d, seed=d)
+    q = (torch.randn(sum(q_lens), hq, d, generator=g) * 2).bfloat16().cuda()
+    lg, m, sg = layer.cuda(), meta.to("cuda"), scales.cuda()
+    want, host = ops.kv_fp4_stage(layer, meta, scales, torch.bfloat16, new_rows=True)
+    got, staged = ops.kv_fp4_stage(lg, m, sg, torch.bfloat16, new_rows=True)
+    assert torch.equal(staged.page_table.cpu(), host.page_table) and torch.equal(got.cpu(), want)
+    assert got.shape[0] == sum(2 * max(1, -(-(a + b) // 128)) for a, b in zip(q_lens, past)) + 1
+    del got
+    loose = replace(m, host_lens=None, max_seq_len=6000)
+    expect = ops.paged_attention_fp4(q, lg, loose, d ** -0.5, sg)
+    ops.paged_attention_fp4(q, lg, m, d ** -0.5, sg)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = ops.paged_attention_fp4(q, lg, m, d ** -0.5, sg)
+    used = torch.cuda.max_memory_allocated() - before
+    assert used < 2 * (sum(q_lens) + sum(past) + 128 * 40) * 2 * hkv * d * 2 < 40 * 5001 * 2 * hkv * d * 2
+    # the same sums, cut into other parts: half a step of the result and of the probabilities on either side
+    top = 6 * 448 * float(scales[1])
+    assert ((out.double() - expect.double()).abs() <= 2 ** -7 * (out.double().abs() + 1.01 * top)).all()
+    ref, top, kq = oracle(q.cpu(), layer, meta, d ** -0.5, scales)
+    for o in (out, expect):
+        assert ((o.cpu().double() - ref).abs() <= bound(ref, top, kq, torch.bfloat16)).all()

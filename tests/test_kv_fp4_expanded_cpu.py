@@ -1,4 +1,6 @@
 """Steps that are too long to read four-bit pages in place, on the host: tables with holes, trees and windows against a 64-bit oracle."""
+from dataclasses import replace
+
 import pytest
 import torch
 
@@ -34,3 +36,19 @@ def test_rows_that_a_window_hides_do_not_reach_the_outputs():
         assert ((got.double() - want).abs() <= top * 2 ** -24 * (2 * 64 * kq + 600)).all()
         for new in (False, True):
             assert ops.kv_fp4_stage(layer, meta, scales, torch.bfloat16, window, new)[0].isfinite().all()
+
+
+def test_copies_are_as_long_as_the_rows():
+    q_lens, past = [1, 40, 0, 3, 128], [0, 300, 0, 126, 0]
+    meta, layer, scales, _ = make_step(q_lens, past, 32, 1, 64)
+    stage, staged = ops.kv_fp4_stage(layer, meta, scales, torch.float32, new_rows=True)
+    assert stage.shape[0] == 2 * (1 + 3 + 1 + 2 + 1) + 1 and staged.page_table.shape == (5, 6)
+    own = [int((row < stage.shape[0] - 1).sum()) for row in staged.page_table]
+    assert own == [2, 6, 2, 4, 2] and sorted(staged.page_table[staged.page_table < 16].tolist()) == list(range(16)) and not stage[-1].any()
+    whole, loose = ops.kv_fp4_stage(layer, replace(meta, host_lens=None, max_seq_len=500), scales, torch.float32, new_rows=True)
+    assert whole.shape[0] == 5 * 8 and torch.equal(loose.page_table.flatten(), torch.arange(40, dtype=torch.int32))
+    for s, (a, b) in enumerate(zip(q_lens, past)):
+        for i in range((a + b + 63) // 64):
+            assert torch.equal(stage[staged.page_table[s, i]], whole[loose.page_table[s, i]])
+    same = make_step([4, 4], [60, 60], 32, 1, 64)
+    assert ops.kv_fp4_stage(same[1], same[0], scales, torch.float32)[0].shape[0] == 4             # nobody shorter: no page of zeros
