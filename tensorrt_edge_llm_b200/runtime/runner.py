@@ -156,13 +156,30 @@ class ModelRunner:
                 return self._prefill(seats, prompts)
             # the prompts' last rows are a step of their own, whose attention weights say what of the prompts stays
             group = self.model.cfg.num_attention_heads // self.model.cfg.num_key_value_heads
-            last = max(1, min(self.BUDGET_VOTERS, ops.FP4_WEIGHT_COLUMNS // group))
+            last = max(1, min(self.BUDGET_VOTERS, ops.FP4_WEIGHT_COLUMNS // group, self.max_num_tokens))
             front = [(s, p[:-last]) for s, p in zip(seats, prompts) if len(p) > last]
             if front:
                 self._prefill([s for s, _ in front], [p for _, p in front])
-            logits = self.step(seats, [p[-last:] for p in prompts])
-            self.trim(seats)
-            return logits
+            logits = []
+            for some in self._voting_groups(seats, [min(last, len(p)) for p in prompts]):
+                logits.append(self.step([seats[i] for i in some], [prompts[i][-last:] for i in some]))
+            return torch.cat(logits)
+
+    VOTE_BYTES = 512 << 20
+
+    def _voting_groups(self, seats, voters: Sequence[int]) -> List[List[int]]:
+        """Prompts that vote in one step: at most ``max_num_tokens`` rows and, where there is more than one, ``VOTE_BYTES`` of scores a layer (4 bytes for a row, a
+        query head and a key of the longest of them)."""
+        size = 4 * self.model.cfg.num_attention_heads * max(voters)
+        groups, rows, keys = [], 0, 0
+        for i, (s, r) in enumerate(zip(seats, voters)):
+            total = self.kv.lengths[s] + r
+            if not groups or rows + r > self.max_num_tokens or size * (len(groups[-1]) + 1) * max(keys, total) > self.VOTE_BYTES:
+                groups.append([])
+                rows = keys = 0
+            groups[-1].append(i)
+            rows, keys = rows + r, max(keys, total)
+        return groups
 
     def _prefill(self, seats, prompts) -> torch.Tensor:
         n = len(seats)

@@ -1,0 +1,62 @@
+"""Sequences cut back to a budget of cached rows, within the limits of a deployment: rows a step, scratch, pages."""
+import pytest
+import torch
+
+from tensorrt_edge_llm_b200 import AutoModel
+from tensorrt_edge_llm_b200.config import tiny_llama_config
+from tensorrt_edge_llm_b200.runtime.kv_cache import KVCacheManager
+from tensorrt_edge_llm_b200.runtime.runner import ModelRunner
+
+
+def _cfg():
+    return tiny_llama_config(num_hidden_layers=2, vocab_size=256, dtype="float32", head_dim=64, num_attention_heads=4, num_key_value_heads=2, hidden_size=128,
+                             max_position_embeddings=512)
+
+
+def _prompts(*lens):
+    g = torch.Generator().manual_seed(6)
+    return [torch.randint(0, 256, (n,), generator=g).tolist() for n in lens]
+
+
+@pytest.mark.parametrize("most,vote_bytes", [(48, 512 << 20), (16, 512 << 20), (8192, 1), (80, 4 * 4 * 32 * 2 * 150)])
+def test_votes_keep_within_the_rows_of_a_step_and_their_scratch(most, vote_bytes):
+    """The prompts' last rows vote a few sequences at a time; what they vote for is the same."""
+    cfg, prompts = _cfg(), _prompts(150, 20, 33, 100, 70)
+    model = AutoModel.from_config(cfg, random_init=0)
+
+    def run(limit, bytes_):
+        kv = KVCacheManager(cfg, num_pages=80, page_size=16, max_seats=5, max_pages_per_seq=16, kv_dtype="nvfp4", keep_weights=True)
+        r = ModelRunner(model, kv, max_num_tokens=limit)
+        r.kv_budget, r.VOTE_BYTES = 400, bytes_
+        rows, scratch = [], []
+        step = r._meta
+
+        def spy(seats, q_lens, *a, **kw):
+            meta = step(seats, q_lens, *a, **kw)
+            rows.append(meta.num_tokens)
+            return meta
+
+        r._meta = spy
+        model_step = r.step
+
+        def spy_step(seats, toks, **kw):
+            if kw.get("votes", True):
+                scratch.append((len(seats), 4 * 4 * max(map(len, toks)) * len(seats) * max(kv.lengths[s] + len(t) for s, t in zip(seats, toks))))
+            return model_step(seats, toks, **kw)
+
+        r.step = spy_step
+        return r.prefill(list(range(5)), prompts), rows, scratch, kv
+
+    want, _, one, kv_a = run(8192, 512 << 20)
+    got, rows, scratch, kv_b = run(most, vote_bytes)
+    assert len(one) == 1 and len(scratch) > 1
+    assert max(rows) <= most and all(n == 1 or b <= vote_bytes for n, b in scratch)
+    assert torch.allclose(got, want, rtol=1e-3, atol=1e-3 * float(want.abs().max()))
+    for s, p in enumerate(prompts):
+        assert kv_b.lengths[s] == len(p)
+        slot = torch.arange(len(p))
+        a, b = (k.weights[:, k.table[s].long()[slot // 16], :, slot % 16] for k in (kv_a, kv_b))
+        if most >= 32:              # as many voters: one a row and query head
+            assert torch.allclose(a, b, atol=1e-2) and abs(float(b.sum()) - min(32, len(p)) * 4 * 2) < 1e-1
+        else:
+            assert abs(float(b.sum()) - most * 4 * 2) < 1e-1
