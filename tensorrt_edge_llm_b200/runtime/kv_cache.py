@@ -131,6 +131,7 @@ class KVCacheManager:
             self.recurrent = RecurrentState(cfg, max_seats, device, cfg.compute_dtype if self.kv_fp8 or self.kv_fp4 else self.dtype)
         self.weights: Optional[torch.Tensor] = None
         self._spare = max_seats                  # the seat that holds a shortened sequence's new pages until it changes over
+        self._held = 0                           # rows that it holds pages for all the time
         if keep_weights:
             if not self.kv_fp4 or self.recurrent is not None or self.window or cfg.layer_windows:
                 raise ValueError("attention weights are kept for four-bit pages of stacks whose layers all attend without a window")
@@ -247,6 +248,13 @@ class KVCacheManager:
         self.table[seat, :upto] = -1
         self.table_version += 1
 
+    def hold_spare(self, rows: int) -> None:
+        """Keep pages for ``rows`` aside, so that :meth:`shorten` to so many never finds the pool empty."""
+        if self.weights is None:
+            raise ValueError("rows are dropped by attention weight: keep_weights")
+        self._held = rows
+        self.reserve(self._spare, rows)
+
     @torch.no_grad()
     def shorten(self, seat: int, keep: int, first: int, recent: int) -> int:
         """Keep ``keep`` rows of ``seat`` in every layer and KV head (:func:`ops.kv_evict`), in new pages; returns how many tokens went.  The pages
@@ -257,18 +265,20 @@ class KVCacheManager:
             raise ValueError("rows are dropped by attention weight: keep_weights")
         if length <= keep:
             return 0
-        spare, dev = self._spare, self.pool.device
+        spare, dev, need = self._spare, self.pool.device, (keep + self.page_size - 1) // self.page_size
         self.reserve(spare, keep)
         try:
-            old, to = self.table_rows([seat]).to(dev), self.table_rows([spare])[:, :(keep + self.page_size - 1) // self.page_size].contiguous().to(dev)
+            old, to = self.table_rows([seat]).to(dev), self.table_rows([spare])[:, :need].contiguous().to(dev)
             n = torch.tensor([length], dtype=torch.int32).to(dev)
             for layer in range(self.num_layers):
                 ops.kv_evict(self.pool[layer], self.weights[layer], old, n, to, keep, first, recent)
-            pages = self.pages_of(spare)
+            pages = self.pages_of(spare)[:need]
             self.free(seat)
             self.adopt_prefix(seat, pages, keep)
         finally:
             self.free(spare)
+            if self._held:                # of the pages that the sequence has just given back
+                self.reserve(spare, self._held)
         return length - keep
 
     def live_pages(self, seat: int) -> int:

@@ -89,12 +89,17 @@ class LLM:
                 raise ValueError(f"kv_budget of at least {4 * ModelRunner.BUDGET_FIRST} rows")
             if kv_budget + ModelRunner.BUDGET_SLACK >= max_kv_cache_capacity:
                 raise ValueError(f"kv_budget {kv_budget} and {ModelRunner.BUDGET_SLACK + 1} more rows must be within max_kv_cache_capacity {max_kv_cache_capacity}")
-            total_pages = kv_pages or total_pages + kv_budget // page_size + 1          # a sequence holds its new pages beside the old while it is cut back
+            spare = -(-kv_budget // page_size)          # a sequence holds its new pages beside the old while it is cut back
+            total_pages = kv_pages or total_pages + spare
+            if total_pages < spare + -(-(kv_budget + ModelRunner.BUDGET_SLACK + 1) // page_size):
+                raise ValueError(f"kv_pages {kv_pages} hold no sequence of {kv_budget + ModelRunner.BUDGET_SLACK + 1} rows beside the {spare} pages of a cut")
         # "fp8": E4M3 KV pages (`--kv-cache-quantization fp8` checkpoints select it through their quantisation config)
         self.kv = KVCacheManager(self.cfg, total_pages, page_size, max_seats=max_batch_size,
                                  max_pages_per_seq=pages_per_seq, device=self.device, kv_dtype=kv_cache_dtype, keep_weights=kv_budget > 0)
         self.runner = ModelRunner(self.model, self.kv, self.device, max_num_tokens=max_num_tokens)
         self.runner.kv_budget = int(kv_budget)
+        if kv_budget:
+            self.kv.hold_spare(kv_budget)
         self.runner.vocab_map = self._vocab_map
         self.lora = None
         self.runner.lora = None
@@ -474,7 +479,7 @@ class LLM:
         for s in seats:
             self.kv.free(s)
         for s, p in zip(seats, ids):
-            self.kv.reserve(s, len(p) + (0 if self.runner.kv_budget else sp.max_tokens))
+            self.kv.reserve(s, self.runner.rows_to_reserve(len(p), sp.max_tokens))
         states = [lp.make_row_state(self.guided_vocab, guided=sp.guided, logit_bias=sp.logit_bias, num_logprobs=sp.logprobs,
                                     vocab_size=self.cfg.vocab_size) for _ in range(n)]
         eos = self.cfg.eos_token_id
@@ -551,7 +556,7 @@ class LLM:
         for s, p in zip(seats, ids):
             if len(p) > self.max_input_len:
                 raise ValueError(f"prompt of {len(p)} tokens exceeds max_input_len {self.max_input_len}")
-            self.kv.reserve(s, len(p) + (0 if self.runner.kv_budget else sp.max_tokens))
+            self.kv.reserve(s, self.runner.rows_to_reserve(len(p), sp.max_tokens))
         t0 = time.perf_counter()
         if isinstance(ids, torch.Tensor):
             logits = self.runner.prefill_tensor(seats, ids)      # pinned host tensor → one H2D copy per chunk

@@ -102,6 +102,11 @@ class ModelRunner:
         if self.kv_budget:
             raise ValueError(f"kv_budget is not built for {what}")
 
+    def rows_to_reserve(self, prompt: int, new: int) -> int:
+        """Rows that a sequence of ``prompt`` tokens holds at most while ``new`` more are generated.  Under a budget: the prompt, or what it grows to between
+        two cuts; each cut gives back what the next growth takes."""
+        return max(prompt, min(prompt + new, self.kv_budget + self.BUDGET_SLACK + 1)) if self.kv_budget else prompt + new
+
     def trim(self, seats: Sequence[int], slack: int = BUDGET_SLACK) -> None:
         """Cut sequences that have outgrown the budget back to it."""
         if not self.kv_budget:

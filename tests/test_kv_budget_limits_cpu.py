@@ -5,7 +5,8 @@ import torch
 from tensorrt_edge_llm_b200 import AutoModel
 from tensorrt_edge_llm_b200.config import tiny_llama_config
 from tensorrt_edge_llm_b200.runtime.kv_cache import KVCacheManager
-from tensorrt_edge_llm_b200.runtime.runner import ModelRunner
+from tensorrt_edge_llm_b200.runtime.llm import LLM
+from tensorrt_edge_llm_b200.runtime.runner import ModelRunner, SamplingParams
 
 
 def _cfg():
@@ -60,3 +61,29 @@ def test_votes_keep_within_the_rows_of_a_step_and_their_scratch(most, vote_bytes
             assert torch.allclose(a, b, atol=1e-2) and abs(float(b.sum()) - min(32, len(p)) * 4 * 2) < 1e-1
         else:
             assert abs(float(b.sum()) - most * 4 * 2) < 1e-1
+
+
+def test_a_generation_that_starts_has_the_pages_to_end():
+    """Pages for a cut and for what a sequence grows to are there before the first step, or the call is refused before it."""
+    prompts = _prompts(100, 30)
+    kw = dict(device="cpu", max_batch_size=2, max_input_len=256, max_kv_cache_capacity=336, page_size=16, kv_cache_dtype="nvfp4", random_init_seed=0, kv_budget=48)
+    sp = SamplingParams(max_tokens=150, ignore_eos=True)
+    want = [o.token_ids for o in LLM(_cfg(), **kw).generate(prompts, sp)]
+    enough = 2 * 8 + 3                       # 113 rows of either sequence, 48 of a cut
+    llm = LLM(_cfg(), kv_pages=enough, **kw)
+    for _ in range(2):
+        assert [o.token_ids for o in llm.generate(prompts, sp)] == want
+    logits = LLM(_cfg(), kv_pages=enough, **kw).generate(prompts, SamplingParams(max_tokens=150, temperature=0.7, seed=1, ignore_eos=True))
+    assert [len(o.token_ids) for o in logits] == [150, 150]
+    short = LLM(_cfg(), kv_pages=enough - 1, **kw)
+    steps = []
+    short.runner.step = lambda *a, **k: steps.append(1)
+    with pytest.raises(Exception, match="page|pool|exhaust"):
+        short.generate(prompts, sp)
+    assert not steps
+    with pytest.raises(ValueError):
+        LLM(_cfg(), kv_pages=10, **kw)
+    LLM(_cfg(), kv_pages=11, **kw).generate([prompts[1]], sp)
+    kv = KVCacheManager(_cfg(), num_pages=4, max_seats=1, max_pages_per_seq=2, kv_dtype="nvfp4")
+    with pytest.raises(ValueError):
+        kv.hold_spare(16)
