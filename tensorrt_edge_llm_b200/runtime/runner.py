@@ -121,11 +121,14 @@ class ModelRunner:
 
     @torch.no_grad()
     def step(self, seats: Sequence[int], token_lists: Sequence[Sequence[int]], logits_all=False,
-             commit=True, tree_mask=None, positions=None, logits_rows=None, votes=True) -> torch.Tensor:
+             commit=True, tree_mask=None, positions=None, logits_rows=None, votes=True, prompt=False) -> torch.Tensor:
         """Run one ragged step; returns logits ``[L, V]`` (last row of each sequence unless
         ``logits_all`` or an explicit list of packed rows, ``logits_rows``).  KV lengths advance by the rows fed when ``commit``.
-        Under a KV budget the rows' attention weights count toward what stays, unless not ``votes``."""
+        Under a KV budget the rows' attention weights count toward what stays, unless not ``votes``; sequences that several tokens at once would take beyond
+        what they may grow to are cut back first, unless the rows end a ``prompt``, all of which has to be there for them."""
         q_lens = [len(t) for t in token_lists]
+        if self.kv_budget and votes and not prompt:
+            self.trim([s for s, q in zip(seats, q_lens) if self.kv.lengths[s] + q > self.kv_budget + self.BUDGET_SLACK + 1], 0)
         for s in seats:
             if self.kv.lengths[s] == 0:
                 self.rope_delta.pop(s, None)          # a fresh sequence on this seat
@@ -167,7 +170,7 @@ class ModelRunner:
                 self._prefill([s for s, _ in front], [p for _, p in front])
             logits = []
             for some in self._voting_groups(seats, [min(last, len(p)) for p in prompts]):
-                logits.append(self.step([seats[i] for i in some], [prompts[i][-last:] for i in some]))
+                logits.append(self.step([seats[i] for i in some], [prompts[i][-last:] for i in some], prompt=True))
             return torch.cat(logits)
 
     VOTE_BYTES = 512 << 20

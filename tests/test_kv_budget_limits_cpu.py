@@ -87,3 +87,15 @@ def test_a_generation_that_starts_has_the_pages_to_end():
     kv = KVCacheManager(_cfg(), num_pages=4, max_seats=1, max_pages_per_seq=2, kv_dtype="nvfp4")
     with pytest.raises(ValueError):
         kv.hold_spare(16)
+
+
+def test_several_tokens_at_once_stay_within_what_a_sequence_may_grow_to():
+    """Grammar-forced tokens ride along with a sampled one."""
+    llm = LLM(_cfg(), device="cpu", max_batch_size=1, max_input_len=64, max_kv_cache_capacity=128, page_size=16, kv_cache_dtype="nvfp4", random_init_seed=0, kv_budget=63)
+    r = llm.runner
+    r.prefill([0], _prompts(60))
+    r.decode_greedy([0], torch.tensor([3], dtype=torch.int32), 66)
+    total = r.kv.lengths[0] + r.dropped.get(0, 0)
+    assert r.kv.lengths[0] > 120                    # nine more rows would not fit its 128
+    r.step([0], [[5, 6, 7, 8, 9, 10, 11, 12, 13]])
+    assert r.kv.lengths[0] == 63 + 9 and r.kv.lengths[0] + r.dropped[0] == total + 9
