@@ -914,25 +914,40 @@ int launch_attention_fp4_nt(const Fp4AttnParams& p, int columns, cudaStream_t st
     constexpr int C = 8 * NT;
     constexpr int kSmem = kFp4Warps * Fp4Ring<D>::kStages * Fp4Ring<D>::kBytes;
     static_assert(kSmem >= kFp4Warps * C * (D + 2) * 4 + C * 24, "the warps' results fit where their rings were");
-    static bool configured[64] = {};
+    static int most_ranks[64] = {};                                              // clusters of 16 where the device places them
     int dev = 0;
     cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64 || !configured[dev]) {
+    if (dev < 0 || dev >= 64) return fail("telb_paged_attention_fp4: device index above 63");
+    if (!most_ranks[dev]) {
         cudaError_t e = cudaFuncSetAttribute(attention_fp4_kernel<T, D, NT, kVotes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT, kVotes>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
         if (e == cudaSuccess) e = cudaFuncSetAttribute(attention_fp4_cluster_kernel<T, D, NT, kVotes>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attention_fp4)", e);
-        if (dev >= 0 && dev < 64) configured[dev] = true;
+        cudaLaunchConfig_t c{};
+        c.gridDim = dim3(16);
+        c.blockDim = dim3(kFp4Warps * 32);
+        c.dynamicSmemBytes = kSmem;
+        cudaLaunchAttribute a;
+        a.id = cudaLaunchAttributeClusterDimension;
+        a.val.clusterDim.x = 16;
+        a.val.clusterDim.y = a.val.clusterDim.z = 1;
+        c.attrs = &a;
+        c.numAttrs = 1;
+        int clusters = 0;
+        const bool placed = cudaOccupancyMaxActiveClusters(&clusters, attention_fp4_cluster_kernel<T, D, NT, kVotes>, &c) == cudaSuccess && clusters > 0;
+        cudaGetLastError();
+        most_ranks[dev] = placed ? 16 : 8;
     }
     if (p.ranks > 0) {
+        const int ranks = min(p.ranks, most_ranks[dev]);
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(p.ranks, p.max_items, p.num_seqs);
+        cfg.gridDim = dim3(ranks, p.max_items, p.num_seqs);
         cfg.blockDim = dim3(kFp4Warps * 32);
         cfg.dynamicSmemBytes = kSmem;
         cfg.stream = stream;
         cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = p.ranks;
+        attr[0].val.clusterDim.x = ranks;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -968,7 +983,7 @@ extern "C" int telb_attention_fp4_ctas(int cols, int d) {
     return sm_count() * (d * nt <= 128 ? 4 : d * nt <= 256 && d < 256 ? 3 : 2);
 }
 
-// ranks > 0: clusters of so many CTAs per item (sequence, KV head, C columns); 0: the line of all items' tiles cut into `ctas` parts, with
+// ranks > 0: clusters of so many CTAs per item (sequence, KV head, C columns; 8 in place of 16 where the device places none of 16); 0: the line of all items' tiles cut into `ctas` parts, with
 // part_o [2 ctas, C, d], part_ml [2 ctas, C, 2] and spans [num_seqs, max_items] (C = cols: 8, or 16 of at most 128 features; max_items = KV heads x chunks of the longest
 // sequence's columns): scratch.  `weights` null: outputs only; else `stat` [tokens, hq, 2]
 // and `scores` [num_seqs, hkv, columns / 8, tiles, 2, 8, pairs] float4 are scratch: `tiles` of 32 keys hold every sequence's, `pairs` columns of 8 (at most 4).

@@ -755,19 +755,24 @@ def _fp4_commit_path(pool, page_table, past_len, path, path_len) -> None:
                                               row * 16 // 9, _raw_stream(dev)), "kv_commit_path")
 
 
-def _fp4_ranks(items: int, tiles: int, most: int = 256) -> int:
+@functools.lru_cache(maxsize=None)
+def _sms(dev: int) -> int:
+    return torch.cuda.get_device_properties(dev).multi_processor_count
+
+
+def _fp4_ranks(items: int, tiles: int, most: int = 256, sms: int = 148) -> int:
     """CTAs of a cluster per item (sequence, KV head, 8 or 16 columns) of ``tiles`` 32-key tiles, or 0 for the form that cuts the line of all items'
     tiles.  Clusters until ``most`` CTAs are there, each warp with a tile at least: 8 sequences of 1000 keys, 8 heads: 2, 4, 8 CTAs 13, 10.9, 11.6 us;
     16 of 8192: 1, 2, 4: 56, 43, 42; 30 of up to 4000: 1, 2, 4: 40, 38, 39; 64 of 1100: 1, 2: 26, 32.  16 CTAs where all of them have an SM (one
     sequence of 8 heads: 2000 keys 8.9 and 9.6 us with 8 and 16, 8000: 13.7 and 13.0).  The line once a warp of such a cluster has many tiles: its
     merge costs 5 us (one sequence, clusters of 16 and the line: 4 heads, 16000 keys 14.3 and 18.4, 60000: 31 and 24; 1 head, 8000 keys: 10.9 and 11.6, 30000:
     19 and 14)."""
-    if items * 16 <= 148 and tiles > 64 * (4 + 2 * items):
+    if items * 16 <= sms and tiles > 64 * (4 + 2 * items):
         return 0
     ranks = 1
     while ranks < 8 and items * ranks < most and ranks * 4 <= tiles:
         ranks *= 2
-    return 16 if ranks == 8 and items * 16 <= 148 and tiles >= 128 else ranks
+    return 16 if ranks == 8 and items * 16 <= sms and tiles >= 128 else ranks
 
 
 @_on_device
@@ -817,7 +822,7 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
     ranks = 0
     if ctas is None:
         # keeping account of the weights, a CTA of 8 columns waits more: 16 sequences of 8192 keys, 8 heads: 2, 4, 8 CTAs 61, 55, 59 us
-        ranks = _fp4_ranks(n * items, tiles, 512 if weights is not None and cols == 8 else 256)
+        ranks = _fp4_ranks(n * items, tiles, 512 if weights is not None and cols == 8 else 256, _sms(dev))
         ctas = 0 if ranks else max(1, min(L.telb_attention_fp4_ctas(cols, d), n * items * tiles // 4))
     elif ctas < 0:
         ranks, ctas = -ctas, 0

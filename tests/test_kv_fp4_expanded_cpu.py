@@ -52,3 +52,10 @@ def test_copies_are_as_long_as_the_rows():
             assert torch.equal(stage[staged.page_table[s, i]], whole[loose.page_table[s, i]])
     same = make_step([4, 4], [60, 60], 32, 1, 64)
     assert ops.kv_fp4_stage(same[1], same[0], scales, torch.float32)[0].shape[0] == 4             # nobody shorter: no page of zeros
+
+
+def test_clusters_follow_the_multiprocessors_of_the_device():
+    ranks = ops.cuda_ops()._fp4_ranks
+    assert ranks(8, 200) == 16 and ranks(9, 200) == 16 and ranks(10, 200) == 8
+    assert ranks(8, 200, sms=120) == 8 and ranks(12, 200, sms=192) == 16        # 16 CTAs an item where each has a multiprocessor
+    assert ranks(4, 4000) == 0 and ranks(9, 4000, sms=100) == 8                 # the line's merge pays for few items only
