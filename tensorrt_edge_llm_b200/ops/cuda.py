@@ -686,6 +686,21 @@ def _fp4_geometry(kv_layer: torch.Tensor, meta: StepMeta, scales: torch.Tensor) 
     return shape[0], shape[2], d
 
 
+def _fp4_step(meta: StepMeta, sequences: tuple, rows: tuple = ()) -> tuple:
+    """``(page table, its columns)``, the table contiguous, after checks of what the kernels index by sequence and by row."""
+    table, n, i32 = meta.page_table, meta.num_seqs, torch.int32
+    shape = table.shape
+    if len(shape) != 2 or shape[0] < n or table.dtype is not i32:
+        raise ValueError(f"a page table is int32 [sequences, pages], not {table.dtype} {tuple(shape)} for {n} sequences")
+    for v in sequences:
+        if v.dtype is not i32 or v.numel() < n or not v.is_contiguous():
+            raise ValueError(f"lengths and first rows are contiguous int32 of {n} sequences, not {v.dtype} {tuple(v.shape)}")
+    for v in rows:
+        if v is not None and (v.dtype is not i32 or v.numel() < meta.num_tokens or not v.is_contiguous()):
+            raise ValueError(f"positions, slots and sequences are contiguous int32 of {meta.num_tokens} rows, not {v.dtype} {tuple(v.shape)}")
+    return table if table.is_contiguous() else table.contiguous(), shape[1]
+
+
 @_on_device
 def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads: int, num_kv_heads: int, head_dim: int, scales, q_norm_w=None, k_norm_w=None,
                       eps: float = 1e-6, stage=None, stage_table=None) -> torch.Tensor:
@@ -713,12 +728,13 @@ def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads: int, 
         if stage_table.dtype != torch.int32 or not stage_table.is_contiguous() or stage_table.dim() != 2 or stage_table.shape[0] != meta.num_seqs:
             raise ValueError("rope_kv_write_fp4: the 16-bit pages' table is int32 [sequences, pages]")
         staged = (stage.shape[3], stage_table.shape[1], stage.shape[0])
+    page_table, width = _fp4_step(meta, (meta.q_start, meta.past_len), (positions, meta.seq_ids, meta.kv_offsets))
     qkv = _aligned(qkv)
     q = qkv.new_empty((t, num_q_heads, d))
     dev = qkv.get_device()
-    p = _FP4_WRITE.pack(*_ptrs("rope_kv_write_fp4", dev, (qkv, q, kv_layer, cos_sin, positions, meta.seq_ids, meta.q_start, meta.past_len, meta.page_table,
+    p = _FP4_WRITE.pack(*_ptrs("rope_kv_write_fp4", dev, (qkv, q, kv_layer, cos_sin, positions, meta.seq_ids, meta.q_start, meta.past_len, page_table,
                                                           meta.kv_offsets, q_norm_w, k_norm_w, scales, stage, stage_table)),
-                        t, num_q_heads, hkv, rot, max_pos, meta.page_size, meta.page_table.shape[1], pages, *staged, eps)
+                        t, num_q_heads, hkv, rot, max_pos, meta.page_size, width, pages, *staged, eps)
     _check(_fp4_lib().telb_rope_kv_write_fp4(p, d, is_bf16, _raw_stream(dev)), "rope_kv_write_fp4")
     return q
 
@@ -737,10 +753,11 @@ def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int
     does not have: a byte per page, a bit per 16 rows."""
     n, dev = meta.num_seqs, kv_layer.get_device()
     per, total, packed = ref_ops.fp4_stage_pages(meta)
+    page_table, width = _fp4_step(meta, (meta.q_len, meta.past_len))
     stage = torch.empty(total, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
     table, holes = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device), torch.empty(n, per, dtype=torch.uint8, device=kv_layer.device)
     _check(_fp4_lib().telb_kv_fp4_stage(
-        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, holes, meta.past_len, meta.q_len, meta.page_table, scales)), n, meta.page_table.shape[1], pages,
+        *_ptrs("kv_fp4_stage", dev, (kv_layer, stage, table, holes, meta.past_len, meta.q_len, page_table, scales)), n, width, pages,
         meta.page_size, per, total, int(packed), hkv, d, window or 0, int(new_rows), int(dtype == torch.bfloat16), _raw_stream(dev)), "kv_fp4_stage")
     return stage, dataclasses.replace(meta, page_table=table, page_size=64), holes
 
@@ -810,6 +827,7 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
         # the two global scales multiply scores and outputs, in 32 bits
         stage, staged, holes = _fp4_stage(kv_layer, meta, None, q.dtype, window, True, pages, hkv, d)
         return paged_attention(q, stage, staged, scale, sliding_window, sinks, kv_scales=scales, kv_holes=holes)
+    page_table, width = _fp4_step(meta, (meta.q_start, meta.q_len, meta.past_len))
     q = _aligned(q)
     out = torch.empty_like(q)
     dev, n, L = q.get_device(), meta.num_seqs, _fp4_lib()
@@ -837,8 +855,8 @@ def paged_attention_fp4(q, kv_layer, meta: StepMeta, scale: float, scales, slidi
         part_ml = part_o + 4 * room[1]
         spans = part_ml + 4 * room[2]
         stat = spans + 4 * room[3] if pairs else 0
-    ptr = _ptrs("paged_attention_fp4", dev, (q, kv_layer, out, meta.q_start, meta.q_len, meta.past_len, meta.page_table, scales, sinks, weights))
-    p = _FP4_ATTN.pack(*ptr[:3], part_o, part_ml, stat, *ptr[3:], spans, scores, n, t, meta.max_q_len, pages, meta.page_table.shape[1], meta.page_size,
+    ptr = _ptrs("paged_attention_fp4", dev, (q, kv_layer, out, meta.q_start, meta.q_len, meta.past_len, page_table, scales, sinks, weights))
+    p = _FP4_ATTN.pack(*ptr[:3], part_o, part_ml, stat, *ptr[3:], spans, scores, n, t, meta.max_q_len, pages, width, meta.page_size,
                        meta.page_size.bit_length() - 1, hq, hkv, window, ctas, ranks, items, tiles, pairs, scale, decay)
     _check(L.telb_paged_attention_fp4(p, cols, d, is_bf16, _raw_stream(dev)), "paged_attention_fp4", (1 if ranks else 2) + (weights is not None and not (ranks and items == hkv)))
     return out

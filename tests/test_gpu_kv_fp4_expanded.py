@@ -95,3 +95,39 @@ def test_copies_are_as_long_as_the_rows(d):
     ref, top, kq = oracle(q.cpu(), layer, meta, d ** -0.5, scales)
     for o in (out, expect):
         assert ((o.cpu().double() - ref).abs() <= bound(ref, top, kq, torch.bfloat16)).all()
+
+
+def test_a_strided_page_table_names_the_same_pages():
+    """Columns of a wider table on the device, as a program that keeps one table for all its seats hands them over."""
+    for q_lens, past in (([1, 1], [100, 300]), ([40, 9], [130, 70])):
+        meta, layer, scales, g = make_step(q_lens, past, 16, 2, 64, seed=5)
+        m, lg, sg = meta.to("cuda"), layer.cuda(), scales.cuda()
+        t = sum(q_lens)
+        wide = torch.randint(0, layer.shape[0], (2, m.page_table.shape[1] + 7), generator=g).int().cuda()
+        wide[:, 3:-4] = m.page_table
+        strided = replace(m, page_table=wide[:, 3:-4])
+        qkv, cs = torch.randn(t, 8 * 64, generator=g).bfloat16().cuda(), torch.randn(512, 64, generator=g).cuda()
+        a, b = lg.clone(), lg.clone()
+        qa, qb = (ops.rope_kv_write_fp4(qkv, x, step, cs, 4, 2, 64, sg) for x, step in ((a, m), (b, strided)))
+        assert torch.equal(a, b) and torch.equal(qa, qb)
+        assert torch.equal(ops.paged_attention_fp4(qa, a, m, 0.125, sg), ops.paged_attention_fp4(qa, a, strided, 0.125, sg))
+        assert torch.equal(ops.kv_fp4_stage(a, m, sg, torch.bfloat16, 0, True)[0], ops.kv_fp4_stage(a, strided, sg, torch.bfloat16, 0, True)[0])
+
+
+def test_steps_of_other_types_and_sizes_are_refused():
+    meta, layer, scales, g = make_step([40, 9], [130, 70], 16, 2, 64, seed=5)
+    m, lg, sg = meta.to("cuda"), layer.cuda(), scales.cuda()
+    q, qkv, cs = torch.randn(49, 4, 64).half().cuda(), torch.randn(49, 8 * 64).half().cuda(), torch.ones(512, 64).cuda()
+    one, pair = m.q_len[:1], torch.stack([m.past_len, m.past_len], 1)[:, 0]
+    for bad in (dict(page_table=m.page_table.long()), dict(page_table=m.page_table[:1]), dict(past_len=m.past_len.long()), dict(past_len=m.past_len[:1]), dict(past_len=pair)):
+        step = replace(m, **bad)
+        for call in (lambda: ops.paged_attention_fp4(q, lg, step, 0.1, sg), lambda: ops.cuda_ops().paged_attention_fp4(q, lg, step, 0.1, sg, direct=True),
+                     lambda: ops.rope_kv_write_fp4(qkv, lg, step, cs, 4, 2, 64, sg), lambda: ops.kv_fp4_stage(lg, step, sg, torch.float16)):
+            with pytest.raises(ValueError):
+                call()
+    for bad in (dict(q_len=one), dict(q_len=m.q_len.long())):
+        with pytest.raises(ValueError):
+            ops.paged_attention_fp4(q, lg, replace(m, **bad), 0.1, sg)
+    for bad in (dict(positions=m.positions[:5]), dict(seq_ids=m.seq_ids.long()), dict(positions=m.positions.float()), dict(kv_offsets=m.positions[:5])):
+        with pytest.raises(ValueError):
+            ops.rope_kv_write_fp4(qkv, lg, replace(m, **bad), cs, 4, 2, 64, sg)
