@@ -2151,7 +2151,7 @@ def candidate_rescore(hidden, lm_head, cand):
 
 def kv_commit_path(pool, page_table, past_len, path, path_len) -> None:
     assert pool.is_contiguous() and pool.element_size() in (1, 2)
-    if pool.dtype == torch.uint8:
+    if ref_ops.is_fp4_pages(pool):
         return _fp4_commit_path(pool, page_table, past_len, path, path_len)
     if pool.element_size() == 1:            # FP8 pages: a row of D bytes moves as D / 2 16-bit elements
         pool = pool.view(torch.int16)

@@ -1036,7 +1036,7 @@ def kv_commit_path(pool: torch.Tensor, page_table: torch.Tensor, past_len: torch
                    path_len: torch.Tensor) -> None:
     """Compact the accepted path in the paged cache ``pool [L, pages, 2, Hkv, P, D]``: the entry at
     slot ``past + path[j]`` moves to slot ``past + j`` (``j ≥ 1``), in place."""
-    if pool.dtype == torch.uint8:               # four-bit pages: a row's codes and its block scales lie apart
+    if is_fp4_pages(pool):                      # a row's codes and its block scales lie apart
         for layer in pool:
             for part in fp4_page_parts(layer):
                 kv_commit_path(part[None].view(torch.int8), page_table, past_len, path, path_len)
@@ -1365,6 +1365,12 @@ def fp4_head_dim(kv_layer: torch.Tensor) -> int:
     if p < 16 or p & (p - 1):
         raise ValueError(f"four-bit pages hold a power of two of rows, at least 16, not {p}")
     return shape[4] * 16 // 9
+
+
+def is_fp4_pages(layer: torch.Tensor) -> bool:
+    """Whether a layer (or a stack of them) of bytes has the shape of four-bit pages, as against rows of one byte a feature."""
+    p = layer.shape[-2]
+    return layer.dtype == torch.uint8 and layer.shape[-1] in (36, 72, 144) and p >= 16 and p & (p - 1) == 0
 
 
 def fp4_page_parts(kv_layer: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

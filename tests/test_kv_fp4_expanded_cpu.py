@@ -59,3 +59,15 @@ def test_clusters_follow_the_multiprocessors_of_the_device():
     assert ranks(8, 200) == 16 and ranks(9, 200) == 16 and ranks(10, 200) == 8
     assert ranks(8, 200, sms=120) == 8 and ranks(12, 200, sms=192) == 16        # 16 CTAs an item where each has a multiprocessor
     assert ranks(4, 4000) == 0 and ranks(9, 4000, sms=100) == 8                 # the line's merge pays for few items only
+
+
+def test_commit_path_still_moves_rows_of_bytes():
+    """Pages of one byte a feature, held as plain bytes, move as they did before there were four-bit pages."""
+    g = torch.Generator().manual_seed(2)
+    pool = torch.randint(0, 256, (2, 6, 2, 3, 16, 64), generator=g, dtype=torch.uint8)
+    table, past = torch.tensor([[4, 1, 0], [2, 5, -1]], dtype=torch.int32), torch.tensor([14, 3])
+    path, plen = torch.tensor([[0, 2, 5, 6], [0, 1, 4, 0]]), torch.tensor([4, 3])
+    want = pool.view(torch.int8).clone()
+    ops.kv_commit_path(want, table, past, path, plen)
+    ops.kv_commit_path(pool, table, past, path, plen)
+    assert torch.equal(pool, want.view(torch.uint8)) and not ops.ref.is_fp4_pages(pool)
