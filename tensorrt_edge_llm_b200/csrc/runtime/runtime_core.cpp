@@ -318,7 +318,11 @@ int LLMEngineConfig::num_attention_layers() const {
 static int element_bytes(const std::string& dtype) { return dtype == "float32" ? 4 : ((dtype == "fp8" || dtype == "FP8") ? 1 : 2); }
 
 long long LLMEngineConfig::kv_bytes_per_token() const {
-    const int eb = (kv_cache_dtype == "auto" || kv_cache_dtype.empty() || kv_cache_dtype == "model") ? element_bytes(dtype) : element_bytes(kv_cache_dtype);
+    // Four-bit pages give way to the compute type where a cache cannot have them (runtime/kv_cache.py holds the same conditions).
+    const bool named = kv_cache_dtype == "nvfp4" || kv_cache_dtype == "NVFP4";
+    const bool four = named && run_kv_elements.empty() && num_kv_shared_layers == 0 && draft_type.empty() && dtype != "float32" &&
+                      (head_dim == 64 || head_dim == 128 || head_dim == 256) && kv_page_size >= 16 && (kv_page_size & (kv_page_size - 1)) == 0;
+    const int eb = (named || kv_cache_dtype == "auto" || kv_cache_dtype.empty() || kv_cache_dtype == "model") ? element_bytes(dtype) : element_bytes(kv_cache_dtype);
     if (!run_kv_elements.empty()) {
         long long n = 0;
         for (const long long e : run_kv_elements) n += e;
@@ -326,8 +330,7 @@ long long LLMEngineConfig::kv_bytes_per_token() const {
     }
     const int kvh = std::max(1, num_kv_heads / std::max(1, world_size));
     const long long elements = 2LL * num_attention_layers() * kvh * head_dim;
-    if (kv_cache_dtype == "nvfp4" || kv_cache_dtype == "NVFP4") return elements * 9 / 16;       // codes of four bits, an E4M3 scale per 16
-    return elements * eb;
+    return four ? elements * 9 / 16 : elements * eb;            // codes of four bits, an E4M3 scale per 16
 }
 
 long long LLMEngineConfig::kv_pool_bytes() const {
