@@ -133,12 +133,17 @@ def test_steps_of_other_types_and_sizes_are_refused():
             ops.rope_kv_write_fp4(qkv, lg, replace(m, **bad), cs, 4, 2, 64, sg)
 
 
-def test_commit_path_still_moves_rows_of_bytes():
+@pytest.mark.parametrize("width", [64, 128, 256])
+def test_commit_path_still_moves_rows_of_bytes(width):
     g = torch.Generator().manual_seed(2)
-    pool = torch.randint(0, 256, (2, 6, 2, 3, 16, 64), generator=g, dtype=torch.uint8)
+    pool = torch.randint(0, 256, (2, 6, 2, 3, 16, width), generator=g, dtype=torch.uint8)
     table, past = torch.tensor([[4, 1, 0], [2, 5, -1]], dtype=torch.int32), torch.tensor([14, 3])
     path, plen = torch.tensor([[0, 2, 5, 6], [0, 1, 4, 0]]), torch.tensor([4, 3])
     got = pool.cuda()
+    if width == 64:                 # 32 elements of 16 bits: never had a kernel
+        with pytest.raises(RuntimeError, match="head_dim"):
+            ops.kv_commit_path(got, table.cuda(), past.int().cuda(), path.int().cuda(), plen.int().cuda())
+        return
     ops.kv_commit_path(got, table.cuda(), past.int().cuda(), path.int().cuda(), plen.int().cuda())
     ops.kv_commit_path(pool, table, past, path, plen)
     assert torch.equal(got.cpu(), pool)
