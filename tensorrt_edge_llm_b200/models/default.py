@@ -102,12 +102,14 @@ class Attention(nn.Module):
 
     def _forward_fp4(self, qkv, meta, kv_layer, cos_sin):
         """Four-bit pages: rows are quantised as they are written.  Steps of few rows read the pages in place; the others attend over 16-bit
-        pages of the step's sequences, which hold the cached rows expanded and the step's own as they were rounded."""
+        pages of the step's sequences: codes times block scales, exact, with the layer's two factors in 32 bits where the prompt kernel takes them, else the
+        cached rows expanded and rounded, and the step's own as the write rounds them."""
         heads = (self.num_q_heads, self.num_kv_heads, self.head_dim, self.kv_scales, None if self.q_norm is None else self.q_norm.weight,
                  None if self.k_norm is None else self.k_norm.weight, self.eps)
         group = self.num_q_heads // self.num_kv_heads
         weights = meta.kv_weights[self.layer_idx] if meta.kv_weights is not None and ops.fp4_weighed(meta, group) else None
-        if weights is not None or ops.fp4_direct(meta, group):
+        shape = (self.num_q_heads, self.head_dim)
+        if weights is not None or ops.fp4_direct(meta, group) or ops.fp4_exact(meta, shape, self.num_kv_heads, self.sliding_window or 0, self.attention_sink_bias):
             q = ops.rope_kv_write_fp4(qkv, kv_layer, meta, cos_sin, *heads)
             return ops.paged_attention_fp4(q, kv_layer, meta, self.scale, self.kv_scales, sliding_window=self.sliding_window, sinks=self.attention_sink_bias,
                                            weights=weights)

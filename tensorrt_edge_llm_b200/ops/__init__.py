@@ -415,6 +415,12 @@ def fp4_weighed(meta, group):
     return meta.tree_mask is None and meta.max_q_len * group <= FP4_WEIGHT_COLUMNS
 
 
+def fp4_exact(meta, q_shape, hkv, window=0, sinks=None):
+    """Whether the prompt kernel that an expanded step takes has a form that multiplies by ``scales`` in 32 bits at the same cost, as
+    :func:`paged_attention_fp4` has it; else rows that were multiplied before they were rounded to 16 bits (:func:`kv_fp4_stage`) are quicker."""
+    return not meta.q_start.is_cuda or cuda_ops().fp4_exact(meta, q_shape, hkv, window, sinks)
+
+
 def kv_fp4_stage(kv_layer, meta, scales, dtype, window=0, new_rows=False):
     """16-bit copies of the rows that the step's sequences have in a four-bit layer, for the prompt kernels: ``(stage, meta)`` with the pages
     ``[*, 2, Hkv, 64, D]`` and the step over their own page table.  They take ``4 Hkv D`` bytes a row of all sequences, rounded up to 128 rows each; of steps

@@ -762,6 +762,17 @@ def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int
     return stage, dataclasses.replace(meta, page_table=table, page_size=64), holes
 
 
+def fp4_exact(meta: StepMeta, q_shape: tuple, hkv: int, window: int = 0, sinks=None) -> bool:
+    """See :func:`ops.fp4_exact`.  The two-tile kernel and the one with extras take factors at no cost, the plain one-tile kernel has no form with them.
+    Write, expansion and attention of a layer, 16-bit rows : factors (us): heads of 128, 8129 rows of one prompt 526 : 533, 8 prompts of 1024 164 : 170, 983 rows
+    behind 7000 144 : 144, heads of 256, 4096 rows 241 : 243; one-tile steps, 8 prompts of 200 37 : 50, heads of 64, 8 prompts of 1024 95 : 128."""
+    hq, d = q_shape[-2:]
+    group = hq // hkv
+    if d == 256 or sinks is not None or meta.skip_thr is not None or 128 % group:
+        return True
+    return d == 128 and _two_tile_pays(meta, hkv, group, window)
+
+
 def _fp4_commit_path(pool, page_table, past_len, path, path_len) -> None:
     """:func:`kv_commit_path` of four-bit pages, whose rows lie in two parts of a page."""
     layers, pages, _, hkv, psz, row = pool.shape

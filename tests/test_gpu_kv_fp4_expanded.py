@@ -133,6 +133,40 @@ def test_steps_of_other_types_and_sizes_are_refused():
             ops.rope_kv_write_fp4(qkv, lg, replace(m, **bad), cs, 4, 2, 64, sg)
 
 
+# rows, cached rows, query heads, KV heads, head size, whether the prompt kernel takes the factors
+PROMPTS = [(700, 0, 8, 2, 128, True), (300, 900, 8, 2, 128, True), (200, 300, 4, 2, 256, True), (60, 100, 8, 2, 64, False), (70, 0, 8, 2, 128, True), (100, 200, 8, 2, 128, False)]
+
+
+@pytest.mark.parametrize("rows,past,hq,hkv,d,factors", PROMPTS)
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_prompt_steps_of_a_model_are_as_exact_as_the_operator(rows, past, hq, hkv, d, factors, dtype):
+    """Scales that are no powers of two, and peaked scores: half a step of the result and of the probabilities (2^-8 or 2^-11, a third of its square on average: 0.8 of it
+    for both), while keys rounded to 16 bits would move scores of |q| |k| some 16 by as many half steps."""
+    from tensorrt_edge_llm_b200.config import tiny_llama_config
+    from tensorrt_edge_llm_b200.models.default import Attention
+    cfg = tiny_llama_config(num_hidden_layers=1, vocab_size=64, dtype=dtype, head_dim=d, num_attention_heads=hq, num_key_value_heads=hkv, hidden_size=128)
+    layer = Attention(cfg, 0, "a").cuda()
+    meta, pool, scales, g = make_step([rows], [past], 64, hkv, d, seed=rows)
+    layer.kv_scales.copy_(scales)
+    t = layer.kv_scales.dtype
+    qkv = torch.randn(rows, (hq + 2 * hkv) * d, generator=g)
+    qkv[:, :hq * d] *= 6.0
+    qkv = qkv.to(getattr(torch, dtype)).cuda()
+    cs = torch.cat([torch.ones(rows + past, d // 2), torch.zeros(rows + past, d // 2)], 1).cuda()
+    m, lg = meta.to("cuda"), pool.cuda()
+    assert t == torch.float32 and ops.fp4_exact(m, (hq, d), hkv) == factors and not ops.fp4_direct(m, hq // hkv)
+    got = layer._forward_fp4(qkv, m, lg, cs).reshape(rows, hq, d)
+    q = ops.rope_kv_write_fp4(qkv, lg, m, cs, hq, hkv, d, layer.kv_scales)
+    want, top, kq = oracle(q.cpu(), lg.cpu(), meta, d ** -0.5, scales)
+    err = float((got.cpu().double() - want).norm() / want.norm())
+    half = torch.finfo(got.dtype).eps / 2
+    if factors:
+        assert torch.equal(got, ops.paged_attention_fp4(q, lg, m, d ** -0.5, layer.kv_scales))
+        assert ((got.cpu().double() - want).abs() <= bound(want, top, kq, got.dtype)).all() and err < half
+    else:
+        assert err < 16 * half
+
+
 @pytest.mark.parametrize("width", [64, 128, 256])
 def test_commit_path_still_moves_rows_of_bytes(width):
     g = torch.Generator().manual_seed(2)
