@@ -173,11 +173,11 @@ struct ValueTile {
             else s[i] = *reinterpret_cast<const uint16_t*>(f + 2 * g);
         }
     }
-    // Keys before `from` and from `live` on, which no row sees: what lies there may be anything, NaN scales too (a zero scale takes them out).
-    __device__ __forceinline__ void clear(int t, int from, int live) {
+    // Keys but the `span` ones from `from` on, which no row sees: what lies there may be anything, NaN scales too (a zero scale takes them out).
+    __device__ __forceinline__ void clear(int t, int from, int span) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (place(i, t) < from || place(i, t) >= live) s[i] = 0;
+            if ((unsigned)(place(i, t) - from) >= (unsigned)span) s[i] = 0;
     }
     template <int NT>
     __device__ __forceinline__ void add(const uint32_t (&pb)[NT][2], float (&o)[NT][D / 16][4]) const {
@@ -512,7 +512,7 @@ __device__ __forceinline__ void fp4_keys(const Fp4AttnParams& p, int seq, int kv
             }
             ValueTile<D> vt;
             vt.load(st + Ring::kCodes + m * (16 * D / 2), st + 2 * Ring::kCodes + Ring::kScales + m * D, g, t);
-            if constexpr (!decltype(open)::value) vt.clear(t, begin - kb - 16 * m, (missing >> m) & 1u ? 0 : end - kb - 16 * m);
+            if constexpr (!decltype(open)::value) vt.clear(t, begin - kb - 16 * m, (missing >> m) & 1u ? 0 : end - begin);
             vt.template add<NT>(pb, o);
         }
     };
