@@ -81,7 +81,7 @@ __device__ __forceinline__ float load_query(const T* src, bool real, uint32_t (&
             b[j][1] = *reinterpret_cast<const uint32_t*>(x + 4 * j + 2);
         }
     } else {
-        // bf16 queries enter as fp16, divided by the power of two below their column's largest: exact for all that is above 2^-25 of it
+        // bf16 queries enter as fp16, divided by the power of two below their column's largest: exact down to 2^-17 of it, off by 2^-25 of it at most below
         uint32_t m = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) m = max(m, __float_as_uint(Cvt<T>::to_f(x[i])) & 0x7fffffffu);
