@@ -556,6 +556,8 @@ class LLM:
         for s, p in zip(seats, ids):
             if len(p) > self.max_input_len:
                 raise ValueError(f"prompt of {len(p)} tokens exceeds max_input_len {self.max_input_len}")
+            if self.runner.positions_short(len(p), sp.max_tokens - 1):
+                raise ValueError(f"{len(p)} tokens and {sp.max_tokens - 1} more exceed the model's {self.cfg.max_position_embeddings} positions")
             self.kv.reserve(s, self.runner.rows_to_reserve(len(p), sp.max_tokens))
         t0 = time.perf_counter()
         if isinstance(ids, torch.Tensor):

@@ -107,6 +107,11 @@ class ModelRunner:
         two cuts; each cut gives back what the next growth takes."""
         return max(prompt, min(prompt + new, self.kv_budget + self.BUDGET_SLACK + 1)) if self.kv_budget else prompt + new
 
+    def positions_short(self, prompt: int, new: int) -> bool:
+        """Whether a sequence that drops rows under the budget would run out of positions within ``new`` more tokens."""
+        total = prompt + new
+        return bool(self.kv_budget) and total > self.kv_budget + self.BUDGET_SLACK and total > self.model.cfg.max_position_embeddings
+
     def trim(self, seats: Sequence[int], slack: int = BUDGET_SLACK) -> None:
         """Cut sequences that have outgrown the budget back to it."""
         if not self.kv_budget:

@@ -99,3 +99,16 @@ def test_several_tokens_at_once_stay_within_what_a_sequence_may_grow_to():
     assert r.kv.lengths[0] > 120                    # nine more rows would not fit its 128
     r.step([0], [[5, 6, 7, 8, 9, 10, 11, 12, 13]])
     assert r.kv.lengths[0] == 63 + 9 and r.kv.lengths[0] + r.dropped[0] == total + 9
+
+
+def test_a_generation_that_would_run_out_of_positions_is_refused_before_it_starts():
+    """A sequence that drops rows goes on behind all its tokens: 512 positions here."""
+    llm = LLM(_cfg(), device="cpu", max_batch_size=1, max_input_len=512, max_kv_cache_capacity=512, page_size=16, kv_cache_dtype="nvfp4", random_init_seed=0, kv_budget=48)
+    for sp in (dict(), dict(temperature=0.9, seed=1)):
+        assert len(llm.generate(_prompts(480), SamplingParams(max_tokens=33, ignore_eos=True, **sp))[0].token_ids) == 33
+        step, runs = llm.runner.step, []
+        llm.runner.step = lambda *a, **k: runs.append(1) or step(*a, **k)
+        with pytest.raises(ValueError, match="positions"):
+            llm.generate(_prompts(480), SamplingParams(max_tokens=34, ignore_eos=True, **sp))
+        llm.runner.step = step
+        assert not runs
