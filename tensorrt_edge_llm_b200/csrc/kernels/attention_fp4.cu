@@ -12,7 +12,7 @@
 // instructions a word of eight codes), block scales and products; the pages' bytes would take a third to a half of the time.  So tiles that every
 // column sees whole have code without masks, and a ring of asynchronous copies per warp keeps three tiles on their way.  Measured with heads of 128:
 // 64 sequences of 1088 keys, 32 / 8 heads, 26.0 us (3.0 TB/s, 0.46 of the copy rate; 16-bit pages 55, E4M3 pages 35); 30 of up to 4000 38.9 us; one of 131000,
-// 32 / 4 heads, 34 us; one of 700 7.5 us, which is latency: launch, page table, first tile, join.  Taken back: bulk copies with mbarriers in place of the
+// 32 / 4 heads, 34 us; one of 700 8.2 us, which is latency: launch, page table, first tile, join.  Taken back: bulk copies with mbarriers in place of the
 // lanes' copies; 32 columns a warp (half the occupancy); operands expanded once for all warps of a CTA, in shared memory (half the instructions, but two
 // barriers for every 128 keys: 2 sequences of 4000 keys, 128 columns, 49 us against 50, one of 8000, 64 columns, 28 against 24).
 #include <type_traits>

@@ -207,7 +207,8 @@ __global__ void __launch_bounds__(128, 6) rope_kv_write_fp4_kernel(const Fp4Writ
     }
 }
 
-// A part of a head turns: one warp per (token, head); a lane holds E neighbouring features.
+// A part of a head turns: one warp per (token, head); a lane holds E neighbouring features, with true divisions and 64-bit roots for every head.  Rows of 32 / 8 heads
+// of 128, half of each turning: 64 rows 3.9 us, 500 10.9, 8129 132 (whole heads 3.5, 6.8, 47): bound by that arithmetic, 2.8 times the form above.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) rope_part_kv_write_fp4_kernel(const Fp4WriteParams p) {
     pdl_prologue();
@@ -408,7 +409,8 @@ __global__ void __launch_bounds__(256) kv_fp4_stage_kernel(const uint8_t* __rest
 }
 
 // Rows of accepted draft tokens move together: the row at slot past + path[j] to past + j, j from 1, of every layer, plane and head.  All words of a row
-// (codes, then block scales) are read before any is written.
+// (codes, then block scales) are read before any is written.  Four rows of 8 heads of 128 in 36 layers: 8 sequences 12.9 us, 64 90 us (latency of a block's
+// look-ups, page table and path, in several waves of blocks).
 constexpr int kCommitWords = 12;                                // of a thread
 template <int D>
 __global__ void __launch_bounds__(256) kv_fp4_commit_path_kernel(uint8_t* __restrict__ pool, const int* __restrict__ page_table, const int* __restrict__ past_len,
