@@ -161,17 +161,17 @@ static int launch_combine_back(const float* ws_o, const float* ws_lse, void* out
     return 0;
 }
 
-template <int D, typename T, int KVS, int MINB>
+template <int D, typename T, int KVS, int MINB, bool kHoles>
 static int launch_attn_extra(const CUtensorMap& tq, const CUtensorMap& tkv, const AttnParams& p, int qtiles, int nseq, cudaStream_t stream) {
     constexpr int smem = 128 * D * 2 + 2 * KVS * kKvTile * D * 2 + 2 * 128 * kKvTile * 2 + 1024 + 512;
     static bool configured = false;
     if (!configured) {
-        cudaError_t e = cudaFuncSetAttribute(attn_tc5_extra_kernel<D, T, KVS, MINB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t e = cudaFuncSetAttribute(attn_tc5_extra_kernel<D, T, KVS, MINB, kHoles>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return fail("cudaFuncSetAttribute(attn_tc5_extra)", e);
         configured = true;
     }
     dim3 grid(qtiles, p.hkv, nseq * p.splits);
-    TELB_LAUNCH("attn_tc5_extra_kernel", (attn_tc5_extra_kernel<D, T, KVS, MINB>), dim3(grid), dim3(kAttnThreads), smem, stream, tq, tkv, p);
+    TELB_LAUNCH("attn_tc5_extra_kernel", (attn_tc5_extra_kernel<D, T, KVS, MINB, kHoles>), dim3(grid), dim3(kAttnThreads), smem, stream, tq, tkv, p);
     TELB_CHECK_LAUNCH("attn_tc5_extra_kernel");
     if (p.splits > 1 && p.back)
         return launch_combine_back<D, T>(p.ws_o, p.ws_lse, p.out, p.total_tokens, p.hq, p.splits, p.back, p.back_mult, p.positions, p.ld_out, stream);
@@ -187,8 +187,10 @@ template <int D, typename T>
 static int launch_attn(const CUtensorMap& tq, const CUtensorMap& tkv, const AttnParams& p, int qtiles, int nseq, cudaStream_t stream) {
     // 256-wide heads (Gemma family): the Q tile alone is 64 KB and O takes 256 TMEM columns, so one CTA per SM with
     // single-stage K / V rings is the only shape that fits; narrower heads run two CTAs per SM
-    if constexpr (D > 128) return launch_attn_extra<D, T, 1, 1>(tq, tkv, p, qtiles, nseq, stream);
-    return launch_attn_extra<D, T, 1, 2>(tq, tkv, p, qtiles, nseq, stream);
+    constexpr int kCtas = D > 128 ? 1 : 2;
+    // hidden keys are a kernel of their own: heads of 256 took 2 % longer with them (4096 rows of 8 heads, 217 and 221 us)
+    if (p.kv_holes) return launch_attn_extra<D, T, 1, kCtas, true>(tq, tkv, p, qtiles, nseq, stream);
+    return launch_attn_extra<D, T, 1, kCtas, false>(tq, tkv, p, qtiles, nseq, stream);
 }
 
 }  // namespace telb
