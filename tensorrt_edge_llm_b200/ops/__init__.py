@@ -416,8 +416,8 @@ def fp4_weighed(meta, group):
 
 
 def fp4_exact(meta, q_shape, hkv, window=0, sinks=None):
-    """Whether the prompt kernel that an expanded step takes has a form that multiplies by ``scales`` in 32 bits at the same cost, as
-    :func:`paged_attention_fp4` has it; else rows that were multiplied before they were rounded to 16 bits (:func:`kv_fp4_stage`) are quicker."""
+    """Whether the prompt kernel that an expanded step takes has a form that multiplies by ``scales`` in 32 bits, as
+    :func:`paged_attention_fp4` has it, at a few per cent more for a layer's attention; else rows that were multiplied before they were rounded to 16 bits (:func:`kv_fp4_stage`) are quicker."""
     return not meta.q_start.is_cuda or cuda_ops().fp4_exact(meta, q_shape, hkv, window, sinks)
 
 

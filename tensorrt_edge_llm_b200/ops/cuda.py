@@ -763,9 +763,10 @@ def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int
 
 
 def fp4_exact(meta: StepMeta, q_shape: tuple, hkv: int, window: int = 0, sinks=None) -> bool:
-    """See :func:`ops.fp4_exact`.  The two-tile kernel and the one with extras take factors at no cost, the plain one-tile kernel has no form with them.
-    Write, expansion and attention of a layer, 16-bit rows : factors (us): heads of 128, 8129 rows of one prompt 526 : 533, 8 prompts of 1024 164 : 170, 983 rows
-    behind 7000 144 : 144, heads of 256, 4096 rows 241 : 243; one-tile steps, 8 prompts of 200 37 : 50, heads of 64, 8 prompts of 1024 95 : 128."""
+    """See :func:`ops.fp4_exact`.  The two-tile kernel and the one with extras take factors and are as quick with them, the plain one-tile kernel has no such form.
+    Write, expansion (of the step's own rows too) and attention of a layer, 16-bit rows : factors (us): heads of 128, 8129 rows of one prompt 510 : 515, 8 prompts of
+    1024 164 : 171, 983 rows behind 7000 144 : 145, heads of 256, 4096 rows 239 : 245, under a window of 512 81 : 86; one-tile steps, 8 prompts of 200 38 : 50, heads of
+    64, 8 prompts of 1024 95 : 129."""
     hq, d = q_shape[-2:]
     group = hq // hkv
     if d == 256 or sinks is not None or meta.skip_thr is not None or 128 % group:
