@@ -752,7 +752,8 @@ def _fp4_stage(kv_layer, meta: StepMeta, scales, dtype: torch.dtype, window: int
     """Without ``scales``: codes times block scales, which both 16-bit types hold exactly.  A third result tells the prompt kernels which rows the cache
     does not have: a byte per page, a bit per 16 rows."""
     n, dev = meta.num_seqs, kv_layer.get_device()
-    per, total, packed = ref_ops.fp4_stage_pages(meta)
+    # a step that is being captured may be run again with other lengths
+    per, total, packed = ref_ops.fp4_stage_pages(meta, known=not torch.cuda.is_current_stream_capturing())
     page_table, width = _fp4_step(meta, (meta.q_len, meta.past_len))
     stage = torch.empty(total, 2, hkv, 64, d, dtype=dtype, device=kv_layer.device)
     table, holes = torch.empty(n, per, dtype=torch.int32, device=kv_layer.device), torch.empty(n, per, dtype=torch.uint8, device=kv_layer.device)

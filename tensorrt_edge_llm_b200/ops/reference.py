@@ -1447,12 +1447,12 @@ def rope_kv_write_fp4(qkv, kv_layer, meta: StepMeta, cos_sin, num_q_heads, num_k
     return q
 
 
-def fp4_stage_pages(meta: StepMeta) -> Tuple[int, int, bool]:
+def fp4_stage_pages(meta: StepMeta, known: bool = True) -> Tuple[int, int, bool]:
     """Size of the 16-bit copy of a step's sequences in pages of 64 rows: ``(columns of its table, pages, whether they are packed)``.  A sequence takes whole
-    128-key tiles: as many as the longest, or, where the host knows that some are shorter, its own, one sequence behind the other, and a page of zeros for
+    128-key tiles: as many as the longest, or, where the host knows that some are shorter (``known``: its lengths hold), its own, one sequence behind the other, and a page of zeros for
     what the table has behind them."""
     per = 2 * max(1, (meta.max_seq_len + 127) // 128)
-    if meta.host_lens is None:
+    if meta.host_lens is None or not known:
         return per, meta.num_seqs * per, False
     total = sum([min(2 * max(1, (q + past + 127) // 128), per) for q, past in meta.host_lens])
     return (per, total + 1, True) if total < meta.num_seqs * per else (per, total, False)

@@ -181,3 +181,30 @@ def test_commit_path_still_moves_rows_of_bytes(width):
     ops.kv_commit_path(got, table.cuda(), past.int().cuda(), path.int().cuda(), plen.int().cuda())
     ops.kv_commit_path(pool, table, past, path, plen)
     assert torch.equal(got.cpu(), pool)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_captured_step_is_run_again_with_other_lengths(d):
+    """The graph was captured with the lengths of one step; its tensors hold those of another by the time it runs."""
+    hq, hkv, page = 8, 2, 64
+    first, layer, scales, g = make_step([70, 40, 60], [0, 10, 5], page, hkv, d, seed=1)
+    second, layer2, _, _ = make_step([70, 40, 60], [300, 0, 700], page, hkv, d, seed=2)
+    m, lg, sg = first.to("cuda"), layer2.cuda(), scales.cuda()
+    m.max_seq_len = 900
+    m.page_table = torch.full(second.page_table.shape, -1, dtype=torch.int32, device="cuda")
+    m.page_table[:, :first.page_table.shape[1]] = first.page_table.cuda()
+    q = (torch.randn(170, hq, d, generator=g) * 2).bfloat16().cuda()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        ops.paged_attention_fp4(q, lg, m, d ** -0.5, sg)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.paged_attention_fp4(q, lg, m, d ** -0.5, sg)
+    m.past_len.copy_(second.past_len)
+    m.page_table.copy_(second.page_table)
+    for _ in range(2):
+        graph.replay()
+    want, top, kq = oracle(q.cpu(), layer2, second, d ** -0.5, scales)
+    assert ((out.cpu().double() - want).abs() <= bound(want, top, kq, torch.bfloat16)).all()
